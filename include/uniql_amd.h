@@ -369,6 +369,110 @@ int uniql_fwht_composite(const void* x, void* y, int64_t rows, int dim, int base
  */
 int uniql_fwht_columns(const void* x, void* y, int rows, int cols, float scale, int dtype, void* stream);
 
+/*
+ * ---- attention: a paged key / value cache held in 4 bits, attention over it and over whole prompts -------------------
+ * The reference keeps fp16 keys and values of transformers' cache classes and calls torch's or flash_attn's attention
+ * (modeling/llama/llama_qblocks.py:104-150); these calls are this library's own and stand between the rotary kernel and
+ * the output projection.  fp16 throughout, head widths 1 to 128, query heads a multiple of the key / value heads (query
+ * head h uses key / value head h / (n_q_heads / n_kv_heads)).
+ *
+ * The cache is a pool of `pages` pages of `page_size` tokens (16, 32, 64, 128 or 256).  Place `slot` = page * page_size +
+ * offset holds one token's vectors, one per key / value head, each as s (c - 8) with
+ *   s = fp16(max|x| 2/15),  c = clamp(round(x / s) + 8, 0, 15)   (round to even; c = 8 where s is 0);
+ * a vector that holds an infinity or a NaN reads back as NaN throughout.
+ *   k_codes   device, int32 [pages, heads, page_size, kw], kw = 4 ceil(k_dim / 32): eight codes a word in nibble order
+ *             [0, 2, 4, 6, 1, 3, 5, 7]; codes from k_dim on are 8
+ *   v_codes   device, int32 [pages, heads, page_size / 4, vw, 4], vw = 4 ceil(v_dim / 32): the words of four tokens side by side
+ *   k_scales, v_scales   device, fp16 [pages, heads, page_size]
+ *   all 16-byte aligned
+ */
+typedef struct uniql_kv4_cache {
+    void *k_codes, *k_scales, *v_codes, *v_scales;
+    int pages, page_size, heads, k_dim, v_dim;
+} uniql_kv4_cache;
+
+/*
+ * Gives pages to requests and places to their new tokens, from lengths that are on the device: nothing is read back, so the
+ * call can be recorded into a graph.  No counterpart in the reference.
+ *   new_tokens   device, int32 [rows]: tokens that each request gets in this step; negative: the request ends
+ *   lengths      device, int32 [rows]: tokens that each has so far
+ *   table        device, int32 [rows, columns]: the pages of each; entry p of a row belongs to its positions
+ *                p page_size ..; modified (entries behind a request's last page are not meaningful)
+ *   free_pages   device, int32 [pool]: a stack of *free_count free pages; modified
+ *   lengths_out, free_count_out   device: lengths and count after the step; may be `lengths` and `free_count` themselves
+ * First the pages of ending requests go on top of the stack, in the order of the rows and of their pages; their lengths
+ * become 0.  Then the others take ceil((length + new) / page_size) - ceil(length / page_size) pages from the top, in the
+ * order of the rows.  A request is refused, and changes nothing, when it would have more tokens than its row has room for, when
+ * the new tokens up to and with its own exceed max_tokens, or when it needs pages and those asked for up to and with its own are more
+ * than there are (none overtakes it: a later one that needs pages is refused too).
+ *   cu           device out, int32 [rows + 1]: token t of the batch belongs to request r with cu[r] <= t < cu[r + 1];
+ *                refused requests' tokens count, everything is cut off at max_tokens
+ *   slots        device out, int64 [max_tokens]: each token's place; -1 for tokens of refused requests and behind the last
+ *   positions    device out, int32 [max_tokens]: each token's position in its request; 0 where slots is -1
+ *   refused      device out, int32 [rows]: 1 where a request with new tokens was refused
+ * columns <= 2^20, columns * page_size < 2^31, rows * columns < 2^31, max_tokens <= 2^30.  Nothing outside these arrays is touched
+ * whatever they hold; lengths below 0 count as 0 where a request ends and are refused otherwise.
+ */
+int uniql_kv_assign_pages(const int32_t* new_tokens, const int32_t* lengths, int32_t* table, int32_t* free_pages,
+                          const int32_t* free_count, int32_t* lengths_out, int32_t* free_count_out,
+                          int64_t* slots, int32_t* positions, int32_t* cu, int32_t* refused,
+                          int rows, int columns, int pool, int page_size, int max_tokens, void* stream);
+
+/*
+ * Writes the keys and values of `tokens` tokens to their places.
+ *   k, v    device, fp16 [tokens, heads, k_dim] and [tokens, heads, v_dim], unit stride along the last axis, k_row / v_row and
+ *           k_head / v_head elements between tokens and heads (ranges of the fused projection's output are read where they are)
+ *   slots   device, int64 [tokens]; places outside the pool (-1) are left out.  A place must not occur twice
+ */
+int uniql_kv4_store(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head,
+                    const int64_t* slots, const uniql_kv4_cache* cache, int tokens, void* stream);
+
+/*
+ * Reads positions back as fp16_rn(s (c - 8)): row t of the outputs is position starts[r] + t - cu[r] of the request r with
+ * cu[r] <= t < cu[r + 1].  Rows in front of cu[0] and from cu[requests] on are left as they were; positions without a page in the
+ * pool give NaN.
+ *   table    device, int32 [requests, columns];  cu  device, int32 [requests + 1];  starts  device, int32 [requests], or NULL: 0
+ *   k, v     device out, fp16 [rows, heads, k_dim] and [rows, heads, v_dim], strides as above
+ */
+int uniql_kv4_load(const uniql_kv4_cache* cache, const int32_t* table, const int32_t* cu, const int32_t* starts,
+                   void* k, int64_t k_row, int64_t k_head, void* v, int64_t v_row, int64_t v_head,
+                   int requests, int columns, int rows, void* stream);
+
+/*
+ * Attention of each request's newest tokens over its pages: out = softmax(scale q k^T) v with the cache's keys and values.
+ *   q        device, fp16 [rows, n_q_heads, k_dim], unit stride along the last axis, q_row and q_head elements between rows and heads
+ *   table    device, int32 [requests, columns];  lengths  device, int32 [requests]: tokens in the cache, the new ones among them
+ *   cu_q     device, int32 [requests + 1]: the rows of each request; NULL: one row each (rows == requests)
+ *   out      device out, fp16 [rows, n_q_heads, v_dim], strides likewise
+ * Row i of a request with t rows sees the positions 0 .. length - t + i.  A row that sees none is 0; rows in front of cu_q[0] and
+ * from cu_q[requests] on are left as they were.  What lies in the pages behind a request's length does not matter; a page number
+ * outside the pool within it makes the rows that see it NaN.
+ *   accum, temp   as for uniql_w4a16_gemm: accum all zero on entry and on exit, temp of any contents, neither shared by calls that may
+ *                 run at the same time; sizes from uniql_kv4_attention_workspace (bounds that follow from the arguments alone)
+ */
+int uniql_kv4_attention_workspace(const uniql_kv4_cache* cache, int rows, int requests, int columns, int n_q_heads,
+                                  size_t* accum_bytes, size_t* temp_bytes);
+int uniql_kv4_attention(const void* q, int64_t q_row, int64_t q_head, const uniql_kv4_cache* cache,
+                        const int32_t* table, const int32_t* lengths, const int32_t* cu_q,
+                        void* out, int64_t out_row, int64_t out_head,
+                        void* accum, size_t accum_bytes, void* temp, size_t temp_bytes,
+                        int rows, int requests, int columns, int n_q_heads, float scale, void* stream);
+
+/*
+ * Attention over the prompts of several sequences that lie behind each other: out = softmax(scale q k^T) v within each.
+ *   q        device, fp16 [rows, n_q_heads, k_dim];  k, v  device, fp16 [k_rows, n_kv_heads, k_dim] and [.., v_dim]; unit stride
+ *            along the last axis, *_row and *_head elements between rows and heads
+ *   cu_q, cu_k   device, int32 [sequences + 1]: the rows of each sequence in q and in k and v (ascending; cu_k may be cu_q)
+ *   out      device out, fp16 [rows, n_q_heads, v_dim], strides likewise; must not overlap q, k or v
+ * With `causal`, row i of a sequence with t rows and n keys sees the keys 0 .. i + n - t, all of them otherwise.  A row that sees
+ * none is 0; rows in front of cu_q[0] and from cu_q[sequences] on are left as they were.  Other sequences' keys and values do
+ * not matter, whatever they hold.
+ */
+int uniql_prompt_attention(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                           const void* v, int64_t v_row, int64_t v_head, const int32_t* cu_q, const int32_t* cu_k,
+                           void* out, int64_t out_row, int64_t out_head, int rows, int k_rows, int sequences,
+                           int n_q_heads, int n_kv_heads, int k_dim, int v_dim, int causal, float scale, void* stream);
+
 
 #ifdef __cplusplus
 }

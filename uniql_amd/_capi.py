@@ -62,6 +62,19 @@ SIGNATURES = {
     "uniql_fwht": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_float, c_int, c_void_p]),
     "uniql_fwht_composite": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_float, c_int, c_void_p]),
     "uniql_fwht_columns": (c_int, [c_void_p, c_void_p, c_int, c_int, c_float, c_int, c_void_p]),
+    "uniql_kv_assign_pages": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "uniql_kv4_store": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p]),
+    "uniql_kv4_load": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                               c_int, c_int, c_int, c_void_p]),
+    "uniql_kv4_attention_workspace": (c_int, [c_void_p, c_int, c_int, c_int, c_int,
+                                              ctypes.POINTER(c_size_t), ctypes.POINTER(c_size_t)]),
+    "uniql_kv4_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_int64, c_int64, c_void_p, c_size_t, c_void_p, c_size_t,
+                                    c_int, c_int, c_int, c_int, c_float, c_void_p]),
+    "uniql_prompt_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                       c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int,
+                                       c_int, c_int, c_int, c_int, c_int, c_float, c_void_p]),
 }
 
 _lib = None
@@ -119,6 +132,9 @@ def host():
             spec = util.spec_from_file_location("uniql_amd._host", HOST_PATH)
             module = util.module_from_spec(spec)
             spec.loader.exec_module(module)
+            module.bind_attention(*(ctypes.cast(fn, ctypes.c_void_p).value
+                                    for fn in (lib.uniql_kv_assign_pages, lib.uniql_kv4_store, lib.uniql_kv4_load,
+                                               lib.uniql_kv4_attention_workspace, lib.uniql_kv4_attention, lib.uniql_prompt_attention)))
             module.bind(*(ctypes.cast(fn, ctypes.c_void_p).value
                           for fn in (lib.uniql_w4a16_linear, lib.uniql_w4a16_linear_workspace, lib.uniql_w4_embedding_lookup,
                                      lib.uniql_fwht, lib.uniql_fwht_composite, lib.uniql_fwht_columns, lib.uniql_w4a16_quantize,

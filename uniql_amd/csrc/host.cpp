@@ -308,6 +308,8 @@ std::pair<Tensor, Tensor> cut_rows(const Tensor& B, const Tensor& s, int n, int 
     return out;
 }
 
+#include "host_attention.hpp"
+
 }  // namespace
 
 PYBIND11_MODULE(_host, module) {
@@ -338,4 +340,10 @@ PYBIND11_MODULE(_host, module) {
     module.def("quantize", &quantize);
     module.def("cut_columns", &cut_columns);
     module.def("cut_rows", &cut_rows);
+    module.def("bind_attention", &bind_attention);
+    module.def("kv_assign_pages", &kv_assign_pages);
+    module.def("kv4_store", &kv4_store);
+    module.def("kv4_load", &kv4_load);
+    module.def("kv4_attention", &kv4_attention);
+    module.def("prompt_attention", &prompt_attention);
 }

@@ -1,0 +1,319 @@
+// The paged 4-bit key / value cache: which pages a request holds and where its new tokens go (assign), writing keys and
+// values into it (store), reading them back as fp16 (load).
+//
+// A vector x of one token and one key / value head is held as s (c - 8), s = fp16(max|x| 2/15), c = clamp(round(x / s) + 8, 0, 15),
+// the arithmetic of the 4-bit projections with one scale for the vector.  Layout: see KvCache in kv_cache.hpp.
+#include "kv_cache.hpp"
+
+namespace uniql {
+
+// ---- pages and slots ---------------------------------------------------------------------------------------------
+struct AssignArgs {
+    const int32_t *new_tokens, *lengths;
+    int32_t *table, *free_pages;
+    const int32_t* free_count;
+    int32_t *lengths_out, *free_count_out;
+    int64_t* slots;
+    int32_t *positions, *cu, *refused;
+    int rows, columns, pool, page_shift, max_tokens;
+};
+constexpr int kAssignThreads = 1024;
+
+// Sums over the workgroup's threads up to and including each; `total` is the whole sum.
+template <typename T>
+__device__ __forceinline__ T scan_inclusive(T v, T* wave_sums, T& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const T other = __shfl_up(v, d, 64);
+        if (lane >= d) v += other;
+    }
+    __syncthreads();  // the sums of an earlier scan have been read
+    if (lane == 63) wave_sums[wave] = v;
+    __syncthreads();
+    T before = 0;
+    total = 0;
+    for (int w = 0; w < kAssignThreads / 64; ++w) {
+        const T s = wave_sums[w];
+        if (w < wave) before += s;
+        total += s;
+    }
+    return v + before;
+}
+
+// The first of `count` ascending values that is greater than `v`.
+template <typename P>
+__device__ __forceinline__ int first_above(const P* ascending, int count, int v) {
+    int low = 0, high = count;
+    while (low < high) {
+        const int mid = (low + high) >> 1;
+        if (ascending[mid] > v) high = mid;
+        else low = mid + 1;
+    }
+    return low;
+}
+
+// Where token t of the batch goes.  `old`: tokens the request held before, or -1 where it was refused.
+__device__ __forceinline__ void place_token(const AssignArgs& a, int t, int request, int first, int old) {
+    const int position = old < 0 ? 0 : old + (t - first);
+    int64_t slot = -1;
+    if (old >= 0) {
+        const int64_t page = a.table[(int64_t)request * a.columns + (position >> a.page_shift)];
+        slot = (page << a.page_shift) + (position & ((1 << a.page_shift) - 1));
+    }
+    a.slots[t] = slot;
+    a.positions[t] = position;
+}
+
+// One workgroup: releases, then requests in order, both by prefix sums over the rows; pages are moved by a flat loop over pages,
+// each of which finds its row among the sums, so that one request with thousands of pages takes no longer than many with a few.
+// PLACE: it also places the tokens (a small batch: no second launch).
+template <bool PLACE>
+__global__ __launch_bounds__(kAssignThreads) void kv_assign_kernel(const AssignArgs a) {
+    __shared__ int64_t sums64[kAssignThreads / 64];
+    __shared__ int sums[kAssignThreads / 64], upto[kAssignThreads], upto_tokens[kAssignThreads], held_by[kAssignThreads], used;
+    const int tid = threadIdx.x;
+    const int page = 1 << a.page_shift;
+    const int64_t capacity = (int64_t)a.columns << a.page_shift;
+    if (tid == 0) used = 0;
+    int count = *a.free_count;
+    count = count < 0 ? 0 : (count > a.pool ? a.pool : count);
+    for (int base = 0; base < a.rows; base += kAssignThreads) {
+        const int r = base + tid;
+        int pages = 0;
+        if (r < a.rows && a.new_tokens[r] < 0) {
+            int64_t n = a.lengths[r];
+            n = n < 0 ? 0 : (n > capacity ? capacity : n);
+            pages = (int)((n + page - 1) >> a.page_shift);
+        }
+        int total;
+        const int sum = scan_inclusive(pages, sums, total);
+        if (total == 0) continue;  // uniform
+        upto[tid] = sum;
+        held_by[tid] = pages;
+        __syncthreads();
+        for (int i = tid; i < total; i += kAssignThreads) {
+            const int row = first_above(upto, kAssignThreads, i), j = i - (upto[row] - held_by[row]);
+            if (count + i < a.pool) a.free_pages[count + i] = a.table[(int64_t)(base + row) * a.columns + j];
+        }
+        count = total > a.pool - count ? a.pool : count + total;
+    }
+    __syncthreads();  // released pages are on the list
+    int64_t tokens_before = 0;
+    int64_t pages_before = 0;
+    for (int base = 0; base < a.rows; base += kAssignThreads) {
+        const int r = base + tid;
+        const bool exists = r < a.rows;
+        const int asked = exists ? a.new_tokens[r] : 0, n = asked > 0 ? asked : 0;
+        const int64_t old = exists ? a.lengths[r] : 0;
+        int64_t tokens, pages_total;
+        const int64_t sum_tokens = tokens_before + scan_inclusive((int64_t)n, sums64, tokens);
+        const bool fits = n > 0 && old >= 0 && old + n <= capacity && sum_tokens <= a.max_tokens;
+        const int held = (int)((old + page - 1) >> a.page_shift);
+        const int need = fits ? (int)((old + n + page - 1) >> a.page_shift) - held : 0;
+        const int64_t sum_pages = pages_before + scan_inclusive((int64_t)need, sums64, pages_total);
+        const bool served = fits && (need == 0 || sum_pages <= count);
+        if (exists) {
+            a.cu[r + 1] = sum_tokens < a.max_tokens ? (int)sum_tokens : a.max_tokens;
+            a.refused[r] = n > 0 && !served;
+            a.lengths_out[r] = asked < 0 ? 0 : (int)(served ? old + n : old);
+        }
+        // those that are served and need pages come before all that are refused for want of them
+        __syncthreads();
+        const int64_t mine = sum_pages - pages_before;
+        upto[tid] = (int)(mine < 0x7fffffff ? mine : 0x7fffffff);
+        held_by[tid] = (int)(need != 0 ? need : 0) ;
+        if (PLACE) upto_tokens[tid] = exists ? a.cu[r + 1] : a.max_tokens;
+        __shared__ int first_page[kAssignThreads], old_or_none[kAssignThreads];
+        first_page[tid] = held;
+        old_or_none[tid] = served ? (int)old : -1;
+        if (served && need) atomicMax(&used, (int)sum_pages);
+        __syncthreads();
+        const int64_t give64 = (int64_t)used - pages_before;
+        const int give = give64 > 0 ? (int)give64 : 0;
+        for (int i = tid; i < give; i += kAssignThreads) {
+            const int row = first_above(upto, kAssignThreads, i), j = i - (upto[row] - held_by[row]);
+            a.table[(int64_t)(base + row) * a.columns + first_page[row] + j] = a.free_pages[count - 1 - (pages_before + i)];
+        }
+        if (PLACE) {
+            __syncthreads();
+            for (int t = tid; t < a.max_tokens; t += kAssignThreads) {
+                const int row = first_above(upto_tokens, a.rows, t);
+                const bool there = row < a.rows;
+                place_token(a, t, row, there && row > 0 ? upto_tokens[row - 1] : 0, there ? old_or_none[row] : -1);
+            }
+        }
+        tokens_before += tokens;
+        pages_before += pages_total;
+    }
+    if (PLACE && a.rows == 0)
+        for (int t = tid; t < a.max_tokens; t += kAssignThreads) place_token(a, t, 0, 0, -1);
+    __syncthreads();
+    if (tid == 0) {
+        a.cu[0] = 0;
+        *a.free_count_out = count - used;
+    }
+}
+
+// Larger batches: a token a thread, behind the kernel above.
+__global__ __launch_bounds__(256) void kv_place_kernel(const AssignArgs a) {
+    const int t = (int)blockIdx.x * 256 + (int)threadIdx.x;
+    if (t >= a.max_tokens) return;
+    const int request = first_above(a.cu + 1, a.rows, t);
+    const bool served = request < a.rows && a.refused[request] == 0;
+    place_token(a, t, request, served ? a.cu[request] : 0, served ? a.lengths_out[request] - a.new_tokens[request] : -1);
+}
+
+int kv_assign_launch(const int32_t* new_tokens, const int32_t* lengths, int32_t* table, int32_t* free_pages, const int32_t* free_count,
+                     int32_t* lengths_out, int32_t* free_count_out, int64_t* slots, int32_t* positions, int32_t* cu, int32_t* refused,
+                     int rows, int columns, int pool, int page_size, int max_tokens, hipStream_t stream) {
+    const AssignArgs a = {new_tokens, lengths, table, free_pages, free_count, lengths_out, free_count_out, slots, positions, cu, refused,
+                          rows, columns, pool, __builtin_ctz((unsigned)page_size), max_tokens};
+    const bool place = rows <= kAssignThreads && max_tokens <= 4096;
+    if (place) {
+        hipLaunchKernelGGL(kv_assign_kernel<true>, dim3(1), dim3(kAssignThreads), 0, stream, a);
+    } else {
+        hipLaunchKernelGGL(kv_assign_kernel<false>, dim3(1), dim3(kAssignThreads), 0, stream, a);
+        if (max_tokens > 0)
+            hipLaunchKernelGGL(kv_place_kernel, dim3(((unsigned)max_tokens + 255u) / 256u), dim3(256), 0, stream, a);
+    }
+    return hipGetLastError() == hipSuccess ? UNIQL_OK : UNIQL_E_LAUNCH;
+}
+
+// ---- store ---------------------------------------------------------------------------------------------------------
+struct StoreArgs {
+    const half_t *k, *v;
+    int64_t k_row, k_head, v_row, v_head;
+    const int64_t* slots;
+    KvCache cache;
+    int64_t vectors;  // tokens x key / value heads x 2
+};
+
+// Eight values of a vector from column j on; those past the vector's width count as zeros.
+__device__ __forceinline__ h8 load_eight_of(const half_t* x, int j, int width) {
+    if (j + 8 <= width) {
+        const h8u v = *reinterpret_cast<const h8u*>(x + j);
+        return h8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+    }
+    h8 v = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (j + i < width) v[i] = x[j + i];
+    return v;
+}
+
+// Sixteen lanes quantise a vector, eight values each, and store one word of codes each.
+__global__ __launch_bounds__(256) void kv4_store_kernel(const StoreArgs a) {
+    const int64_t vector = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (vector >= a.vectors) return;
+    const int part = threadIdx.x & 15;
+    const int64_t both = vector >> 1;
+    const bool is_v = vector & 1;
+    const int64_t token = both / a.cache.heads;
+    const int head = (int)(both - token * a.cache.heads);
+    const int64_t slot = a.slots[token];
+    if (slot < 0 || slot >= ((int64_t)a.cache.pages << a.cache.page_shift)) return;
+    const int width = is_v ? a.cache.v_dim : a.cache.k_dim, words = is_v ? a.cache.v_words : a.cache.k_words;
+    const half_t* x = is_v ? a.v + token * a.v_row + head * a.v_head : a.k + token * a.k_row + head * a.k_head;
+    const h8 v = load_eight_of(x, part * 8, width);
+    uint32_t top = 0;  // the largest magnitude's bits: they order as the magnitudes do, infinities and NaN above all
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const half_t value = v[i];  // (a bit cast of the element itself takes the vector's first one)
+        const uint32_t bits = __builtin_bit_cast(uint16_t, value) & 0x7fffu;
+        top = bits > top ? bits : top;
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+        const uint32_t other = (uint32_t)__shfl_xor((int)top, d, 64);
+        top = other > top ? other : top;
+    }
+    const bool finite = top < 0x7c00u;
+    // fp16(max 2/15): twice an 11-bit number over 15 stays 2^-16 of itself away from the midpoints between fp16 numbers, so
+    // the products' and the constant's errors in fp32 (2^-23) do not show
+    const half_t scale = finite ? scaled_to_half((float)__builtin_bit_cast(half_t, (uint16_t)top), 2.0f / 15.0f)
+                                : __builtin_bit_cast(half_t, (uint16_t)0x7e00);
+    const float s = (float)scale;
+    const bool usable = finite && s > 0.f;
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // a correctly rounded quotient: x / s that is not a midpoint between whole numbers is 2^-12 away from one
+        const float c = usable ? fminf(fmaxf(rintf((float)v[i] / s), -8.f), 7.f) + 8.f : 8.f;
+        word |= (uint32_t)(int)c << kNibble(i);
+    }
+    if (part < words) {
+        if (is_v) a.cache.v_codes[a.cache.v_word(slot, head, part)] = word;
+        else a.cache.k_codes[a.cache.k_word(slot, head, part)] = word;
+    }
+    if (part == 0) (is_v ? a.cache.v_scales : a.cache.k_scales)[a.cache.scale_at(slot, head)] = scale;
+}
+
+int kv4_store_launch(const void* k, int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const int64_t* slots,
+                     const KvCache& cache, int tokens, hipStream_t stream) {
+    const StoreArgs a = {reinterpret_cast<const half_t*>(k), reinterpret_cast<const half_t*>(v), k_row, k_head, v_row, v_head, slots, cache,
+                         (int64_t)tokens * cache.heads * 2};
+    const int64_t blocks = (a.vectors + 15) / 16;
+    if (blocks > 0x7fffffffLL) return UNIQL_E_SHAPE;
+    hipLaunchKernelGGL(kv4_store_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    return hipGetLastError() == hipSuccess ? UNIQL_OK : UNIQL_E_LAUNCH;
+}
+
+// ---- load ----------------------------------------------------------------------------------------------------------
+struct LoadArgs {
+    KvCache cache;
+    const int32_t *table, *cu, *starts;
+    half_t *k, *v;
+    int64_t k_row, k_head, v_row, v_head, vectors;
+    int requests, columns, rows;
+};
+
+__global__ __launch_bounds__(256) void kv4_load_kernel(const LoadArgs a) {
+    const int64_t vector = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (vector >= a.vectors) return;
+    const int part = threadIdx.x & 15;
+    const int64_t both = vector >> 1;
+    const bool is_v = vector & 1;
+    const int row = (int)(both / a.cache.heads), head = (int)(both - (int64_t)row * a.cache.heads);
+    if (row < a.cu[0]) return;
+    const int request = first_above(a.cu + 1, a.requests, row);
+    if (request >= a.requests) return;   // behind the last request
+    const int64_t position = (int64_t)row - a.cu[request] + (a.starts ? a.starts[request] : 0);
+    const int width = is_v ? a.cache.v_dim : a.cache.k_dim;
+    if (part * 8 >= width) return;
+    const int64_t column = position >> a.cache.page_shift;
+    int64_t page = -1;
+    if (position >= 0 && column < a.columns) page = a.table[(int64_t)request * a.columns + column];
+    const bool there = page >= 0 && page < a.cache.pages;
+    uint32_t word = 0;
+    half_t s = __builtin_bit_cast(half_t, (uint16_t)0x7e00);   // no such page: NaN
+    if (there) {
+        const int64_t slot = (page << a.cache.page_shift) + (position & ((1 << a.cache.page_shift) - 1));
+        word = is_v ? a.cache.v_codes[a.cache.v_word(slot, head, part)] : a.cache.k_codes[a.cache.k_word(slot, head, part)];
+        s = (is_v ? a.cache.v_scales : a.cache.k_scales)[a.cache.scale_at(slot, head)];
+    }
+    const h2 s2 = {s, s};
+    const h2 p0 = code_pair_low(word) * s2, p1 = code_pair_high(word) * s2, p2 = code_pair_low(word >> 8) * s2,
+             p3 = code_pair_high(word >> 8) * s2;
+    const half_t out[8] = {p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+    half_t* to = (is_v ? a.v + row * a.v_row + head * a.v_head : a.k + row * a.k_row + head * a.k_head) + part * 8;
+    if (part * 8 + 8 <= width) {
+        *reinterpret_cast<h8u*>(to) = h8u{out[0], out[1], out[2], out[3], out[4], out[5], out[6], out[7]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (part * 8 + i < width) to[i] = out[i];
+    }
+}
+
+int kv4_load_launch(const KvCache& cache, const int32_t* table, const int32_t* cu, const int32_t* starts, void* k, int64_t k_row,
+                    int64_t k_head, void* v, int64_t v_row, int64_t v_head, int requests, int columns, int rows, hipStream_t stream) {
+    const LoadArgs a = {cache, table, cu, starts, reinterpret_cast<half_t*>(k), reinterpret_cast<half_t*>(v), k_row, k_head, v_row, v_head,
+                        (int64_t)rows * cache.heads * 2, requests, columns, rows};
+    const int64_t blocks = (a.vectors + 15) / 16;
+    if (blocks > 0x7fffffffLL) return UNIQL_E_SHAPE;
+    hipLaunchKernelGGL(kv4_load_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    return hipGetLastError() == hipSuccess ? UNIQL_OK : UNIQL_E_LAUNCH;
+}
+
+}  // namespace uniql

@@ -26,6 +26,7 @@ __all__ = [
     "composite_hadamard_variant",
     "w4a16_read_floor", "w4a16_quantize", "w4a16_pack", "w4a16_unpack", "w4a16_cut_columns",
     "w4a16_cut_rows", "w4_embedding_quantize", "rope_indices_",
+    "kv_assign_pages", "kv4_store", "kv4_load", "kv4_attention", "prompt_attention",
 ]
 
 
@@ -606,3 +607,58 @@ def composite_hadamard_variant(base: int):
         return hadamard_composite(x, scale, base)
     _fn.__name__ = f"fast_hadamard_transform_{base}N"
     return _fn
+
+
+# ---- the 4-bit key / value cache and attention ---------------------------------------------------------------
+# No counterpart in the reference's extensions: its blocks use transformers' fp16 caches and torch's attention.
+# A cache is four tensors (k_codes, k_scales, v_codes, v_scales), see uniql_kv4_cache in the C header;
+# quantize.quant_kv_cache.W4KVCache owns them.
+
+def kv_assign_pages(new_tokens: torch.Tensor, lengths: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor,
+                    free_count: torch.Tensor, page_size: int, max_tokens: int, *, lengths_out: torch.Tensor | None = None,
+                    count_out: torch.Tensor | None = None):
+    """Gives pages to requests and places to their new tokens (uniql_kv_assign_pages), on the device alone: new_tokens and lengths
+    int32 [requests] (new_tokens < 0 ends a request), table int32 [requests, columns], free_pages int32 [pages] a stack of
+    free_count (int32 [1]) pages.  table and free_pages are modified; lengths and free_count too, unless lengths_out and
+    count_out receive the new ones.  Returns (slots int64 [max_tokens], positions int32 [max_tokens], cu int32 [requests + 1],
+    refused int32 [requests])."""
+    return _capi.host().kv_assign_pages(new_tokens, lengths, table, free_pages, free_count, page_size, max_tokens, lengths_out, count_out,
+                                        _stream_of(new_tokens, "new_tokens"))
+
+
+def kv4_store(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
+              v_codes: torch.Tensor, v_scales: torch.Tensor) -> None:
+    """Writes k and v (fp16 [tokens, heads, width], ranges of a larger buffer too) to the places `slots` (int64 [tokens]) of a cache;
+    places outside the pool are left out, and none may occur twice."""
+    _capi.host().kv4_store(k, v, slots, k_codes, k_scales, v_codes, v_scales, _stream_of(k, "k"))
+
+
+def kv4_load(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor, table: torch.Tensor,
+             cu: torch.Tensor, rows: int, k_dim: int, v_dim: int, *, starts: torch.Tensor | None = None,
+             k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None):
+    """Reads positions back as fp16: row t of the results is position starts[r] + t - cu[r] of the request r with
+    cu[r] <= t < cu[r + 1] (starts: 0 for all when None).  Returns (k [rows, heads, k_dim], v [rows, heads, v_dim]); rows
+    outside every request are left as they were (in k_out / v_out) or as allocated."""
+    return _capi.host().kv4_load(k_codes, k_scales, v_codes, v_scales, table, cu, rows, k_dim, v_dim, starts, k_out, v_out,
+                                 _stream_of(k_codes, "k_codes"))
+
+
+def kv4_attention(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor,
+                  table: torch.Tensor, lengths: torch.Tensor, v_dim: int, *, cu_q: torch.Tensor | None = None,
+                  scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of each request's newest tokens over its pages of a cache: q fp16 [rows, q heads, k_dim]; table int32 [requests,
+    columns]; lengths int32 [requests], the new tokens among them; cu_q int32 [requests + 1]: each request's rows (None: one
+    each).  scale: 1 / sqrt(k_dim) when None.  Returns fp16 [rows, q heads, v_dim]; rows outside every request are left as they
+    were (in out) or as allocated."""
+    return _capi.host().kv4_attention(q, k_codes, k_scales, v_codes, v_scales, table, lengths, v_dim, cu_q,
+                                      q.shape[-1] ** -0.5 if scale is None else scale, out, _stream_of(q, "q"), _accumulator)
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor | None = None, *,
+                     causal: bool = True, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention within each of several sequences that lie behind each other: q fp16 [rows, q heads, width], k and v fp16
+    [rows, kv heads, ..] (ranges of the fused projection's output too), cu_q / cu_k int32 [sequences + 1].  Causal masks are aligned
+    at the sequences' ends.  scale: 1 / sqrt(width) when None.  Returns fp16 [rows, q heads, v width]; rows outside every sequence
+    are left as they were (in out) or as allocated."""
+    return _capi.host().prompt_attention(q, k, v, cu_q, cu_k, causal, q.shape[-1] ** -0.5 if scale is None else scale, out,
+                                         _stream_of(q, "q"))
