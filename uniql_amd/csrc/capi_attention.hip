@@ -23,7 +23,7 @@ static constexpr int kMaxHeads = 4096, kMaxWidth = 128;
 static bool page_size_ok(int n) { return n == 16 || n == 32 || n == 64 || n == 128 || n == 256; }
 // columns of a table, and the tokens that a row of it has room for
 static bool columns_ok(int64_t rows, int64_t columns, int64_t page_size) {
-    return columns > 0 && columns <= (1 << 20) && columns * page_size <= 0x7fffffffLL && rows * columns <= 0x7fffffffLL;
+    return columns > 0 && columns <= (1 << 20) && columns * page_size <= (1LL << 30) && rows * columns <= 0x7fffffffLL;
 }
 
 // Sizes first, then (when there is work to do) pointers.
@@ -94,6 +94,7 @@ static int attention_sizes(const uniql_kv4_cache* cache, KvCache& c, int rows, i
     if (const int code = cache_sizes(cache, c)) return code;
     if (rows < 0 || requests < 0 || !columns_ok(requests, columns, cache->page_size)) return UNIQL_E_SHAPE;
     if (n_q_heads <= 0 || n_q_heads > kMaxHeads || n_q_heads % c.heads != 0) return UNIQL_E_SHAPE;
+    if ((int64_t)rows * (n_q_heads / c.heads) > (1LL << 30)) return UNIQL_E_SHAPE;
     return UNIQL_OK;
 }
 

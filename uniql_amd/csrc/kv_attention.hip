@@ -1,96 +1,413 @@
 // Attention of each request's newest tokens over its pages of the 4-bit cache: o = sum_j p_j v_j / sum_j p_j,
-// p_j = exp(scale q . k_j - m), over the positions j that the row sees.
+// p_j = exp(scale q . k_j - m), over the positions j that the row sees; k_j = s_j (c_j - 8), v_j = s'_j (c'_j - 8).
+//
+// A workgroup takes 16 rows (query heads of one key / value head, of one or several tokens) of a request over a run of positions;
+// its four waves take 64 positions in turn.  Both products are matrix instructions of 16 x 16 x 32 on fp16 with the codes as they are: a code
+// c in an fp16 number's low bits is the subnormal c 2^-24 (c 2^-20 four bits higher), which the instruction multiplies exactly, so that a
+// pair of codes costs one mask.  The 8 that belongs off the codes and the scales come in around the products:
+//   scores   scale s_j (2^24 (q . c_j 2^-24) - 8 sum q)      positions along the rows of the first product, so that
+//   output   2^24 sum_j w_j (c'_j 2^-24) - 8 sum_j w_j       its results are the second one's operand in the lanes where they are
+// with w_j = fp16(p_j s'_j).  For w_j to use fp16's range whatever the values' sizes, m is the running maximum of the scores plus
+// the exponent of s'_j: w_j <= 1 at the maximum, and it moves only when some w_j would pass 2^8.
+// The rounding of w_j (2^-11) is what a matrix instruction on fp16 asks for; sums, maxima and the output stay in fp32.
+//
+// Bound by HBM: 132 bytes for a position of 128 + 128 channels.  The lengths are on the device, so every workgroup finds its share from them
+// (kPositions x request tiles, shared out evenly): requests of any lengths fill the GPU alike.  Where several workgroups share a
+// request's rows they leave (m, sum p, o) in scratch memory and the last to arrive adds them up in their order.
 #include "kv_attention.hpp"
 
 namespace uniql {
 
-// One wave per row and head; 64 positions at a time, a lane each.
-__global__ __launch_bounds__(64) void kv4_attention_kernel(const KvAttentionArgs a) {
-    const int lane = threadIdx.x, row = blockIdx.x, head = blockIdx.y, kv_head = head / a.group;
-    __shared__ float q[128];
-    int request = row, first = 0, last = 1;
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
+
+constexpr int kTile = 64;              // positions a wave takes at a time
+constexpr int kRows = 16;              // rows of a workgroup
+constexpr int kWaves = 4;
+constexpr int kSlotFloats = 16 * 132;  // a workgroup's partial result: 16 rows of 128 channels, m and sum p
+constexpr int kOutStride = 132;
+constexpr float kNoMaximum = -3.0e38f;
+constexpr float kSlack = 8.0f;         // weights may grow to 2^8 before the maximum follows
+constexpr int kWorkgroups = 1024;      // that a call is shared out to, four a compute unit
+
+template <int S>
+struct Words;
+template <>
+struct Words<1> { typedef uint32_t type; };
+template <>
+struct Words<2> { typedef u32x2 type; };
+template <>
+struct Words<3> { typedef u32x3 type __attribute__((aligned(4))); };
+template <>
+struct Words<4> { typedef u32x4 type; };
+template <int S>
+__device__ __forceinline__ uint32_t word_of(const typename Words<S>::type& v, int i) {
+    if constexpr (S == 1) return v;
+    else return v[i];
+}
+
+__device__ __forceinline__ float quad_max(float v) {  // over the lanes l, l ^ 16, l ^ 32, l ^ 48
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+__device__ __forceinline__ h8 halves(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __builtin_bit_cast(h8, u32x4{a, b, c, d}); }
+
+// What a request asks for: its rows [first, first + count) and the positions in the cache.
+struct Request {
+    int first, count;
+    int length;
+};
+__device__ __forceinline__ Request request_of(const KvAttentionArgs& a, int r) {
+    Request q;
     if (a.cu_q) {
-        if (row < a.cu_q[0]) return;
-        int low = 0, high = a.requests;
-        while (low < high) {
-            const int mid = (low + high) >> 1;
-            if (a.cu_q[mid + 1] > row) high = mid;
-            else low = mid + 1;
-        }
-        request = low;
-        if (request >= a.requests) return;
-        first = a.cu_q[request];
-        last = a.cu_q[request + 1];
+        int b = a.cu_q[r], e = a.cu_q[r + 1];
+        b = b < 0 ? 0 : (b > a.rows ? a.rows : b);
+        e = e < b ? b : (e > a.rows ? a.rows : e);
+        q.first = b;
+        q.count = e - b;
     } else {
-        first = row;
-        last = row + 1;
+        q.first = r;
+        q.count = 1;
     }
+    const int64_t room = (int64_t)a.columns << a.cache.page_shift;
+    const int n = a.lengths[r];
+    q.length = n < 0 ? 0 : (n > room ? (int)room : n);
+    return q;
+}
+__device__ __forceinline__ int row_tiles(const KvAttentionArgs& a, const Request& q) { return (int)(((int64_t)q.count * a.group + kRows - 1) / kRows); }
+__device__ __forceinline__ int position_tiles(const Request& q) { return (q.length + kTile - 1) / kTile; }
+
+// A workgroup's share: `run` position tiles from tile `run * chunk` on, for row tile `rows` of request `request`; `index0` is the
+// index of the first of the `chunks` workgroups that share these rows.
+struct Share {
+    int request, rows, chunk, chunks, run, index0;
+};
+// Every wave finds it for itself.  Position tiles times row tiles of all requests, over the workgroups there are, give the run's
+// length; requests in order take one workgroup for each run.
+__device__ __forceinline__ bool find_share(const KvAttentionArgs& a, int index, Share& s) {
+    const int lane = threadIdx.x & 63;
+    float total = 0.f;
+    for (int r = lane; r < a.requests; r += 64) {
+        const Request q = request_of(a, r);
+        total += (float)row_tiles(a, q) * (float)position_tiles(q);
+    }
+    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d, 64);
+    // (a little more than the quotient: sums in fp32 must not make more runs than there are workgroups for)
+    const float run_f = total * 1.0001f / (float)a.shares;
+    int run = run_f < 1.0e9f ? (int)run_f + 1 : 1 << 30;
+    run = (run + kWaves - 1) / kWaves * kWaves;
+    int64_t before = 0;
+    for (int base = 0; base < a.requests; base += 64) {
+        const int r = base + lane;
+        int64_t mine = 0;
+        int tiles = 0, chunks = 1;
+        if (r < a.requests) {
+            const Request q = request_of(a, r);
+            tiles = row_tiles(a, q);
+            const int positions = position_tiles(q);
+            chunks = positions > run ? (positions + run - 1) / run : 1;
+            mine = (int64_t)tiles * chunks;
+        }
+        int64_t upto = mine;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t other = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += other;
+        }
+        const unsigned long long above = __ballot(before + upto > index);
+        if (above) {
+            const int owner = __builtin_ctzll(above);
+            const int64_t start = before + __shfl(upto - mine, owner, 64);
+            const int c = __shfl(chunks, owner, 64);
+            const int at = (int)(index - start);
+            s.request = __builtin_amdgcn_readfirstlane(base + owner);
+            s.chunks = __builtin_amdgcn_readfirstlane(c);
+            s.rows = __builtin_amdgcn_readfirstlane(at / c);
+            s.chunk = __builtin_amdgcn_readfirstlane(at % c);
+            s.run = run;
+            s.index0 = index - s.chunk;
+            return true;
+        }
+        before += __shfl(upto, 63, 64);
+    }
+    return false;
+}
+
+template <int S>
+__global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttentionArgs a) {
+    __shared__ __attribute__((aligned(16))) float merge[kWaves * 16 * kOutStride];
+    __shared__ float merge_m[kWaves * 16], merge_l[kWaves * 16];
+    __shared__ int last_flag;
     const KvCache& c = a.cache;
-    const int64_t capacity = (int64_t)a.columns << c.page_shift;
-    int64_t length = a.lengths[request];
-    length = length > capacity ? capacity : length;
-    const int64_t limit = length - (last - first) + (row - first) + 1;
-    const half_t* q_row = a.q + row * a.q_row + head * a.q_head;
-    for (int i = lane; i < 128; i += 64) q[i] = i < c.k_dim ? (float)q_row[i] : 0.f;
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    const float nan = __builtin_nanf("");
-    for (int64_t base = 0; base < limit; base += 64) {
-        const int64_t j = base + lane;
-        float score = -INFINITY, vs = 0.f;
-        int64_t slot = -1;
-        if (j < limit) {
-            const int64_t page = a.table[(int64_t)request * a.columns + (j >> c.page_shift)];
-            if (page >= 0 && page < c.pages) {
-                slot = (page << c.page_shift) + (j & ((1 << c.page_shift) - 1));
-                float dot = 0.f;
-                for (int w = 0; w < c.k_words; ++w) {
-                    const uint32_t word = c.k_codes[c.k_word(slot, kv_head, w)];
+    const int heads = c.heads, kv_head = (int)(blockIdx.x % (unsigned)heads), index = (int)(blockIdx.x / (unsigned)heads);
+    Share s;
+    if (!find_share(a, index, s)) return;
+    const Request rq = request_of(a, s.request);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quad = lane >> 4;
+    const int rows_total = rq.count * a.group, flat = s.rows * kRows + col;
+    const bool row_exists = flat < rows_total;
+    const int token = row_exists ? flat / a.group : 0, sub_head = row_exists ? flat - token * a.group : 0;
+    // positions that the lane's row sees; the first and the last row of the tile have the fewest and the most
+    const int limit = row_exists ? rq.length - rq.count + token + 1 : 0;
+    const int last_flat = rows_total - 1 < s.rows * kRows + kRows - 1 ? rows_total - 1 : s.rows * kRows + kRows - 1;
+    const int seen_by_all = rq.length - rq.count + s.rows * kRows / a.group + 1, seen_by_any = rq.length - rq.count + last_flat / a.group + 1;
+    const int tiles = (seen_by_any + kTile - 1) / kTile;
+    const int end = (s.chunk + 1) * s.run < tiles ? (s.chunk + 1) * s.run : tiles;
+
+    h8 q[S];
+    float q_sum = 0.f;
+    {
+        const half_t* row = a.q + (int64_t)(rq.first + token) * a.q_row + (int64_t)(kv_head * a.group + sub_head) * a.q_head;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) dot += q[8 * w + i] * ((float)((word >> kNibble(i)) & 15u) - 8.f);
-                }
-                score = dot * (float)c.k_scales[c.scale_at(slot, kv_head)] * a.scale;
-                vs = (float)c.v_scales[c.scale_at(slot, kv_head)];
-            } else {
-                score = nan;
-            }
-        }
-        float top = score;
-        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-        const float next = fmaxf(m, top);
-        const float p = j < limit ? (next == -INFINITY ? (score != score ? nan : 0.f) : expf(score - next)) : 0.f;
-        const float keep = m == -INFINITY ? 0.f : expf(m - next);
-        m = next;
-        l = l * keep + p;
-        o0 *= keep;
-        o1 *= keep;
-        const float w = j < limit ? p * vs : 0.f;
-        for (int t = 0; t < 64; ++t) {
-            if (base + t >= limit) break;
-            const float wt = __shfl(w, t, 64);
-            const int64_t st = __shfl(slot, t, 64);
-            if (st < 0) {
-                o0 = o1 = nan;
-                continue;
-            }
-            const int w0 = lane >> 3, w1 = 8 + (lane >> 3), n = kNibble(lane & 7);
-            if (w0 < c.v_words) o0 += wt * ((float)((c.v_codes[c.v_word(st, kv_head, w0)] >> n) & 15u) - 8.f);
-            if (w1 < c.v_words) o1 += wt * ((float)((c.v_codes[c.v_word(st, kv_head, w1)] >> n) & 15u) - 8.f);
+        for (int i = 0; i < S; ++i) {
+            q[i] = h8{};
+            if (row_exists) q[i] = load_eight_of(row, 8 * (S * quad + i), c.k_dim);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q_sum += (float)q[i][j];
         }
     }
-    for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
-    half_t* out = a.out + row * a.out_row + head * a.out_head;
-    const bool empty = limit <= 0;
-    if (lane < c.v_dim) out[lane] = empty ? (half_t)0.f : (half_t)(o0 / l);
-    if (lane + 64 < c.v_dim) out[lane + 64] = empty ? (half_t)0.f : (half_t)(o1 / l);
+    q_sum = quad_sum(q_sum);
+    const float log2e = 1.4426950408889634f;
+    const float by_code = a.scale * log2e * 16777216.0f, by_sum = -8.0f * q_sum * a.scale * log2e;
+
+    f4 out[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = f4{0.f, 0.f, 0.f, 0.f};
+    float m = kNoMaximum, l = 0.f, w_sum = 0.f;
+    const int32_t* table = a.table + (int64_t)s.request * a.columns;
+    const int last_column = rq.length > 0 ? (rq.length - 1) >> c.page_shift : 0;
+    const int n_word = col < c.v_words ? col : 0;
+    const uint32_t mask_low = 0x000f000fu, mask_high = 0x00f000f0u;
+
+    for (int t = s.chunk * s.run + wave; t < end; t += kWaves) {
+        const int j0 = t * kTile;
+        typename Words<S>::type kw[4];
+        u32x4 vw[4];
+        uint64_t ks[4], vs[4];
+        unsigned bad = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int j = j0 + 16 * u;
+            const int column = j >> c.page_shift;
+            int page = table[column < last_column ? column : last_column];
+            if ((unsigned)page >= (unsigned)c.pages) {
+                page = 0;
+                bad |= 1u << u;
+            }
+            const int64_t at = (((int64_t)page * heads + kv_head) << c.page_shift) + (j & ((1 << c.page_shift) - 1));
+            kw[u] = *reinterpret_cast<const typename Words<S>::type*>(c.k_codes + at * (4 * S) + col * (4 * S) + quad * S);
+            ks[u] = *reinterpret_cast<const uint64_t*>(c.k_scales + at + 4 * quad);
+            vs[u] = *reinterpret_cast<const uint64_t*>(c.v_scales + at + 4 * quad);
+            vw[u] = *reinterpret_cast<const u32x4*>(c.v_codes + at * c.v_words + quad * (4 * c.v_words) + 4 * n_word);
+        }
+        if (bad) {  // pages that do not exist: NaN
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (bad & (1u << u)) ks[u] = 0x7e007e007e007e00ull;
+        }
+        float score[16];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            f4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                const uint32_t w = word_of<S>(kw[u], i);
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    halves(w & mask_low, (w >> 4) & mask_low, (w >> 8) & mask_low, (w >> 12) & mask_low), q[i], acc, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const half_t scale = __builtin_bit_cast(half_t, (uint16_t)(ks[u] >> (16 * i)));
+                score[4 * u + i] = (acc[i] * by_code + by_sum) * (float)scale;
+            }
+        }
+        const bool masked = j0 + kTile > seen_by_all;
+        if (masked) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                uint64_t keep = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = j0 + 16 * u + 4 * quad + i;
+                    if (j < limit) keep |= 0xffffull << (16 * i);
+                    else score[4 * u + i] = -INFINITY;
+                }
+                vs[u] &= keep;
+            }
+        }
+        // the largest score and the largest exponent of a value's scale (fp16 numbers order as their bits do)
+        float top = score[0];
+        uint32_t scale_bits = 0;
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, score[i]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t b = (uint32_t)(vs[u] >> (16 * i)) & 0xffffu;
+                scale_bits = b > scale_bits ? b : scale_bits;
+            }
+        const float size = (float)(int)(scale_bits >> 10) - 14.f;
+        if (__any(top + size > m + kSlack)) {
+            const float next = fmaxf(m, quad_max(top + size));
+            const float fade = __builtin_amdgcn_exp2f(m - next);
+            m = next;
+            l *= fade;
+            w_sum *= fade;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) out[i] *= fade;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            h8 weight;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int u = 2 * k + h;
+                    const float p = __builtin_amdgcn_exp2f(score[4 * u + i] - m);
+                    l += p;
+                    weight[4 * h + i] = (half_t)(p * (float)__builtin_bit_cast(half_t, (uint16_t)(vs[u] >> (16 * i))));
+                }
+            const h2 one = {(half_t)1.f, (half_t)1.f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w_sum = __builtin_amdgcn_fdot2(h2{weight[2 * i], weight[2 * i + 1]}, one, w_sum, false);
+            const u32x4 first = vw[2 * k], second = vw[2 * k + 1];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                // byte b of four and four tokens' words, two tokens a register: value 2 (b & 1) .. in its low nibble, the next but one above
+                const uint32_t pick = 0x0c000c00u + ((uint32_t)(4 + b) << 16) + (uint32_t)b;
+                const uint32_t x0 = __builtin_amdgcn_perm(first[1], first[0], pick), x1 = __builtin_amdgcn_perm(first[3], first[2], pick);
+                const uint32_t x2 = __builtin_amdgcn_perm(second[1], second[0], pick), x3 = __builtin_amdgcn_perm(second[3], second[2], pick);
+                const int low = 4 * (b & 1) + (b >> 1), high = low + 2;
+                out[low] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(x0 & mask_low, x1 & mask_low, x2 & mask_low, x3 & mask_low), weight,
+                                                                  out[low], 0, 0, 0);
+                out[high] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(x0 & mask_high, x1 & mask_high, x2 & mask_high, x3 & mask_high),
+                                                                   weight, out[high], 0, 0, 0);
+            }
+        }
+    }
+    l = quad_sum(l);
+    w_sum = quad_sum(w_sum);
+    // the lane's row: channels 32 quad + 8 i + (0 .. 7); value index 2, 3, 6, 7 came from the high nibbles
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float* to = merge + (wave * 16 + col) * kOutStride + 32 * quad + 8 * i;
+        f4 lo, hi;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float unit = (j & 2) ? 1048576.0f : 16777216.0f;
+            lo[j] = out[j][i] * unit - 8.f * w_sum;
+            hi[j] = out[4 + j][i] * unit - 8.f * w_sum;
+        }
+        *reinterpret_cast<f4*>(to) = lo;
+        *reinterpret_cast<f4*>(to + 4) = hi;
+    }
+    if (quad == 0) {
+        merge_m[wave * 16 + col] = m;
+        merge_l[wave * 16 + col] = l;
+    }
+    __syncthreads();
+    // a thread: eight channels of a row
+    const int my_row = tid >> 4, my_channel = 8 * (tid & 15);
+    float top = kNoMaximum, sum = 0.f, o[8] = {};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, merge_m[w * 16 + my_row]);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        const float part = __builtin_amdgcn_exp2f(merge_m[w * 16 + my_row] - top);
+        sum += merge_l[w * 16 + my_row] * part;
+        const float* from = merge + (w * 16 + my_row) * kOutStride + my_channel;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] += from[i] * part;
+    }
+    const int my_flat = s.rows * kRows + my_row;
+    const bool mine = my_flat < rows_total;
+    if (s.chunks > 1) {
+        // The exchange: relaxed stores at device scope, which pass the local L2; a wait until they have been acknowledged; the
+        // barrier; the count.  The last to arrive reads with relaxed loads at device scope.
+        float* slot = a.temp + (int64_t)blockIdx.x * kSlotFloats;
+        if (mine) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) __hip_atomic_store(slot + my_row * kOutStride + my_channel + i, o[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if ((tid & 15) == 0) {
+                __hip_atomic_store(slot + my_row * kOutStride + 128, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __hip_atomic_store(slot + my_row * kOutStride + 129, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        unsigned* count = reinterpret_cast<unsigned*>(a.accum) + (int64_t)s.index0 * heads + kv_head;
+        if (tid == 0) last_flag = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)s.chunks - 1;
+        __syncthreads();
+        if (!last_flag) return;
+        if (tid == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (!mine) return;
+        top = kNoMaximum, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = 0.f;
+        for (int k = 0; k < s.chunks; ++k) {
+            const float* from = a.temp + ((int64_t)(s.index0 + k) * heads + kv_head) * kSlotFloats + my_row * kOutStride;
+            const float other = __hip_atomic_load(from + 128, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const float other_sum = __hip_atomic_load(from + 129, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __hip_atomic_load(from + my_channel + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const float next = fmaxf(top, other), keep = __builtin_amdgcn_exp2f(top - next), add = __builtin_amdgcn_exp2f(other - next);
+            top = next;
+            sum = sum * keep + other_sum * add;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = o[i] * keep + v[i] * add;
+        }
+    }
+    if (!mine) return;
+    const int my_token = my_flat / a.group, my_head = kv_head * a.group + my_flat - my_token * a.group;
+    const bool empty = rq.length - rq.count + my_token + 1 <= 0;
+    half_t* to = a.out + (int64_t)(rq.first + my_token) * a.out_row + (int64_t)my_head * a.out_head + my_channel;
+    h8u result;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) result[i] = empty ? (half_t)0.f : (half_t)(o[i] / sum);
+    if (my_channel + 8 <= c.v_dim) {
+        *reinterpret_cast<h8u*>(to) = result;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (my_channel + i < c.v_dim) to[i] = result[i];
+    }
+}
+
+// Workgroups for each key / value head: one for each run, and one more for each row tile whose last run is not whole.
+static int64_t shares_of(int heads) { return heads < kWorkgroups ? (kWorkgroups + heads - 1) / heads : 1; }
+static int64_t workgroups_of(int rows, int requests, int group, int heads, bool single) {
+    const int64_t tiles = single ? (int64_t)rows * ((group + kRows - 1) / kRows)
+                                 : (int64_t)rows * group / kRows + (requests < rows ? requests : rows);
+    return shares_of(heads) + tiles;
 }
 
 void kv4_attention_needs(int rows, int requests, int q_heads, const KvCache& cache, size_t* accum_bytes, size_t* temp_bytes) {
-    *accum_bytes = *temp_bytes = 0;
+    // (with and without cu_q alike: the larger of the two)
+    const int group = q_heads / cache.heads;
+    const int64_t one = workgroups_of(rows, requests, group, cache.heads, true), many = workgroups_of(rows, requests, group, cache.heads, false);
+    const int64_t workgroups = (rows == requests && one > many ? one : many) * cache.heads;
+    *accum_bytes = (size_t)(workgroups * 4 + 7) / 8 * 8;
+    *temp_bytes = (size_t)workgroups * kSlotFloats * 4;
 }
 
-int kv4_attention_launch(const KvAttentionArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL(kv4_attention_kernel, dim3((unsigned)a.rows, (unsigned)(a.group * a.cache.heads)), dim3(64), 0, stream, a);
+int kv4_attention_launch(const KvAttentionArgs& args, hipStream_t stream) {
+    KvAttentionArgs a = args;
+    a.shares = (int)shares_of(a.cache.heads);
+    const int64_t workgroups = workgroups_of(a.rows, a.requests, a.group, a.cache.heads, a.cu_q == nullptr) * a.cache.heads;
+    if (workgroups > 0x7fffffffLL) return UNIQL_E_SHAPE;
+    const dim3 grid((unsigned)workgroups), block(64 * kWaves);
+    switch (a.cache.k_words / 4) {
+        case 1: hipLaunchKernelGGL(kv4_attention_kernel<1>, grid, block, 0, stream, a); break;
+        case 2: hipLaunchKernelGGL(kv4_attention_kernel<2>, grid, block, 0, stream, a); break;
+        case 3: hipLaunchKernelGGL(kv4_attention_kernel<3>, grid, block, 0, stream, a); break;
+        default: hipLaunchKernelGGL(kv4_attention_kernel<4>, grid, block, 0, stream, a); break;
+    }
     return hipGetLastError() == hipSuccess ? UNIQL_OK : UNIQL_E_LAUNCH;
 }
 

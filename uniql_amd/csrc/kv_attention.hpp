@@ -15,6 +15,7 @@ struct KvAttentionArgs {
     void* accum;
     float* temp;
     int rows, requests, columns, group;  // group: query heads of a key / value head
+    int shares;                          // runs of positions that a head's work is shared out to
     float scale;
 };
 

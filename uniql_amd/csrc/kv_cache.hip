@@ -189,19 +189,6 @@ struct StoreArgs {
     int64_t vectors;  // tokens x key / value heads x 2
 };
 
-// Eight values of a vector from column j on; those past the vector's width count as zeros.
-__device__ __forceinline__ h8 load_eight_of(const half_t* x, int j, int width) {
-    if (j + 8 <= width) {
-        const h8u v = *reinterpret_cast<const h8u*>(x + j);
-        return h8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
-    }
-    h8 v = {};
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (j + i < width) v[i] = x[j + i];
-    return v;
-}
-
 // Sixteen lanes quantise a vector, eight values each, and store one word of codes each.
 __global__ __launch_bounds__(256) void kv4_store_kernel(const StoreArgs a) {
     const int64_t vector = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);

@@ -8,6 +8,19 @@ namespace uniql {
 // eight fp16 values at any address that holds fp16 values: the hardware takes a 16-byte access at any alignment
 typedef _Float16 h8u __attribute__((ext_vector_type(8), aligned(2)));
 
+// Eight values of a vector from column j on; those past the vector's width count as zeros.
+__device__ __forceinline__ h8 load_eight_of(const half_t* x, int j, int width) {
+    if (j + 8 <= width) {
+        const h8u v = *reinterpret_cast<const h8u*>(x + j);
+        return h8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+    }
+    h8 v = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (j + i < width) v[i] = x[j + i];
+    return v;
+}
+
 // bit position of value i of eight in a word: the order of the embedding's words, in which the pairs (0, 1), (2, 3), (4, 5),
 // (6, 7) lie 16 bits apart and come out with a mask and at most one shift each
 __device__ __host__ constexpr int kNibble(int i) { return 4 * (i >> 1) + 16 * (i & 1); }
