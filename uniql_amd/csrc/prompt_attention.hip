@@ -1,65 +1,329 @@
 // Causal attention over the prompts of several sequences that lie behind each other: o = sum_j p_j v_j / sum_j p_j,
 // p_j = exp(scale q . k_j - m), row i of a sequence with t queries and n keys over the keys j <= i + n - t.
+//
+// A workgroup takes 32 rows of a head for each of its waves and goes through the keys 64 at a time, in LDS, the next 64 on their way
+// meanwhile (two buffers, straight from memory to LDS).  Matrix instructions of 32 x 32 x 16: the scores come transposed, keys along
+// the rows, K q^T, because a lane then holds scores of one query and of just those keys that the second product, V^T P^T, wants
+// from it: the weights never leave its registers.  That product takes V transposed, four keys of one channel at a time, which the
+// transposing LDS read gives.  Rows of K and V lie in LDS with their 16-byte pieces exchanged by the row's number, so that neither
+// kind of read meets itself in a bank.
+// The maximum follows the scores only when a weight would pass 2^8 (weights are fp16, sums and outputs fp32): mostly once.
+// The rounding of the weights to fp16 (2^-11) is what a matrix instruction on fp16 asks for; their sum takes the rounded ones.
 #include "prompt_attention.hpp"
 
 namespace uniql {
 
+constexpr int kKeys = 64;               // keys of a step
+constexpr int kQueries = 32;            // rows of a wave
+constexpr float kLowest = -3.0e38f;
+constexpr float kRoom = 8.0f;           // weights may grow to 2^8 before the maximum follows
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4* lds_s4_ptr;
+typedef _Float16 h4u __attribute__((ext_vector_type(4), aligned(2)));
+
+#define UNIQL_WAIT_ALL_LOADS() __builtin_amdgcn_s_waitcnt(0x0F70)  // vmcnt(0), the other counters left alone (gfx9 encoding)
+
 __device__ __forceinline__ int clamp_to(int v, int low, int high) { return v < low ? low : (v > high ? high : v); }
 
-// One wave per row and head; 64 keys at a time, a lane each.
-__global__ __launch_bounds__(64) void prompt_attention_kernel(const PromptArgs a) {
-    const int lane = threadIdx.x, row = blockIdx.x, head = blockIdx.y, kv_head = head / a.group;
-    __shared__ float q[128];
-    if (row < a.cu_q[0]) return;
-    int low = 0, high = a.sequences;
-    while (low < high) {
-        const int mid = (low + high) >> 1;
-        if (a.cu_q[mid + 1] > row) high = mid;
-        else low = mid + 1;
-    }
-    if (low >= a.sequences) return;
-    const int first = a.cu_q[low], last = a.cu_q[low + 1];
-    const int k_first = clamp_to(a.cu_k[low], 0, a.k_rows), k_last = clamp_to(a.cu_k[low + 1], k_first, a.k_rows);
-    const int length = k_last - k_first;
-    const int64_t seen = a.causal ? (int64_t)length - (last - first) + (row - first) + 1 : length;
-    const int limit = seen < 0 ? 0 : (seen > length ? length : (int)seen);
-    const half_t* q_row = a.q + row * a.q_row + head * a.q_head;
-    for (int i = lane; i < 128; i += 64) q[i] = i < a.k_dim ? (float)q_row[i] : 0.f;
-    __syncthreads();
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int base = 0; base < limit; base += 64) {
-        const int j = base + lane;
-        float score = -INFINITY;
-        if (j < limit) {
-            const half_t* k = a.k + (int64_t)(k_first + j) * a.k_row + kv_head * a.k_head;
-            float dot = 0.f;
-            for (int i = 0; i < a.k_dim; ++i) dot += q[i] * (float)k[i];
-            score = dot * a.scale;
+struct Rows {
+    int q_first, q_count, k_first, k_count;
+};
+__device__ __forceinline__ Rows rows_of(const PromptArgs& a, int s) {
+    Rows r;
+    r.q_first = clamp_to(a.cu_q[s], 0, a.rows);
+    r.q_count = clamp_to(a.cu_q[s + 1], r.q_first, a.rows) - r.q_first;
+    r.k_first = clamp_to(a.cu_k[s], 0, a.k_rows);
+    r.k_count = clamp_to(a.cu_k[s + 1], r.k_first, a.k_rows) - r.k_first;
+    return r;
+}
+// The sequence and the block of rows in it that block `index` of all is; every wave finds it for itself.
+__device__ __forceinline__ bool find_block(const PromptArgs& a, int index, int block_rows, int& sequence, int& block) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int base = 0; base < a.sequences; base += 64) {
+        const int s = base + lane;
+        int mine = 0;
+        if (s < a.sequences) mine = (rows_of(a, s).q_count + block_rows - 1) / block_rows;
+        int upto = mine;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int other = __shfl_up(upto, d, 64);
+            if (lane >= d) upto += other;
         }
-        float top = score;
-        for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-        const float next = fmaxf(m, top);
-        const float p = j < limit ? (next == -INFINITY ? (score != score ? score : 0.f) : expf(score - next)) : 0.f;
-        const float keep = m == -INFINITY ? 0.f : expf(m - next);
-        m = next;
-        l = l * keep + p;
-        o0 *= keep;
-        o1 *= keep;
-        for (int t = 0; t < 64 && base + t < limit; ++t) {
-            const float pt = __shfl(p, t, 64);
-            const half_t* v = a.v + (int64_t)(k_first + base + t) * a.v_row + kv_head * a.v_head;
-            if (lane < a.v_dim) o0 += pt * (float)v[lane];
-            if (lane + 64 < a.v_dim) o1 += pt * (float)v[lane + 64];
+        const unsigned long long above = __ballot(before + upto > index);
+        if (above) {
+            const int owner = __builtin_ctzll(above);
+            sequence = __builtin_amdgcn_readfirstlane(base + owner);
+            block = __builtin_amdgcn_readfirstlane(index - before - __shfl(upto - mine, owner, 64));
+            return true;
         }
+        before += __shfl(upto, 63, 64);
     }
-    for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
-    half_t* out = a.out + row * a.out_row + head * a.out_head;
-    if (lane < a.v_dim) out[lane] = limit == 0 ? (half_t)0.f : (half_t)(o0 / l);
-    if (lane + 64 < a.v_dim) out[lane + 64] = limit == 0 ? (half_t)0.f : (half_t)(o1 / l);
+    return false;
 }
 
-int prompt_attention_launch(const PromptArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL(prompt_attention_kernel, dim3((unsigned)a.rows, (unsigned)a.heads), dim3(64), 0, stream, a);
+// Eight values of a row from column j on; those past its width count as zeros.
+__device__ __forceinline__ h8 row_piece(const half_t* x, int j, int width) {
+    typedef _Float16 h8u __attribute__((ext_vector_type(8), aligned(2)));
+    if (j + 8 <= width) {
+        const h8u v = *reinterpret_cast<const h8u*>(x + j);
+        return h8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+    }
+    h8 v = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (j + i < width) v[i] = x[j + i];
+    return v;
+}
+
+// D: the wider of the two head widths in units of 32, 2 to 4.  PIECES: rows of 16-byte pieces at multiples of 16 bytes, which go to LDS by
+// themselves; otherwise they pass through registers.
+template <int D, int WAVES, bool PIECES>
+__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attention_kernel(const PromptArgs a) {
+    constexpr int kSteps = 2 * D;                      // of 16 channels, of the first product
+    constexpr int kPieces = D == 2 ? 8 : 16;           // 16-byte pieces of a row in LDS
+    constexpr int kRowBytes = kPieces * 16;
+    constexpr int kTileBytes = kKeys * kRowBytes;
+    constexpr int kRowsAtOnce = 64 / kPieces;          // rows that a wave's access covers
+    constexpr int kAccesses = kKeys / (kRowsAtOnce * WAVES);
+    extern __shared__ __attribute__((aligned(16))) char lds[];  // two buffers of a K tile and a V tile
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
+    // neighbouring workgroups have different key / value heads: those of one head stay on an XCD and share its L2
+    const unsigned kv_heads = (unsigned)(a.heads / a.group), kv_head = blockIdx.x % kv_heads, rest = blockIdx.x / kv_heads;
+    const int head = (int)(kv_head * a.group + rest % a.group);
+    // later blocks see more keys: they come first
+    int sequence, block;
+    if (!find_block(a, (int)(a.blocks - 1 - rest / a.group), kQueries * WAVES, sequence, block)) return;
+    const Rows r = rows_of(a, sequence);
+    const int offset = r.k_count - r.q_count;
+    const int row0 = block * kQueries * WAVES + wave * kQueries, row = row0 + col;
+    const bool row_exists = row < r.q_count;
+    const int seen = a.causal ? clamp_to(row + offset + 1, 0, r.k_count) : r.k_count;  // keys of the lane's row
+    // of the wave's first row and of its last, and of the workgroup's last
+    const int last_row = clamp_to(row0 + kQueries - 1, 0, r.q_count - 1), block_last = clamp_to((block + 1) * kQueries * WAVES - 1, 0, r.q_count - 1);
+    const int fewest = a.causal ? clamp_to(row0 + offset + 1, 0, r.k_count) : r.k_count;
+    const int most = row0 < r.q_count ? (a.causal ? clamp_to(last_row + offset + 1, 0, r.k_count) : r.k_count) : 0;
+    const int block_most = a.causal ? clamp_to(block_last + offset + 1, 0, r.k_count) : r.k_count;
+    const int tiles = (block_most + kKeys - 1) / kKeys;
+
+    h8 q[kSteps];
+    {
+        const half_t* from = a.q + (int64_t)(r.q_first + (row_exists ? row : 0)) * a.q_row + (int64_t)head * a.q_head;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            q[i] = h8{};
+            if (row_exists && a.q_sign != 0) q[i] = row_piece(from, 16 * i + 8 * half, a.k_dim);
+            if (a.q_sign < 0) q[i] = -q[i];
+        }
+    }
+    f16 out[D];
+#pragma unroll
+    for (int i = 0; i < D; ++i) out[i] = f16{};
+    float m = kLowest, l = 0.f;
+    const float unit = a.scale * 1.4426950408889634f;  // positive: a negative scale has turned q
+
+    const half_t* const k_base = a.k + (int64_t)r.k_first * a.k_row + (int64_t)kv_head * a.k_head;
+    const half_t* const v_base = a.v + (int64_t)r.k_first * a.v_row + (int64_t)kv_head * a.v_head;
+    // this lane's part of an access: a row of the tile and a piece of it
+    const int part_row = wave * kRowsAtOnce + lane / kPieces, part = lane % kPieces;
+    const int k_piece = part ^ (part_row & (kPieces - 1)), v_piece = part ^ (2 * (part_row & 3));
+    auto fetch = [&](int tile, int buffer) __attribute__((always_inline)) {
+        const int key0 = tile * kKeys, left = r.k_count - key0 < kKeys ? r.k_count - key0 : kKeys;
+        char* const k_lds = lds + buffer * 2 * kTileBytes;
+        char* const v_lds = k_lds + kTileBytes;
+        if constexpr (PIECES) {
+            // rows behind the sequence lie beyond the descriptors and come as zeros, and so do pieces behind the width
+            const __amdgpu_buffer_rsrc_t k_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<half_t*>(k_base + (int64_t)key0 * a.k_row), 0, (unsigned)(((int64_t)(left - 1) * a.k_row + a.k_dim) * 2), 0x00020000);
+            const __amdgpu_buffer_rsrc_t v_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<half_t*>(v_base + (int64_t)key0 * a.v_row), 0, (unsigned)(((int64_t)(left - 1) * a.v_row + a.v_dim) * 2), 0x00020000);
+#pragma unroll
+            for (int i = 0; i < kAccesses; ++i) {
+                const int at = i * kRowsAtOnce * WAVES;  // a multiple of 16 or 8 rows: the exchange of pieces is the same
+                const unsigned k_off = k_piece * 8 < a.k_dim ? 2u * ((unsigned)(at + part_row) * (unsigned)a.k_row) + 16u * k_piece : 0xfffffff0u;
+                const unsigned v_off = v_piece * 8 < a.v_dim ? 2u * ((unsigned)(at + part_row) * (unsigned)a.v_row) + 16u * v_piece : 0xfffffff0u;
+                const int lds_at = (at + wave * kRowsAtOnce) * kRowBytes;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(k_rsrc, (lds_ptr)(k_lds + lds_at), 16, k_off, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(v_rsrc, (lds_ptr)(v_lds + lds_at), 16, v_off, 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kAccesses; ++i) {
+                const int at = i * kRowsAtOnce * WAVES + part_row;
+                h8 kv = {}, vv = {};
+                if (at < left) {
+                    kv = row_piece(k_base + (int64_t)(key0 + at) * a.k_row, 8 * k_piece, a.k_dim);
+                    vv = row_piece(v_base + (int64_t)(key0 + at) * a.v_row, 8 * v_piece, a.v_dim);
+                }
+                *reinterpret_cast<h8*>(k_lds + at * kRowBytes + part * 16) = kv;
+                *reinterpret_cast<h8*>(v_lds + at * kRowBytes + part * 16) = vv;
+            }
+        }
+    };
+    // where the lane reads: K rows col and 32 + col, piece 2 step + half; V rows 4 half + j (+ 8), j = (lane / 4) % 4, four channels
+    const int k_read = col * kRowBytes, k_swap = col & (kPieces - 1);
+    const int v_j = (lane >> 2) & 3, v_read = (4 * half + v_j) * kRowBytes + (lane & 1) * 8;
+    const int v_sub = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+
+    if (tiles > 0) fetch(0, 0);
+    for (int t = 0; t < tiles; ++t) {
+        UNIQL_WAIT_ALL_LOADS();
+        __syncthreads();
+        if (t + 1 < tiles) fetch(t + 1, (t + 1) & 1);
+        const char* const k_lds = lds + (t & 1) * 2 * kTileBytes;
+        const char* const v_lds = k_lds + kTileBytes;
+        const int key0 = t * kKeys;
+        if (key0 >= most) continue;  // the wave's rows see none of them (all waves take part in the barriers)
+        const bool masked = key0 + kKeys > fewest;
+        // A key that some rows of the tile see and others do not: its weight is zero for those, but zero times an infinity is not.  Keys
+        // with such values are found first and taken out of the product, see below; each lane looks at one key.
+        unsigned long long odd_keys = 0;
+        if (a.causal && masked) {
+            uint32_t any = 0;
+#pragma unroll 4
+            for (int i = 0; i < kPieces; ++i) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(v_lds + lane * kRowBytes + ((i + lane) & (kPieces - 1)) * 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    // an exponent of all ones overflows into the next bit
+                    any |= ((w[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+                }
+            }
+            odd_keys = __ballot(any != 0);
+        }
+        f16 score[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            score[k] = f16{};
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const h8 keys = *reinterpret_cast<const h8*>(k_lds + k_read + k * 32 * kRowBytes + (((2 * i + half) ^ k_swap) * 16));
+                score[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys, q[i], score[k], 0, 0, 0);
+            }
+        }
+        if (masked) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (key0 + 32 * k + 8 * (i / 4) + 4 * half + i % 4 >= seen) score[k][i] = -INFINITY;
+        }
+        float top = score[0][0];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, score[k][i]);
+        if (__any(top * unit > m + kRoom)) {
+            const float next = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * unit);
+            const float fade = __builtin_amdgcn_exp2f(m - next);
+            m = next;
+            l *= fade;
+#pragma unroll
+            for (int i = 0; i < D; ++i) out[i] *= fade;
+        }
+        h8 weight[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                weight[s][i] = (half_t)__builtin_amdgcn_exp2f(__builtin_fmaf(score[s >> 1][8 * (s & 1) + i], unit, -m));
+            const h2 one = {(half_t)1.f, (half_t)1.f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l = __builtin_amdgcn_fdot2(h2{weight[s][2 * i], weight[s][2 * i + 1]}, one, l, false);
+        }
+        if (odd_keys) {
+            // one key at a time, in the rows that see it
+            for (unsigned long long left = odd_keys; left; left &= left - 1) {
+                const int key = __builtin_ctzll(left);
+                const int index = 8 * (key >> 4) + 4 * ((key >> 3) & 1) + (key & 3);  // of the weights, in the half (key >> 2) & 1
+                float p = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) p = i == index ? (float)weight[i >> 3][i & 7] : p;
+                p = __shfl(p, col + 32 * ((key >> 2) & 1), 64);
+                if (key0 + key < seen && row_exists) {
+#pragma unroll
+                    for (int i = 0; i < D; ++i)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const int channel = 32 * i + 8 * (j / 4) + 4 * half + j % 4;
+                            const half_t v = *reinterpret_cast<const half_t*>(v_lds + key * kRowBytes + ((channel >> 3) ^ (2 * (key & 3))) * 16 +
+                                                                              (channel & 7) * 2);
+                            out[i][j] += p * (float)v;
+                        }
+                }
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int i = 0; i < D; ++i) {
+                const int piece = ((4 * i + v_sub) ^ (2 * v_j)) * 16;
+                s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(v_lds + v_read + piece + s * 16 * kRowBytes));
+                s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(v_lds + v_read + piece + (s * 16 + 8) * kRowBytes));
+                if (odd_keys) {
+                    const unsigned keys_lo = (unsigned)(odd_keys >> (16 * s + 4 * half)), keys_hi = (unsigned)(odd_keys >> (16 * s + 8 + 4 * half));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if ((keys_lo >> j) & 1) lo[j] = 0;
+                        if ((keys_hi >> j) & 1) hi[j] = 0;
+                    }
+                }
+                typedef short s8 __attribute__((ext_vector_type(8)));
+                const h8 values = __builtin_bit_cast(h8, s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+                out[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values, weight[s], out[i], 0, 0, 0);
+            }
+        }
+    }
+    l += __shfl_xor(l, 32, 64);
+    if (!row_exists) return;
+    half_t* to = a.out + (int64_t)(r.q_first + row) * a.out_row + (int64_t)head * a.out_head;
+    const float inverse = seen > 0 ? 1.0f / l : 0.f;
+#pragma unroll
+    for (int i = 0; i < D; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int channel = 32 * i + 8 * j + 4 * half;
+            half_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = seen > 0 ? (half_t)(out[i][4 * j + e] * inverse) : (half_t)0.f;
+            if (channel + 4 <= a.v_dim) {
+                *reinterpret_cast<h4u*>(to + channel) = h4u{v[0], v[1], v[2], v[3]};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (channel + e < a.v_dim) to[channel + e] = v[e];
+            }
+        }
+}
+
+template <int D, int WAVES, bool PIECES>
+static void go(const PromptArgs& a, hipStream_t stream) {
+    const unsigned lds = 4u * kKeys * (D == 2 ? 8 : 16) * 16;
+    hipLaunchKernelGGL((prompt_attention_kernel<D, WAVES, PIECES>), dim3((unsigned)(a.blocks * a.heads)), dim3(64 * WAVES), lds, stream, a);
+}
+template <int D>
+static void go(const PromptArgs& a, bool pieces, hipStream_t stream) {
+    if (pieces) go<D, 4, true>(a, stream);
+    else go<D, 4, false>(a, stream);
+}
+
+int prompt_attention_launch(const PromptArgs& args, hipStream_t stream) {
+    PromptArgs a = args;
+    a.q_sign = a.scale == 0.f ? 0 : (a.scale < 0.f ? -1 : 1);
+    a.scale = a.q_sign == 0 ? 1.0f : (a.scale < 0.f ? -a.scale : a.scale);
+    const int waves = 4;
+    const int64_t blocks = (int64_t)a.rows / (kQueries * waves) + (a.sequences < a.rows ? a.sequences : a.rows);
+    if (blocks * a.heads > 0x7fffffffLL) return UNIQL_E_SHAPE;
+    a.blocks = (int)blocks;
+    // 64 rows of K or V stay below 2^32 bytes
+    const int64_t far = 1LL << 25;
+    const uintptr_t bases = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
+    const bool pieces = ((a.k_row | a.k_head | a.v_row | a.v_head | a.k_dim | a.v_dim) & 7) == 0 && (bases & 15) == 0 && a.k_row >= 0 &&
+                        a.v_row >= 0 && a.k_row <= far && a.v_row <= far;
+    const int width = ((a.k_dim > a.v_dim ? a.k_dim : a.v_dim) + 31) / 32;
+    if (width <= 2) go<2>(a, pieces, stream);
+    else if (width == 3) go<3>(a, pieces, stream);
+    else go<4>(a, pieces, stream);
     return hipGetLastError() == hipSuccess ? UNIQL_OK : UNIQL_E_LAUNCH;
 }
 

@@ -12,6 +12,7 @@ struct PromptArgs {
     half_t* out;
     int rows, k_rows, sequences, heads, group, k_dim, v_dim, causal;
     float scale;
+    int q_sign, blocks;  // set by the launch: the scale's sign, and blocks of rows in all sequences at most
 };
 
 }  // namespace uniql
