@@ -19,6 +19,8 @@ constexpr float kLowest = -3.0e38f;
 constexpr float kRoom = 8.0f;           // weights may grow to 2^8 before the maximum follows
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef short s4 __attribute__((ext_vector_type(4)));
+typedef short s8 __attribute__((ext_vector_type(8)));
+typedef float f2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s4* lds_s4_ptr;
 typedef _Float16 h4u __attribute__((ext_vector_type(4), aligned(2)));
 
@@ -86,7 +88,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
     constexpr int kTileBytes = kKeys * kRowBytes;
     constexpr int kRowsAtOnce = 64 / kPieces;          // rows that a wave's access covers
     constexpr int kAccesses = kKeys / (kRowsAtOnce * WAVES);
-    extern __shared__ __attribute__((aligned(16))) char lds[];  // two buffers of a K tile and a V tile
+    extern __shared__ __attribute__((aligned(16))) char lds[];  // two K tiles, two V tiles
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     // neighbouring workgroups have different key / value heads: those of one head stay on an XCD and share its L2
     const unsigned kv_heads = (unsigned)(a.heads / a.group), kv_head = blockIdx.x % kv_heads, rest = blockIdx.x / kv_heads;
@@ -104,6 +106,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
     const int fewest = a.causal ? clamp_to(row0 + offset + 1, 0, r.k_count) : r.k_count;
     const int most = row0 < r.q_count ? (a.causal ? clamp_to(last_row + offset + 1, 0, r.k_count) : r.k_count) : 0;
     const int block_most = a.causal ? clamp_to(block_last + offset + 1, 0, r.k_count) : r.k_count;
+    const int block_fewest = a.causal ? clamp_to(block * kQueries * WAVES + offset + 1, 0, r.k_count) : r.k_count;
     const int tiles = (block_most + kKeys - 1) / kKeys;
 
     h8 q[kSteps];
@@ -127,151 +130,157 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
     // this lane's part of an access: a row of the tile and a piece of it
     const int part_row = wave * kRowsAtOnce + lane / kPieces, part = lane % kPieces;
     const int k_piece = part ^ (part_row & (kPieces - 1)), v_piece = part ^ (2 * (part_row & 3));
-    auto fetch = [&](int tile, int buffer) __attribute__((always_inline)) {
+    // Rows behind the sequence lie beyond the descriptor and come as zeros, and so do pieces behind the width.
+    auto fetch = [&](const half_t* base, int64_t stride, int width, int piece, int tile, char* to) __attribute__((always_inline)) {
         const int key0 = tile * kKeys, left = r.k_count - key0 < kKeys ? r.k_count - key0 : kKeys;
-        char* const k_lds = lds + buffer * 2 * kTileBytes;
-        char* const v_lds = k_lds + kTileBytes;
         if constexpr (PIECES) {
-            // rows behind the sequence lie beyond the descriptors and come as zeros, and so do pieces behind the width
-            const __amdgpu_buffer_rsrc_t k_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<half_t*>(k_base + (int64_t)key0 * a.k_row), 0, (unsigned)(((int64_t)(left - 1) * a.k_row + a.k_dim) * 2), 0x00020000);
-            const __amdgpu_buffer_rsrc_t v_rsrc = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<half_t*>(v_base + (int64_t)key0 * a.v_row), 0, (unsigned)(((int64_t)(left - 1) * a.v_row + a.v_dim) * 2), 0x00020000);
+            const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<half_t*>(base + (int64_t)key0 * stride), 0,
+                                                                                  (unsigned)(((int64_t)(left - 1) * stride + width) * 2), 0x00020000);
 #pragma unroll
             for (int i = 0; i < kAccesses; ++i) {
-                const int at = i * kRowsAtOnce * WAVES;  // a multiple of 16 or 8 rows: the exchange of pieces is the same
-                const unsigned k_off = k_piece * 8 < a.k_dim ? 2u * ((unsigned)(at + part_row) * (unsigned)a.k_row) + 16u * k_piece : 0xfffffff0u;
-                const unsigned v_off = v_piece * 8 < a.v_dim ? 2u * ((unsigned)(at + part_row) * (unsigned)a.v_row) + 16u * v_piece : 0xfffffff0u;
-                const int lds_at = (at + wave * kRowsAtOnce) * kRowBytes;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(k_rsrc, (lds_ptr)(k_lds + lds_at), 16, k_off, 0, 0, 0);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(v_rsrc, (lds_ptr)(v_lds + lds_at), 16, v_off, 0, 0, 0);
+                const int at = i * kRowsAtOnce * WAVES;  // a multiple of 16 rows: the exchange of pieces is the same
+                const unsigned off = piece * 8 < width ? 2u * ((unsigned)(at + part_row) * (unsigned)stride) + 16u * piece : 0xfffffff0u;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(to + (at + wave * kRowsAtOnce) * kRowBytes), 16, off, 0, 0, 0);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < kAccesses; ++i) {
                 const int at = i * kRowsAtOnce * WAVES + part_row;
-                h8 kv = {}, vv = {};
-                if (at < left) {
-                    kv = row_piece(k_base + (int64_t)(key0 + at) * a.k_row, 8 * k_piece, a.k_dim);
-                    vv = row_piece(v_base + (int64_t)(key0 + at) * a.v_row, 8 * v_piece, a.v_dim);
-                }
-                *reinterpret_cast<h8*>(k_lds + at * kRowBytes + part * 16) = kv;
-                *reinterpret_cast<h8*>(v_lds + at * kRowBytes + part * 16) = vv;
+                h8 v = {};
+                if (at < left) v = row_piece(base + (int64_t)(key0 + at) * stride, 8 * piece, width);
+                *reinterpret_cast<h8*>(to + at * kRowBytes + part * 16) = v;
             }
         }
     };
+    auto fetch_k = [&](int tile, int buffer) __attribute__((always_inline)) { fetch(k_base, a.k_row, a.k_dim, k_piece, tile, lds + buffer * kTileBytes); };
+    auto fetch_v = [&](int tile, int buffer) __attribute__((always_inline)) { fetch(v_base, a.v_row, a.v_dim, v_piece, tile, lds + (2 + buffer) * kTileBytes); };
     // where the lane reads: K rows col and 32 + col, piece 2 step + half; V rows 4 half + j (+ 8), j = (lane / 4) % 4, four channels
     const int k_read = col * kRowBytes, k_swap = col & (kPieces - 1);
     const int v_j = (lane >> 2) & 3, v_read = (4 * half + v_j) * kRowBytes + (lane & 1) * 8;
     const int v_sub = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-
-    if (tiles > 0) fetch(0, 0);
-    for (int t = 0; t < tiles; ++t) {
+    auto products = [&](int buffer, int k, f16& score) __attribute__((always_inline)) {
+        score = f16{};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const h8 keys = *reinterpret_cast<const h8*>(lds + buffer * kTileBytes + k_read + k * 32 * kRowBytes + (((2 * i + half) ^ k_swap) * 16));
+            score = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys, q[i], score, 0, 0, 0);
+        }
+    };
+    // A step: the weights of tile t from its scores, which the step before has computed, the next tile's scores, the second product.
+    auto step = [&](int t, f16 (&score)[2], f16 (&next)[2]) __attribute__((always_inline)) {
+        const int buffer = t & 1, key0 = t * kKeys;
         UNIQL_WAIT_ALL_LOADS();
         __syncthreads();
-        if (t + 1 < tiles) fetch(t + 1, (t + 1) & 1);
-        const char* const k_lds = lds + (t & 1) * 2 * kTileBytes;
-        const char* const v_lds = k_lds + kTileBytes;
-        const int key0 = t * kKeys;
-        if (key0 >= most) continue;  // the wave's rows see none of them (all waves take part in the barriers)
+        if (t + 2 < tiles) fetch_k(t + 2, buffer);
+        if (t + 1 < tiles) fetch_v(t + 1, buffer ^ 1);
+        char* const v_lds = lds + (2 + buffer) * kTileBytes;
         const bool masked = key0 + kKeys > fewest;
         // A key that some rows of the tile see and others do not: its weight is zero for those, but zero times an infinity is not.  Keys
         // with such values are found first and taken out of the product, see below; each lane looks at one key.
         unsigned long long odd_keys = 0;
-        if (a.causal && masked) {
+        if (a.causal && key0 + kKeys > block_fewest) {
             uint32_t any = 0;
 #pragma unroll 4
             for (int i = 0; i < kPieces; ++i) {
                 const u32x4 w = *reinterpret_cast<const u32x4*>(v_lds + lane * kRowBytes + ((i + lane) & (kPieces - 1)) * 16);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    // an exponent of all ones overflows into the next bit
-                    any |= ((w[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
-                }
+                for (int j = 0; j < 4; ++j) any |= ((w[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;  // an exponent of all ones runs over
             }
             odd_keys = __ballot(any != 0);
         }
-        f16 score[2];
+        const bool active = key0 < most;  // the wave's rows see some of the keys (all waves take part in the barriers)
+        h8 weight[4];
+        if (active) {
+            if (masked) {
+                asm volatile("");  // keeps the comparisons out of the other tiles' way
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            score[k] = f16{};
+                for (int k = 0; k < 2; ++k)
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const h8 keys = *reinterpret_cast<const h8*>(k_lds + k_read + k * 32 * kRowBytes + (((2 * i + half) ^ k_swap) * 16));
-                score[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys, q[i], score[k], 0, 0, 0);
+                    for (int i = 0; i < 16; ++i)
+                        if (key0 + 32 * k + 8 * (i / 4) + 4 * half + i % 4 >= seen) score[k][i] = -INFINITY;
             }
-        }
-        if (masked) {
+            float top = score[0][0];
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (key0 + 32 * k + 8 * (i / 4) + 4 * half + i % 4 >= seen) score[k][i] = -INFINITY;
-        }
-        float top = score[0][0];
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, score[k][i]);
+            if (__any(top * unit > m + kRoom)) {
+                const float higher = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * unit);
+                const float fade = __builtin_amdgcn_exp2f(m - higher);
+                m = higher;
+                l *= fade;
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+                for (int i = 0; i < D; ++i) out[i] *= fade;
+            }
+            products(buffer ^ 1, 0, next[0]);
+            products(buffer ^ 1, 1, next[1]);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, score[k][i]);
-        if (__any(top * unit > m + kRoom)) {
-            const float next = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * unit);
-            const float fade = __builtin_amdgcn_exp2f(m - next);
-            m = next;
-            l *= fade;
+            for (int s = 0; s < 4; ++s) {
+                h2 pair[4];
 #pragma unroll
-            for (int i = 0; i < D; ++i) out[i] *= fade;
-        }
-        h8 weight[4];
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                weight[s][i] = (half_t)__builtin_amdgcn_exp2f(__builtin_fmaf(score[s >> 1][8 * (s & 1) + i], unit, -m));
-            const h2 one = {(half_t)1.f, (half_t)1.f};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) l = __builtin_amdgcn_fdot2(h2{weight[s][2 * i], weight[s][2 * i + 1]}, one, l, false);
-        }
-        if (odd_keys) {
-            // one key at a time, in the rows that see it
-            for (unsigned long long left = odd_keys; left; left &= left - 1) {
-                const int key = __builtin_ctzll(left);
-                const int index = 8 * (key >> 4) + 4 * ((key >> 3) & 1) + (key & 3);  // of the weights, in the half (key >> 2) & 1
-                float p = 0.f;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) p = i == index ? (float)weight[i >> 3][i & 7] : p;
-                p = __shfl(p, col + 32 * ((key >> 2) & 1), 64);
-                if (key0 + key < seen && row_exists) {
-#pragma unroll
-                    for (int i = 0; i < D; ++i)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const int channel = 32 * i + 8 * (j / 4) + 4 * half + j % 4;
-                            const half_t v = *reinterpret_cast<const half_t*>(v_lds + key * kRowBytes + ((channel >> 3) ^ (2 * (key & 3))) * 16 +
-                                                                              (channel & 7) * 2);
-                            out[i][j] += p * (float)v;
-                        }
+                for (int i = 0; i < 4; ++i) {
+                    const f2 p = {__builtin_amdgcn_exp2f(__builtin_fmaf(score[s >> 1][8 * (s & 1) + 2 * i], unit, -m)),
+                                  __builtin_amdgcn_exp2f(__builtin_fmaf(score[s >> 1][8 * (s & 1) + 2 * i + 1], unit, -m))};
+                    pair[i] = __builtin_convertvector(p, h2);
+                    l = __builtin_amdgcn_fdot2(pair[i], h2{(half_t)1.f, (half_t)1.f}, l, false);
                 }
+                weight[s] = h8{pair[0][0], pair[0][1], pair[1][0], pair[1][1], pair[2][0], pair[2][1], pair[3][0], pair[3][1]};
             }
         }
+        if (odd_keys) {  // the same for all waves
+            // one key at a time, in the rows that see it; then zeros take the keys' place in LDS
+            if (active) {
+                for (unsigned long long left = odd_keys; left; left &= left - 1) {
+                    const int key = __builtin_ctzll(left);
+                    const int index = 4 * (key >> 4) + 2 * ((key >> 3) & 1) + ((key >> 1) & 1);  // of the pair of weights, in the half (key >> 2) & 1
+                    uint32_t pair = 0;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
+                    for (int i = 0; i < 16; ++i) pair = i == index ? __builtin_bit_cast(u32x4, weight[i >> 2])[i & 3] : pair;
+                    pair = (uint32_t)__shfl((int)pair, col + 32 * ((key >> 2) & 1), 64);
+                    const float p = (float)bits_to_h2(pair)[key & 1];
+                    if (key0 + key < seen && row_exists) {
 #pragma unroll
-            for (int i = 0; i < D; ++i) {
-                const int piece = ((4 * i + v_sub) ^ (2 * v_j)) * 16;
-                s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(v_lds + v_read + piece + s * 16 * kRowBytes));
-                s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(v_lds + v_read + piece + (s * 16 + 8) * kRowBytes));
-                if (odd_keys) {
-                    const unsigned keys_lo = (unsigned)(odd_keys >> (16 * s + 4 * half)), keys_hi = (unsigned)(odd_keys >> (16 * s + 8 + 4 * half));
+                        for (int i = 0; i < D; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if ((keys_lo >> j) & 1) lo[j] = 0;
-                        if ((keys_hi >> j) & 1) hi[j] = 0;
+                            for (int j = 0; j < 16; ++j) {
+                                const int channel = 32 * i + 8 * (j / 4) + 4 * half + j % 4;
+                                const half_t v = *reinterpret_cast<const half_t*>(v_lds + key * kRowBytes +
+                                                                                  ((channel >> 3) ^ (2 * (key & 3))) * 16 + (channel & 7) * 2);
+                                out[i][j] += p * (float)v;
+                            }
                     }
                 }
-                typedef short s8 __attribute__((ext_vector_type(8)));
-                const h8 values = __builtin_bit_cast(h8, s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
-                out[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values, weight[s], out[i], 0, 0, 0);
             }
+            __syncthreads();
+            if (wave == 0 && ((odd_keys >> lane) & 1))
+                for (int i = 0; i < kPieces; ++i) *reinterpret_cast<u32x4*>(v_lds + lane * kRowBytes + i * 16) = u32x4{0u, 0u, 0u, 0u};
+            __syncthreads();
+        }
+        if (active) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int i = 0; i < D; ++i) {
+                    const int piece = ((4 * i + v_sub) ^ (2 * v_j)) * 16;
+                    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(v_lds + v_read + piece + s * 16 * kRowBytes));
+                    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(v_lds + v_read + piece + (s * 16 + 8) * kRowBytes));
+                    const h8 values = __builtin_bit_cast(h8, s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+                    out[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values, weight[s], out[i], 0, 0, 0);
+                }
+        }
+    };
+    if (tiles > 0) {
+        f16 even[2], odd[2];
+        fetch_k(0, 0);
+        fetch_v(0, 0);
+        if (tiles > 1) fetch_k(1, 1);
+        UNIQL_WAIT_ALL_LOADS();
+        __syncthreads();
+        products(0, 0, even[0]);
+        products(0, 1, even[1]);
+        for (int t = 0; t < tiles; t += 2) {
+            step(t, even, odd);
+            if (t + 1 < tiles) step(t + 1, odd, even);
         }
     }
     l += __shfl_xor(l, 32, 64);
