@@ -226,6 +226,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
                 }
                 weight[s] = h8{pair[0][0], pair[0][1], pair[1][0], pair[1][1], pair[2][0], pair[2][1], pair[3][0], pair[3][1]};
             }
+            // the next tile's scores: operands four reads ahead, each matrix instruction beside its share of this tile's weights
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int i = 0; i < 2 * kSteps; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x400, 32 / (2 * kSteps), 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 64 / (2 * kSteps), 0);
+            }
         }
         if (odd_keys) {  // the same for all waves
             // one key at a time, in the rows that see it; then zeros take the keys' place in LDS
