@@ -88,7 +88,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
     constexpr int kTileBytes = kKeys * kRowBytes;
     constexpr int kRowsAtOnce = 64 / kPieces;          // rows that a wave's access covers
     constexpr int kAccesses = kKeys / (kRowsAtOnce * WAVES);
-    extern __shared__ __attribute__((aligned(16))) char lds[];  // two K tiles, two V tiles
+    // Two K tiles and two V tiles: variables of their own, which tells the compiler that reading one does not wait for what is on its way
+    // into another.
+    __shared__ __attribute__((aligned(16))) char k_even[kTileBytes], k_odd[kTileBytes], v_even[kTileBytes], v_odd[kTileBytes];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
     // neighbouring workgroups have different key / value heads: those of one head stay on an XCD and share its L2
     const unsigned kv_heads = (unsigned)(a.heads / a.group), kv_head = blockIdx.x % kv_heads, rest = blockIdx.x / kv_heads;
@@ -152,28 +154,22 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
             }
         }
     };
-    auto fetch_k = [&](int tile, int buffer) __attribute__((always_inline)) { fetch(k_base, a.k_row, a.k_dim, k_piece, tile, lds + buffer * kTileBytes); };
-    auto fetch_v = [&](int tile, int buffer) __attribute__((always_inline)) { fetch(v_base, a.v_row, a.v_dim, v_piece, tile, lds + (2 + buffer) * kTileBytes); };
+    auto fetch_k = [&](int tile, char* to) __attribute__((always_inline)) { fetch(k_base, a.k_row, a.k_dim, k_piece, tile, to); };
+    auto fetch_v = [&](int tile, char* to) __attribute__((always_inline)) { fetch(v_base, a.v_row, a.v_dim, v_piece, tile, to); };
     // where the lane reads: K rows col and 32 + col, piece 2 step + half; V rows 4 half + j (+ 8), j = (lane / 4) % 4, four channels
     const int k_read = col * kRowBytes, k_swap = col & (kPieces - 1);
     const int v_j = (lane >> 2) & 3, v_read = (4 * half + v_j) * kRowBytes + (lane & 1) * 8;
     const int v_sub = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-    auto products = [&](int buffer, int k, f16& score) __attribute__((always_inline)) {
-        score = f16{};
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            const h8 keys = *reinterpret_cast<const h8*>(lds + buffer * kTileBytes + k_read + k * 32 * kRowBytes + (((2 * i + half) ^ k_swap) * 16));
-            score = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys, q[i], score, 0, 0, 0);
-        }
+    auto keys_of = [&](const char* tile, int k, int i) __attribute__((always_inline)) {
+        return *reinterpret_cast<const h8*>(tile + k_read + k * 32 * kRowBytes + (((2 * i + half) ^ k_swap) * 16));
     };
     // A step: the weights of tile t from its scores, which the step before has computed, the next tile's scores, the second product.
-    auto step = [&](int t, f16 (&score)[2], f16 (&next)[2]) __attribute__((always_inline)) {
-        const int buffer = t & 1, key0 = t * kKeys;
+    auto step = [&](int t, char* k_lds, char* v_lds, char* next_k_lds, char* next_v_lds, f16 (&score)[2], f16 (&next)[2]) __attribute__((always_inline)) {
+        const int key0 = t * kKeys;
         UNIQL_WAIT_ALL_LOADS();
         __syncthreads();
-        if (t + 2 < tiles) fetch_k(t + 2, buffer);
-        if (t + 1 < tiles) fetch_v(t + 1, buffer ^ 1);
-        char* const v_lds = lds + (2 + buffer) * kTileBytes;
+        if (t + 2 < tiles) fetch_k(t + 2, k_lds);
+        if (t + 1 < tiles) fetch_v(t + 1, next_v_lds);
         const bool masked = key0 + kKeys > fewest;
         // A key that some rows of the tile see and others do not: its weight is zero for those, but zero times an infinity is not.  Keys
         // with such values are found first and taken out of the product, see below; each lane looks at one key.
@@ -189,7 +185,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
             odd_keys = __ballot(any != 0);
         }
         const bool active = key0 < most;  // the wave's rows see some of the keys (all waves take part in the barriers)
-        h8 weight[4];
         if (active) {
             if (masked) {
                 asm volatile("");  // keeps the comparisons out of the other tiles' way
@@ -212,41 +207,18 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
 #pragma unroll
                 for (int i = 0; i < D; ++i) out[i] *= fade;
             }
-            products(buffer ^ 1, 0, next[0]);
-            products(buffer ^ 1, 1, next[1]);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                h2 pair[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const f2 p = {__builtin_amdgcn_exp2f(__builtin_fmaf(score[s >> 1][8 * (s & 1) + 2 * i], unit, -m)),
-                                  __builtin_amdgcn_exp2f(__builtin_fmaf(score[s >> 1][8 * (s & 1) + 2 * i + 1], unit, -m))};
-                    pair[i] = __builtin_convertvector(p, h2);
-                    l = __builtin_amdgcn_fdot2(pair[i], h2{(half_t)1.f, (half_t)1.f}, l, false);
-                }
-                weight[s] = h8{pair[0][0], pair[0][1], pair[1][0], pair[1][1], pair[2][0], pair[2][1], pair[3][0], pair[3][1]};
-            }
-            // the next tile's scores: operands four reads ahead, each matrix instruction beside its share of this tile's weights
-            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-            for (int i = 0; i < 2 * kSteps; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x400, 32 / (2 * kSteps), 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 64 / (2 * kSteps), 0);
-            }
         }
         if (odd_keys) {  // the same for all waves
             // one key at a time, in the rows that see it; then zeros take the keys' place in LDS
             if (active) {
                 for (unsigned long long left = odd_keys; left; left &= left - 1) {
                     const int key = __builtin_ctzll(left);
-                    const int index = 4 * (key >> 4) + 2 * ((key >> 3) & 1) + ((key >> 1) & 1);  // of the pair of weights, in the half (key >> 2) & 1
-                    uint32_t pair = 0;
+                    const int index = 4 * (key >> 3) + (key & 3);  // of the scores, in the half (key >> 2) & 1
+                    float value = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) pair = i == index ? __builtin_bit_cast(u32x4, weight[i >> 2])[i & 3] : pair;
-                    pair = (uint32_t)__shfl((int)pair, col + 32 * ((key >> 2) & 1), 64);
-                    const float p = (float)bits_to_h2(pair)[key & 1];
+                    for (int i = 0; i < 32; ++i) value = i == index ? score[i >> 4][i & 15] : value;
+                    value = __shfl(value, col + 32 * ((key >> 2) & 1), 64);
+                    const float p = (float)(half_t)__builtin_amdgcn_exp2f(__builtin_fmaf(value, unit, -m));
                     if (key0 + key < seen && row_exists) {
 #pragma unroll
                         for (int i = 0; i < D; ++i)
@@ -265,31 +237,73 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
                 for (int i = 0; i < kPieces; ++i) *reinterpret_cast<u32x4*>(v_lds + lane * kRowBytes + i * 16) = u32x4{0u, 0u, 0u, 0u};
             __syncthreads();
         }
-        if (active) {
+        if (!active) return;
+        // Slots of one matrix instruction each, closed by scheduling barriers.  First the next tile's scores, operands four slots ahead,
+        // beside them this tile's weights, a pair or two a slot; then the second product, operands kAhead slots ahead.
+        constexpr int kFirst = 2 * kSteps, kSecond = 4 * D, kAhead = 3;
+        h8 keys[4];
+        s4 values[kAhead][2];
+        auto read_keys = [&](int i) __attribute__((always_inline)) { keys[i & 3] = keys_of(next_k_lds, i & 1, i >> 1); };
+        auto read_values = [&](int i) __attribute__((always_inline)) {
+            const int piece = ((4 * (i % D) + v_sub) ^ (2 * v_j)) * 16, at = (i / D) * 16;
+            values[i % kAhead][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(v_lds + v_read + piece + at * kRowBytes));
+            values[i % kAhead][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(v_lds + v_read + piece + (at + 8) * kRowBytes));
+        };
+        f2 power[2];
+        h2 pair[16];
+        auto raise = [&](int i) __attribute__((always_inline)) {
+            power[i & 1] = f2{__builtin_amdgcn_exp2f(__builtin_fmaf(score[i >> 3][2 * (i & 7)], unit, -m)),
+                              __builtin_amdgcn_exp2f(__builtin_fmaf(score[i >> 3][2 * (i & 7) + 1], unit, -m))};
+        };
+        auto round_pair = [&](int i) __attribute__((always_inline)) {
+            pair[i] = __builtin_convertvector(power[i & 1], h2);
+            l = __builtin_amdgcn_fdot2(pair[i], h2{(half_t)1.f, (half_t)1.f}, l, false);
+        };
+        next[0] = next[1] = f16{};
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
+        for (int i = 0; i < 4; ++i) read_keys(i);
+        __builtin_amdgcn_sched_barrier(0);
+        int raised = 0;
 #pragma unroll
-                for (int i = 0; i < D; ++i) {
-                    const int piece = ((4 * i + v_sub) ^ (2 * v_j)) * 16;
-                    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(v_lds + v_read + piece + s * 16 * kRowBytes));
-                    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(v_lds + v_read + piece + (s * 16 + 8) * kRowBytes));
-                    const h8 values = __builtin_bit_cast(h8, s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
-                    out[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(values, weight[s], out[i], 0, 0, 0);
-                }
+        for (int i = 0; i < kFirst; ++i) {
+            next[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys[i & 3], q[i >> 1], next[i & 1], 0, 0, 0);
+            if (i + 4 < kFirst) read_keys(i + 4);
+            else if (i + 4 - kFirst < kAhead) read_values(i + 4 - kFirst);
+#pragma unroll
+            for (; raised < 16 * (i + 1) / kFirst; ++raised) {
+                if (raised > 0) round_pair(raised - 1);
+                raise(raised);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        round_pair(15);
+#pragma unroll
+        for (int i = 0; i < kSecond; ++i) {
+            const int s = i / D;
+            const s4 lo = values[i % kAhead][0], hi = values[i % kAhead][1];
+            const h8 weight = {pair[4 * s][0], pair[4 * s][1], pair[4 * s + 1][0], pair[4 * s + 1][1],
+                               pair[4 * s + 2][0], pair[4 * s + 2][1], pair[4 * s + 3][0], pair[4 * s + 3][1]};
+            out[i % D] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}),
+                                                                weight, out[i % D], 0, 0, 0);
+            if (i + kAhead < kSecond) read_values(i + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     if (tiles > 0) {
         f16 even[2], odd[2];
-        fetch_k(0, 0);
-        fetch_v(0, 0);
-        if (tiles > 1) fetch_k(1, 1);
+        fetch_k(0, k_even);
+        fetch_v(0, v_even);
+        if (tiles > 1) fetch_k(1, k_odd);
         UNIQL_WAIT_ALL_LOADS();
         __syncthreads();
-        products(0, 0, even[0]);
-        products(0, 1, even[1]);
+        even[0] = even[1] = f16{};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) even[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys_of(k_even, k, i), q[i], even[k], 0, 0, 0);
         for (int t = 0; t < tiles; t += 2) {
-            step(t, even, odd);
-            if (t + 1 < tiles) step(t + 1, odd, even);
+            step(t, k_even, v_even, k_odd, v_odd, even, odd);
+            if (t + 1 < tiles) step(t + 1, k_odd, v_odd, k_even, v_even, odd, even);
         }
     }
     l += __shfl_xor(l, 32, 64);
@@ -316,8 +330,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
 
 template <int D, int WAVES, bool PIECES>
 static void go(const PromptArgs& a, hipStream_t stream) {
-    const unsigned lds = 4u * kKeys * (D == 2 ? 8 : 16) * 16;
-    hipLaunchKernelGGL((prompt_attention_kernel<D, WAVES, PIECES>), dim3((unsigned)(a.blocks * a.heads)), dim3(64 * WAVES), lds, stream, a);
+    hipLaunchKernelGGL((prompt_attention_kernel<D, WAVES, PIECES>), dim3((unsigned)(a.blocks * a.heads)), dim3(64 * WAVES), 0, stream, a);
 }
 template <int D>
 static void go(const PromptArgs& a, bool pieces, hipStream_t stream) {
