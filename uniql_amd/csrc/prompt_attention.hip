@@ -10,6 +10,7 @@
 // The maximum follows the scores only when a weight would pass 2^8 (weights are fp16, sums and outputs fp32): mostly once.
 // The rounding of the weights to fp16 (2^-11) is what a matrix instruction on fp16 asks for; their sum takes the rounded ones.
 #include "prompt_attention.hpp"
+#include <stdlib.h>
 
 namespace uniql {
 
@@ -21,6 +22,7 @@ typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
 typedef float f2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) s4* lds_s4_ptr;
 typedef _Float16 h4u __attribute__((ext_vector_type(4), aligned(2)));
 
@@ -39,14 +41,16 @@ __device__ __forceinline__ Rows rows_of(const PromptArgs& a, int s) {
     r.k_count = clamp_to(a.cu_k[s + 1], r.k_first, a.k_rows) - r.k_first;
     return r;
 }
-// The sequence and the block of rows in it that block `index` of all is; every wave finds it for itself.
-__device__ __forceinline__ bool find_block(const PromptArgs& a, int index, int block_rows, int& sequence, int& block) {
+// The sequence and the block of rows (of its queries times the heads of a key / value head) that block `index` of all is; every wave
+// finds it for itself.
+__device__ __forceinline__ bool find_block(const PromptArgs& a, int index, int block_rows, Rows& rows, int& block) {
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int base = 0; base < a.sequences; base += 64) {
         const int s = base + lane;
-        int mine = 0;
-        if (s < a.sequences) mine = (rows_of(a, s).q_count + block_rows - 1) / block_rows;
+        Rows r = {0, 0, 0, 0};
+        if (s < a.sequences) r = rows_of(a, s);
+        const int mine = (int)(((int64_t)r.q_count * a.group + block_rows - 1) / block_rows);
         int upto = mine;
         for (int d = 1; d < 64; d <<= 1) {
             const int other = __shfl_up(upto, d, 64);
@@ -55,70 +59,96 @@ __device__ __forceinline__ bool find_block(const PromptArgs& a, int index, int b
         const unsigned long long above = __ballot(before + upto > index);
         if (above) {
             const int owner = __builtin_ctzll(above);
-            sequence = __builtin_amdgcn_readfirstlane(base + owner);
-            block = __builtin_amdgcn_readfirstlane(index - before - __shfl(upto - mine, owner, 64));
+            rows.q_first = __builtin_amdgcn_readlane(r.q_first, owner);
+            rows.q_count = __builtin_amdgcn_readlane(r.q_count, owner);
+            rows.k_first = __builtin_amdgcn_readlane(r.k_first, owner);
+            rows.k_count = __builtin_amdgcn_readlane(r.k_count, owner);
+            block = index - before - __builtin_amdgcn_readlane(upto - mine, owner);
             return true;
         }
-        before += __shfl(upto, 63, 64);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
     return false;
 }
 
-// Eight values of a row from column j on; those past its width count as zeros.
-__device__ __forceinline__ h8 row_piece(const half_t* x, int j, int width) {
+// Eight values at any address that holds fp16 values.
+__device__ __forceinline__ h8 whole_piece(const half_t* x) {
     typedef _Float16 h8u __attribute__((ext_vector_type(8), aligned(2)));
-    if (j + 8 <= width) {
-        const h8u v = *reinterpret_cast<const h8u*>(x + j);
-        return h8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
-    }
-    h8 v = {};
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (j + i < width) v[i] = x[j + i];
-    return v;
+    const h8u v = *reinterpret_cast<const h8u*>(x);
+    return h8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
 }
 
-// D: the wider of the two head widths in units of 32, 2 to 4.  PIECES: rows of 16-byte pieces at multiples of 16 bytes, which go to LDS by
-// themselves; otherwise they pass through registers.
-template <int D, int WAVES, bool PIECES>
-__global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attention_kernel(const PromptArgs a) {
+// How K and V come to LDS: straight, rows in whole 16-byte pieces at multiples of 16 bytes; straight, rows of any even width at
+// multiples of 4 bytes, the last piece of K masked where it is read; or through registers.
+enum { kWhole = 0, kTail = 1, kThrough = 2 };
+
+// D: the wider of the two head widths in units of 32, 2 to 4.  GROUPS waves share a tile, 32 rows each; SPLIT such sets take every
+// SPLIT-th tile of the same rows and add up their results at the end.
+template <int D, int GROUPS, int SPLIT, int LOAD>
+__global__ __launch_bounds__(64 * GROUPS * SPLIT, LOAD == kThrough ? 1 : 2) void prompt_attention_kernel(const PromptArgs a) {
     constexpr int kSteps = 2 * D;                      // of 16 channels, of the first product
     constexpr int kPieces = D == 2 ? 8 : 16;           // 16-byte pieces of a row in LDS
     constexpr int kRowBytes = kPieces * 16;
     constexpr int kTileBytes = kKeys * kRowBytes;
     constexpr int kRowsAtOnce = 64 / kPieces;          // rows that a wave's access covers
-    constexpr int kAccesses = kKeys / (kRowsAtOnce * WAVES);
+    constexpr int kAccesses = kKeys / (kRowsAtOnce * GROUPS);
+    constexpr int kBlockRows = kQueries * GROUPS;
     // Two K tiles and two V tiles: variables of their own, which tells the compiler that reading one does not wait for what is on its way
     // into another.
-    __shared__ __attribute__((aligned(16))) char k_even[kTileBytes], k_odd[kTileBytes], v_even[kTileBytes], v_odd[kTileBytes];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
+    __shared__ __attribute__((aligned(16))) char k_even_all[SPLIT * kTileBytes], k_odd_all[SPLIT * kTileBytes], v_even_all[SPLIT * kTileBytes],
+        v_odd_all[SPLIT * kTileBytes];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
+    const int wave_of_all = __builtin_amdgcn_readfirstlane(tid >> 6), set = wave_of_all / GROUPS, wave = wave_of_all % GROUPS;
+    char *const k_even = k_even_all + set * kTileBytes, *const k_odd = k_odd_all + set * kTileBytes;
+    char *const v_even = v_even_all + set * kTileBytes, *const v_odd = v_odd_all + set * kTileBytes;
     // neighbouring workgroups have different key / value heads: those of one head stay on an XCD and share its L2
-    const unsigned kv_heads = (unsigned)(a.heads / a.group), kv_head = blockIdx.x % kv_heads, rest = blockIdx.x / kv_heads;
-    const int head = (int)(kv_head * a.group + rest % a.group);
+    const unsigned kv_heads = (unsigned)(a.heads / a.group);
+    const int kv_head = (int)(blockIdx.x % kv_heads);
     // later blocks see more keys: they come first
-    int sequence, block;
-    if (!find_block(a, (int)(a.blocks - 1 - rest / a.group), kQueries * WAVES, sequence, block)) return;
-    const Rows r = rows_of(a, sequence);
-    const int offset = r.k_count - r.q_count;
-    const int row0 = block * kQueries * WAVES + wave * kQueries, row = row0 + col;
-    const bool row_exists = row < r.q_count;
-    const int seen = a.causal ? clamp_to(row + offset + 1, 0, r.k_count) : r.k_count;  // keys of the lane's row
-    // of the wave's first row and of its last, and of the workgroup's last
-    const int last_row = clamp_to(row0 + kQueries - 1, 0, r.q_count - 1), block_last = clamp_to((block + 1) * kQueries * WAVES - 1, 0, r.q_count - 1);
-    const int fewest = a.causal ? clamp_to(row0 + offset + 1, 0, r.k_count) : r.k_count;
-    const int most = row0 < r.q_count ? (a.causal ? clamp_to(last_row + offset + 1, 0, r.k_count) : r.k_count) : 0;
-    const int block_most = a.causal ? clamp_to(block_last + offset + 1, 0, r.k_count) : r.k_count;
-    const int block_fewest = a.causal ? clamp_to(block * kQueries * WAVES + offset + 1, 0, r.k_count) : r.k_count;
+    Rows r;
+    int block;
+    if (!find_block(a, (int)(a.blocks - 1 - blockIdx.x / kv_heads), kBlockRows, r, block)) return;
+    // Rows are a sequence's queries times the query heads that share the key / value head, one query's heads side by side: short
+    // sequences fill a tile of rows, and the rows of a tile see almost the same keys.
+    const int offset = r.k_count - r.q_count, rows = r.q_count * a.group;
+    auto seen_by = [&](int row) __attribute__((always_inline)) { return a.causal ? clamp_to(row / a.group + offset + 1, 0, r.k_count) : r.k_count; };
+    auto uniform = [](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(v); };
+    const int row0 = block * kBlockRows + wave * kQueries, row = row0 + col;
+    const int seen = seen_by(row);  // keys of the lane's row
+    // of the wave's first row and of its last, and of the workgroup's
+    const int last_row = rows - 1, fewest = uniform(seen_by(row0));
+    const int most = row0 < rows ? uniform(seen_by(row0 + kQueries - 1 < last_row ? row0 + kQueries - 1 : last_row)) : 0;
+    const int block_end = (block + 1) * kBlockRows - 1, block_most = uniform(seen_by(block_end < last_row ? block_end : last_row));
+    const int block_fewest = uniform(seen_by(block * kBlockRows));
     const int tiles = (block_most + kKeys - 1) / kKeys;
 
+    // With a width that is no multiple of eight the last two pieces that K has change places with the last two that LDS has, so that the
+    // last step reads them.
+    const int tail_pair = LOAD == kTail && (a.k_dim >> 4) < kSteps ? a.k_dim >> 4 : kSteps - 1;
+    auto moved = [&](int pair) __attribute__((always_inline)) {
+        return LOAD == kTail ? (pair == kSteps - 1 ? tail_pair : (pair == tail_pair ? kSteps - 1 : pair)) : pair;
+    };
     h8 q[kSteps];
+    const bool row_exists = row < rows;
     {
-        const half_t* from = a.q + (int64_t)(r.q_first + (row_exists ? row : 0)) * a.q_row + (int64_t)head * a.q_head;
+        const int token = row_exists ? row / a.group : 0, head = kv_head * a.group + (row_exists ? row - token * a.group : 0);
+        const half_t* from = a.q + (int64_t)(r.q_first + token) * a.q_row + (int64_t)head * a.q_head;
+        // whole pieces, then the one that is not whole
+        const int partial = a.k_dim >> 3;
+        h8 rest = {};
+        if (row_exists && (partial & 1) == half)
+            for (int j = 0; j < (a.k_dim & 7); ++j) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e == j) rest[e] = from[8 * partial + j];
+            }
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
+            const int piece = 2 * moved(i) + half;
             q[i] = h8{};
-            if (row_exists && a.q_sign != 0) q[i] = row_piece(from, 16 * i + 8 * half, a.k_dim);
-            if (a.q_sign < 0) q[i] = -q[i];
+            if (row_exists && piece < partial) q[i] = whole_piece(from + 8 * piece);
+            if (piece == partial) q[i] = rest;
+            if (a.q_sign <= 0) q[i] = a.q_sign < 0 ? -q[i] : h8{};
         }
     }
     f16 out[D];
@@ -131,31 +161,50 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
     const half_t* const v_base = a.v + (int64_t)r.k_first * a.v_row + (int64_t)kv_head * a.v_head;
     // this lane's part of an access: a row of the tile and a piece of it
     const int part_row = wave * kRowsAtOnce + lane / kPieces, part = lane % kPieces;
-    const int k_piece = part ^ (part_row & (kPieces - 1)), v_piece = part ^ (2 * (part_row & 3));
     // Rows behind the sequence lie beyond the descriptor and come as zeros, and so do pieces behind the width.
-    auto fetch = [&](const half_t* base, int64_t stride, int width, int piece, int tile, char* to) __attribute__((always_inline)) {
-        const int key0 = tile * kKeys, left = r.k_count - key0 < kKeys ? r.k_count - key0 : kKeys;
-        if constexpr (PIECES) {
-            const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<half_t*>(base + (int64_t)key0 * stride), 0,
-                                                                                  (unsigned)(((int64_t)(left - 1) * stride + width) * 2), 0x00020000);
+    auto fetch = [&](const half_t* tile, unsigned stride, int width, bool keys, int left, char* to) __attribute__((always_inline)) {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<half_t*>(tile), 0, 2u * ((unsigned)((left < kKeys ? left : kKeys) - 1) * stride + (unsigned)width), 0x00020000);
 #pragma unroll
-            for (int i = 0; i < kAccesses; ++i) {
-                const int at = i * kRowsAtOnce * WAVES;  // a multiple of 16 rows: the exchange of pieces is the same
-                const unsigned off = piece * 8 < width ? 2u * ((unsigned)(at + part_row) * (unsigned)stride) + 16u * piece : 0xfffffff0u;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(to + (at + wave * kRowsAtOnce) * kRowBytes), 16, off, 0, 0, 0);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kAccesses; ++i) {
-                const int at = i * kRowsAtOnce * WAVES + part_row;
+        for (int i = 0; i < kAccesses; ++i) {
+            const int at = i * kRowsAtOnce * GROUPS, row = at + part_row;
+            int piece = keys ? part ^ (row & (kPieces - 1)) : part ^ (2 * (row & 3));
+            if (keys) piece = 2 * moved(piece >> 1) + (piece & 1);
+            if constexpr (LOAD == kThrough) {
+                // (value by value in the last piece of a row; these layouts are for other callers than the fused projection)
                 h8 v = {};
-                if (at < left) v = row_piece(base + (int64_t)(key0 + at) * stride, 8 * piece, width);
-                *reinterpret_cast<h8*>(to + at * kRowBytes + part * 16) = v;
+                if (row < left) {
+                    const half_t* const from = tile + (int64_t)row * (keys ? a.k_row : a.v_row) + 8 * piece;
+                    if (8 * piece + 8 <= width) v = whole_piece(from);
+                    else
+                        for (int j = 0; 8 * piece + j < width; ++j) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (e == j) v[e] = from[j];
+                        }
+                }
+                *reinterpret_cast<h8*>(to + row * kRowBytes + part * 16) = v;
+            } else {
+                const unsigned first = piece * 8 < width ? 2u * ((unsigned)part_row * stride) + 16u * piece : 0x80000000u;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(to + (at + wave * kRowsAtOnce) * kRowBytes), 16,
+                                                         first + 2u * (unsigned)at * stride, 0, 0, 0);
             }
         }
     };
-    auto fetch_k = [&](int tile, char* to) __attribute__((always_inline)) { fetch(k_base, a.k_row, a.k_dim, k_piece, tile, to); };
-    auto fetch_v = [&](int tile, char* to) __attribute__((always_inline)) { fetch(v_base, a.v_row, a.v_dim, v_piece, tile, to); };
+    // Tile t of this set.  The tiles come one after the other, K and V each.
+    auto key_of = [&](int t) __attribute__((always_inline)) { return (t * SPLIT + set) * kKeys; };
+    const half_t *k_tile = k_base + (int64_t)key_of(0) * a.k_row, *v_tile = v_base + (int64_t)key_of(0) * a.v_row;
+    const int64_t k_ahead = (int64_t)(SPLIT * kKeys) * a.k_row, v_ahead = (int64_t)(SPLIT * kKeys) * a.v_row;
+    auto fetch_k = [&](int t, char* to) __attribute__((always_inline)) {
+        if (t * SPLIT + set >= tiles) return;
+        fetch(k_tile, (unsigned)a.k_row, a.k_dim, true, r.k_count - key_of(t), to);
+        k_tile += k_ahead;
+    };
+    auto fetch_v = [&](int t, char* to) __attribute__((always_inline)) {
+        if (t * SPLIT + set >= tiles) return;
+        fetch(v_tile, (unsigned)a.v_row, a.v_dim, false, r.k_count - key_of(t), to);
+        v_tile += v_ahead;
+    };
     // where the lane reads: K rows col and 32 + col, piece 2 step + half; V rows 4 half + j (+ 8), j = (lane / 4) % 4, four channels
     const int k_read = col * kRowBytes, k_swap = col & (kPieces - 1);
     const int v_j = (lane >> 2) & 3, v_read = (4 * half + v_j) * kRowBytes + (lane & 1) * 8;
@@ -163,18 +212,30 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
     auto keys_of = [&](const char* tile, int k, int i) __attribute__((always_inline)) {
         return *reinterpret_cast<const h8*>(tile + k_read + k * 32 * kRowBytes + (((2 * i + half) ^ k_swap) * 16));
     };
+    // what the last step's piece holds of the width, two values a word; the rest of it is another head's
+    uint32_t inside[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) inside[j] = 16 * tail_pair + 8 * half + 2 * j < a.k_dim ? 0xffffffffu : 0u;
+    auto product = [&](h8 keys, int i, const f16& sum) __attribute__((always_inline)) {
+        if (LOAD == kTail && i == kSteps - 1) {
+            const u32x4 w = __builtin_bit_cast(u32x4, keys);
+            keys = __builtin_bit_cast(h8, u32x4{w[0] & inside[0], w[1] & inside[1], w[2] & inside[2], w[3] & inside[3]});
+        }
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(keys, q[i], sum, 0, 0, 0);
+    };
     // A step: the weights of tile t from its scores, which the step before has computed, the next tile's scores, the second product.
     auto step = [&](int t, char* k_lds, char* v_lds, char* next_k_lds, char* next_v_lds, f16 (&score)[2], f16 (&next)[2]) __attribute__((always_inline)) {
-        const int key0 = t * kKeys;
+        const int key0 = key_of(t);
         UNIQL_WAIT_ALL_LOADS();
         __syncthreads();
-        if (t + 2 < tiles) fetch_k(t + 2, k_lds);
-        if (t + 1 < tiles) fetch_v(t + 1, next_v_lds);
+        fetch_k(t + 2, k_lds);
+        fetch_v(t + 1, next_v_lds);
         const bool masked = key0 + kKeys > fewest;
-        // A key that some rows of the tile see and others do not: its weight is zero for those, but zero times an infinity is not.  Keys
-        // with such values are found first and taken out of the product, see below; each lane looks at one key.
+        // A key that some rows of the tile see and others do not: its weight is zero for those, but zero times an infinity is not.  Where
+        // the workgroup has such keys each lane looks at one; those with such values become zeros in LDS, and what they give to the rows that
+        // see them is added on its own, below.
         unsigned long long odd_keys = 0;
-        if (a.causal && key0 + kKeys > block_fewest) {
+        if (a.causal && (t + 1) * SPLIT * kKeys > block_fewest) {  // the same for all waves
             uint32_t any = 0;
 #pragma unroll 4
             for (int i = 0; i < kPieces; ++i) {
@@ -182,7 +243,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
 #pragma unroll
                 for (int j = 0; j < 4; ++j) any |= ((w[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;  // an exponent of all ones runs over
             }
-            odd_keys = __ballot(any != 0);
+            odd_keys = key0 < block_most ? __ballot(any != 0) : 0ull;
+            __syncthreads();
+            if ((odd_keys >> lane) & 1)
+                for (int i = 0; i < kPieces; ++i) *reinterpret_cast<u32x4*>(v_lds + lane * kRowBytes + i * 16) = u32x4{0u, 0u, 0u, 0u};
         }
         const bool active = key0 < most;  // the wave's rows see some of the keys (all waves take part in the barriers)
         if (active) {
@@ -208,35 +272,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
                 for (int i = 0; i < D; ++i) out[i] *= fade;
             }
         }
-        if (odd_keys) {  // the same for all waves
-            // one key at a time, in the rows that see it; then zeros take the keys' place in LDS
-            if (active) {
-                for (unsigned long long left = odd_keys; left; left &= left - 1) {
-                    const int key = __builtin_ctzll(left);
-                    const int index = 4 * (key >> 3) + (key & 3);  // of the scores, in the half (key >> 2) & 1
-                    float value = 0.f;
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) value = i == index ? score[i >> 4][i & 15] : value;
-                    value = __shfl(value, col + 32 * ((key >> 2) & 1), 64);
-                    const float p = (float)(half_t)__builtin_amdgcn_exp2f(__builtin_fmaf(value, unit, -m));
-                    if (key0 + key < seen && row_exists) {
-#pragma unroll
-                        for (int i = 0; i < D; ++i)
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                const int channel = 32 * i + 8 * (j / 4) + 4 * half + j % 4;
-                                const half_t v = *reinterpret_cast<const half_t*>(v_lds + key * kRowBytes +
-                                                                                  ((channel >> 3) ^ (2 * (key & 3))) * 16 + (channel & 7) * 2);
-                                out[i][j] += p * (float)v;
-                            }
-                    }
-                }
-            }
-            __syncthreads();
-            if (wave == 0 && ((odd_keys >> lane) & 1))
-                for (int i = 0; i < kPieces; ++i) *reinterpret_cast<u32x4*>(v_lds + lane * kRowBytes + i * 16) = u32x4{0u, 0u, 0u, 0u};
-            __syncthreads();
-        }
         if (!active) return;
         // Slots of one matrix instruction each, closed by scheduling barriers.  First the next tile's scores, operands four slots ahead,
         // beside them this tile's weights, a pair or two a slot; then the second product, operands kAhead slots ahead.
@@ -250,14 +285,15 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
             values[i % kAhead][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4_ptr)(v_lds + v_read + piece + (at + 8) * kRowBytes));
         };
         f2 power[2];
-        h2 pair[16];
+        u32x16 pair = {};
         auto raise = [&](int i) __attribute__((always_inline)) {
             power[i & 1] = f2{__builtin_amdgcn_exp2f(__builtin_fmaf(score[i >> 3][2 * (i & 7)], unit, -m)),
                               __builtin_amdgcn_exp2f(__builtin_fmaf(score[i >> 3][2 * (i & 7) + 1], unit, -m))};
         };
         auto round_pair = [&](int i) __attribute__((always_inline)) {
-            pair[i] = __builtin_convertvector(power[i & 1], h2);
-            l = __builtin_amdgcn_fdot2(pair[i], h2{(half_t)1.f, (half_t)1.f}, l, false);
+            const h2 both = __builtin_convertvector(power[i & 1], h2);
+            pair[i] = h2_to_bits(both);
+            l = __builtin_amdgcn_fdot2(both, h2{(half_t)1.f, (half_t)1.f}, l, false);
         };
         next[0] = next[1] = f16{};
 #pragma unroll
@@ -266,7 +302,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
         int raised = 0;
 #pragma unroll
         for (int i = 0; i < kFirst; ++i) {
-            next[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys[i & 3], q[i >> 1], next[i & 1], 0, 0, 0);
+            next[i & 1] = product(keys[i & 3], i >> 1, next[i & 1]);
             if (i + 4 < kFirst) read_keys(i + 4);
             else if (i + 4 - kFirst < kAhead) read_values(i + 4 - kFirst);
 #pragma unroll
@@ -281,34 +317,89 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
         for (int i = 0; i < kSecond; ++i) {
             const int s = i / D;
             const s4 lo = values[i % kAhead][0], hi = values[i % kAhead][1];
-            const h8 weight = {pair[4 * s][0], pair[4 * s][1], pair[4 * s + 1][0], pair[4 * s + 1][1],
-                               pair[4 * s + 2][0], pair[4 * s + 2][1], pair[4 * s + 3][0], pair[4 * s + 3][1]};
+            const h8 weight = __builtin_bit_cast(h8, u32x4{pair[4 * s], pair[4 * s + 1], pair[4 * s + 2], pair[4 * s + 3]});
             out[i % D] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, s8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}),
                                                                 weight, out[i % D], 0, 0, 0);
             if (i + kAhead < kSecond) read_values(i + kAhead);
             __builtin_amdgcn_sched_barrier(0);
         }
+        if (odd_keys) {
+            for (unsigned long long left = odd_keys; left; left &= left - 1) {
+                const int key = __builtin_ctzll(left);
+                const int index = 4 * (key >> 4) + 2 * ((key >> 3) & 1) + ((key >> 1) & 1);  // of the pair of weights, in the half (key >> 2) & 1
+                uint32_t both = 0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t other = pair[i];
+                    both = i == index ? other : both;
+                    asm volatile("" : "+v"(both));  // or the weights become an array in memory
+                }
+                both = (uint32_t)__shfl((int)both, col + 32 * ((key >> 2) & 1), 64);
+                const float p = (float)bits_to_h2(both)[key & 1];
+                // (columns behind the width are beyond the descriptor)
+                const __amdgpu_buffer_rsrc_t v = __builtin_amdgcn_make_buffer_rsrc(const_cast<half_t*>(v_base + (int64_t)(key0 + key) * a.v_row), 0,
+                                                                                   2u * (unsigned)a.v_dim, 0x00020000);
+                if (key0 + key < seen) {
+#pragma unroll
+                    for (int i = 0; i < D; ++i)
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            out[i][j] += p * (float)__builtin_bit_cast(half_t, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(
+                                                                                   v, 8 * half, 2 * (32 * i + 8 * (j / 4) + j % 4), 0));
+                }
+            }
+        }
     };
-    if (tiles > 0) {
+    const int rounds = (tiles + SPLIT - 1) / SPLIT;
+    if (rounds > 0) {
         f16 even[2], odd[2];
         fetch_k(0, k_even);
         fetch_v(0, v_even);
-        if (tiles > 1) fetch_k(1, k_odd);
+        fetch_k(1, k_odd);
         UNIQL_WAIT_ALL_LOADS();
         __syncthreads();
         even[0] = even[1] = f16{};
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) even[k] = __builtin_amdgcn_mfma_f32_32x32x16_f16(keys_of(k_even, k, i), q[i], even[k], 0, 0, 0);
-        for (int t = 0; t < tiles; t += 2) {
+            for (int k = 0; k < 2; ++k) even[k] = product(keys_of(k_even, k, i), i, even[k]);
+        for (int t = 0; t < rounds; t += 2) {
             step(t, k_even, v_even, k_odd, v_odd, even, odd);
-            if (t + 1 < tiles) step(t + 1, k_odd, v_odd, k_even, v_even, odd, even);
+            if (t + 1 < rounds) step(t + 1, k_odd, v_odd, k_even, v_even, odd, even);
         }
     }
     l += __shfl_xor(l, 32, 64);
-    if (!row_exists) return;
-    half_t* to = a.out + (int64_t)(r.q_first + row) * a.out_row + (int64_t)head * a.out_head;
+    if constexpr (SPLIT == 2) {
+        // the second set's results go through LDS, 16 KiB a wave: half of them in each of the two K tiles' and V tiles' places
+        constexpr int kPart = 8 * D;  // values of a lane
+        float* const place[2] = {reinterpret_cast<float*>(k_even_all), reinterpret_cast<float*>(v_even_all)};
+        float* const extra = reinterpret_cast<float*>(k_odd_all);
+        static_assert(GROUPS * kPart * 64 * 4 <= SPLIT * kTileBytes, "the results fit the tiles' places");
+        __syncthreads();
+        if (set == 1) {
+#pragma unroll
+            for (int i = 0; i < D; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) place[(16 * i + j) / kPart][(wave * kPart + (16 * i + j) % kPart) * 64 + lane] = out[i][j];
+            extra[wave * 128 + lane] = m;
+            extra[wave * 128 + 64 + lane] = l;
+        }
+        __syncthreads();
+        if (set == 1) return;
+        const float other = extra[wave * 128 + lane], other_l = extra[wave * 128 + 64 + lane];
+        const float higher = fmaxf(m, other), keep = __builtin_amdgcn_exp2f(m - higher), add = __builtin_amdgcn_exp2f(other - higher);
+        l = l * keep + other_l * add;
+#pragma unroll
+        for (int i = 0; i < D; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                out[i][j] = out[i][j] * keep + place[(16 * i + j) / kPart][(wave * kPart + (16 * i + j) % kPart) * 64 + lane] * add;
+    }
+    int my_row = row;
+    asm volatile("" : "+v"(my_row));  // the quotient is not kept over the loop
+    if (my_row >= rows) return;
+    const int token = my_row / a.group, head = kv_head * a.group + my_row - token * a.group;
+    half_t* to = a.out + (int64_t)(r.q_first + token) * a.out_row + (int64_t)head * a.out_head;
     const float inverse = seen > 0 ? 1.0f / l : 0.f;
 #pragma unroll
     for (int i = 0; i < D; ++i)
@@ -328,33 +419,48 @@ __global__ __launch_bounds__(64 * WAVES, WAVES == 8 ? 1 : 2) void prompt_attenti
         }
 }
 
-template <int D, int WAVES, bool PIECES>
+template <int D, int GROUPS, int SPLIT, int LOAD>
 static void go(const PromptArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL((prompt_attention_kernel<D, WAVES, PIECES>), dim3((unsigned)(a.blocks * a.heads)), dim3(64 * WAVES), 0, stream, a);
+    hipLaunchKernelGGL((prompt_attention_kernel<D, GROUPS, SPLIT, LOAD>), dim3((unsigned)(a.blocks * (a.heads / a.group))), dim3(64 * GROUPS * SPLIT), 0,
+                       stream, a);
+}
+template <int D, int LOAD>
+static void go(const PromptArgs& a, int shape, hipStream_t stream) {
+    if (shape == 0) go<D, 4, 1, LOAD>(a, stream);
+    else if (shape == 1) go<D, 4, 2, LOAD>(a, stream);
+    else go<D, 2, 2, LOAD>(a, stream);
 }
 template <int D>
-static void go(const PromptArgs& a, bool pieces, hipStream_t stream) {
-    if (pieces) go<D, 4, true>(a, stream);
-    else go<D, 4, false>(a, stream);
+static void go(const PromptArgs& a, int shape, int load, hipStream_t stream) {
+    if (load == kWhole) go<D, kWhole>(a, shape, stream);
+    else if (load == kTail) go<D, kTail>(a, shape, stream);
+    else go<D, 4, 1, kThrough>(a, stream);
+}
+
+static int prompt_shape(const PromptArgs& a) {
+    if (const char* e = getenv("UNIQL_SHAPE")) return atoi(e);
+    return 0;
 }
 
 int prompt_attention_launch(const PromptArgs& args, hipStream_t stream) {
     PromptArgs a = args;
     a.q_sign = a.scale == 0.f ? 0 : (a.scale < 0.f ? -1 : 1);
     a.scale = a.q_sign == 0 ? 1.0f : (a.scale < 0.f ? -a.scale : a.scale);
-    const int waves = 4;
-    const int64_t blocks = (int64_t)a.rows / (kQueries * waves) + (a.sequences < a.rows ? a.sequences : a.rows);
-    if (blocks * a.heads > 0x7fffffffLL) return UNIQL_E_SHAPE;
-    a.blocks = (int)blocks;
-    // 64 rows of K or V stay below 2^32 bytes
-    const int64_t far = 1LL << 25;
+    // 64 rows of K or V stay below 2^31 bytes
+    const int64_t far = 1LL << 24, strides = a.k_row | a.k_head | a.v_row | a.v_head | a.k_dim | a.v_dim;
     const uintptr_t bases = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v);
-    const bool pieces = ((a.k_row | a.k_head | a.v_row | a.v_head | a.k_dim | a.v_dim) & 7) == 0 && (bases & 15) == 0 && a.k_row >= 0 &&
-                        a.v_row >= 0 && a.k_row <= far && a.v_row <= far;
+    const bool near = a.k_row >= a.k_dim && a.v_row >= a.v_dim && a.k_row <= far && a.v_row <= far;
+    const int load = near && (strides & 7) == 0 && (bases & 15) == 0 ? kWhole
+                     : near && (strides & 1) == 0 && (bases & 3) == 0 && a.k_row >= 8 && a.v_row >= 8 ? kTail : kThrough;
+    const int shape = load == kThrough ? 0 : prompt_shape(a);
+    const int block_rows = kQueries * (shape == 2 ? 2 : 4);
+    const int64_t rows = (int64_t)a.rows * a.group, blocks = rows / block_rows + (a.sequences < a.rows ? a.sequences : a.rows);
+    if (rows > (1LL << 30) || blocks * (a.heads / a.group) > 0x7fffffffLL) return UNIQL_E_SHAPE;
+    a.blocks = (int)blocks;
     const int width = ((a.k_dim > a.v_dim ? a.k_dim : a.v_dim) + 31) / 32;
-    if (width <= 2) go<2>(a, pieces, stream);
-    else if (width == 3) go<3>(a, pieces, stream);
-    else go<4>(a, pieces, stream);
+    if (width <= 2) go<2>(a, shape, load, stream);
+    else if (width == 3) go<3>(a, shape, load, stream);
+    else go<4>(a, shape, load, stream);
     return hipGetLastError() == hipSuccess ? UNIQL_OK : UNIQL_E_LAUNCH;
 }
 
