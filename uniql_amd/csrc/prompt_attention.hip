@@ -10,12 +10,13 @@
 // The maximum follows the scores only when a weight would pass 2^8 (weights are fp16, sums and outputs fp32): mostly once.
 // The rounding of the weights to fp16 (2^-11) is what a matrix instruction on fp16 asks for; their sum takes the rounded ones.
 #include "prompt_attention.hpp"
-#include <stdlib.h>
 
 namespace uniql {
 
 constexpr int kKeys = 64;               // keys of a step
 constexpr int kQueries = 32;            // rows of a wave
+constexpr int kWaves = 4;
+constexpr int kBlockRows = kWaves * kQueries;
 constexpr float kLowest = -3.0e38f;
 constexpr float kRoom = 8.0f;           // weights may grow to 2^8 before the maximum follows
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -24,7 +25,7 @@ typedef short s8 __attribute__((ext_vector_type(8)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) s4* lds_s4_ptr;
-typedef _Float16 h4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef _Float16 h8u __attribute__((ext_vector_type(8), aligned(2)));
 
 #define UNIQL_WAIT_ALL_LOADS() __builtin_amdgcn_s_waitcnt(0x0F70)  // vmcnt(0), the other counters left alone (gfx9 encoding)
 
@@ -41,9 +42,29 @@ __device__ __forceinline__ Rows rows_of(const PromptArgs& a, int s) {
     r.k_count = clamp_to(a.cu_k[s + 1], r.k_first, a.k_rows) - r.k_first;
     return r;
 }
+// Sums over the lanes up to and including each.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int add_from(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int sums_upto(int v) {
+    v = add_from<0x111, 0xf>(v);  // one, two, four, eight lanes below, within sixteen
+    v = add_from<0x112, 0xf>(v);
+    v = add_from<0x114, 0xf>(v);
+    v = add_from<0x118, 0xf>(v);
+    v = add_from<0x142, 0xa>(v);  // the last of the sixteen below, for the second and fourth sixteen
+    return add_from<0x143, 0xc>(v);  // lane 31, for the upper half
+}
+
+// row / a.group for rows below 2^30 (see the launch)
+__device__ __forceinline__ int query_of(const PromptArgs& a, int row) { return (int)(((uint64_t)(unsigned)row * a.group_factor) >> a.group_shift); }
+
 // The sequence and the block of rows (of its queries times the heads of a key / value head) that block `index` of all is; every wave
 // finds it for itself.
 __device__ __forceinline__ bool find_block(const PromptArgs& a, int index, int block_rows, Rows& rows, int& block) {
+    if (a.sequences == 1) {
+        rows = rows_of(a, 0);
+        block = index;
+        return (int64_t)index * block_rows < (int64_t)rows.q_count * a.group;
+    }
     const int lane = threadIdx.x & 63;
     int before = 0;
     for (int base = 0; base < a.sequences; base += 64) {
@@ -51,11 +72,7 @@ __device__ __forceinline__ bool find_block(const PromptArgs& a, int index, int b
         Rows r = {0, 0, 0, 0};
         if (s < a.sequences) r = rows_of(a, s);
         const int mine = (int)(((int64_t)r.q_count * a.group + block_rows - 1) / block_rows);
-        int upto = mine;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int other = __shfl_up(upto, d, 64);
-            if (lane >= d) upto += other;
-        }
+        const int upto = sums_upto(mine);
         const unsigned long long above = __ballot(before + upto > index);
         if (above) {
             const int owner = __builtin_ctzll(above);
@@ -73,7 +90,6 @@ __device__ __forceinline__ bool find_block(const PromptArgs& a, int index, int b
 
 // Eight values at any address that holds fp16 values.
 __device__ __forceinline__ h8 whole_piece(const half_t* x) {
-    typedef _Float16 h8u __attribute__((ext_vector_type(8), aligned(2)));
     const h8u v = *reinterpret_cast<const h8u*>(x);
     return h8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
 }
@@ -82,25 +98,20 @@ __device__ __forceinline__ h8 whole_piece(const half_t* x) {
 // multiples of 4 bytes, the last piece of K masked where it is read; or through registers.
 enum { kWhole = 0, kTail = 1, kThrough = 2 };
 
-// D: the wider of the two head widths in units of 32, 2 to 4.  GROUPS waves share a tile, 32 rows each; SPLIT such sets take every
-// SPLIT-th tile of the same rows and add up their results at the end.
-template <int D, int GROUPS, int SPLIT, int LOAD>
-__global__ __launch_bounds__(64 * GROUPS * SPLIT, LOAD == kThrough ? 1 : 2) void prompt_attention_kernel(const PromptArgs a) {
+// D: the wider of the two head widths in units of 32, 2 to 4.
+template <int D, int LOAD>
+__global__ __launch_bounds__(64 * kWaves, LOAD == kThrough ? 1 : 2) void prompt_attention_kernel(const PromptArgs a) {
     constexpr int kSteps = 2 * D;                      // of 16 channels, of the first product
     constexpr int kPieces = D == 2 ? 8 : 16;           // 16-byte pieces of a row in LDS
     constexpr int kRowBytes = kPieces * 16;
     constexpr int kTileBytes = kKeys * kRowBytes;
     constexpr int kRowsAtOnce = 64 / kPieces;          // rows that a wave's access covers
-    constexpr int kAccesses = kKeys / (kRowsAtOnce * GROUPS);
-    constexpr int kBlockRows = kQueries * GROUPS;
+    constexpr int kAccesses = kKeys / (kRowsAtOnce * kWaves);
     // Two K tiles and two V tiles: variables of their own, which tells the compiler that reading one does not wait for what is on its way
     // into another.
-    __shared__ __attribute__((aligned(16))) char k_even_all[SPLIT * kTileBytes], k_odd_all[SPLIT * kTileBytes], v_even_all[SPLIT * kTileBytes],
-        v_odd_all[SPLIT * kTileBytes];
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
-    const int wave_of_all = __builtin_amdgcn_readfirstlane(tid >> 6), set = wave_of_all / GROUPS, wave = wave_of_all % GROUPS;
-    char *const k_even = k_even_all + set * kTileBytes, *const k_odd = k_odd_all + set * kTileBytes;
-    char *const v_even = v_even_all + set * kTileBytes, *const v_odd = v_odd_all + set * kTileBytes;
+    __shared__ __attribute__((aligned(16))) char k_even[kTileBytes], k_odd[kTileBytes], v_even[kTileBytes], v_odd[kTileBytes];
+    __shared__ int spoilt[kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // neighbouring workgroups have different key / value heads: those of one head stay on an XCD and share its L2
     const unsigned kv_heads = (unsigned)(a.heads / a.group);
     const int kv_head = (int)(blockIdx.x % kv_heads);
@@ -111,15 +122,14 @@ __global__ __launch_bounds__(64 * GROUPS * SPLIT, LOAD == kThrough ? 1 : 2) void
     // Rows are a sequence's queries times the query heads that share the key / value head, one query's heads side by side: short
     // sequences fill a tile of rows, and the rows of a tile see almost the same keys.
     const int offset = r.k_count - r.q_count, rows = r.q_count * a.group;
-    auto seen_by = [&](int row) __attribute__((always_inline)) { return a.causal ? clamp_to(row / a.group + offset + 1, 0, r.k_count) : r.k_count; };
-    auto uniform = [](int v) __attribute__((always_inline)) { return __builtin_amdgcn_readfirstlane(v); };
+    auto seen_by = [&](int row) __attribute__((always_inline)) { return a.causal ? clamp_to(query_of(a, row) + offset + 1, 0, r.k_count) : r.k_count; };
     const int row0 = block * kBlockRows + wave * kQueries, row = row0 + col;
     const int seen = seen_by(row);  // keys of the lane's row
     // of the wave's first row and of its last, and of the workgroup's
-    const int last_row = rows - 1, fewest = uniform(seen_by(row0));
-    const int most = row0 < rows ? uniform(seen_by(row0 + kQueries - 1 < last_row ? row0 + kQueries - 1 : last_row)) : 0;
-    const int block_end = (block + 1) * kBlockRows - 1, block_most = uniform(seen_by(block_end < last_row ? block_end : last_row));
-    const int block_fewest = uniform(seen_by(block * kBlockRows));
+    const int last_row = rows - 1, fewest = seen_by(row0);
+    const int most = row0 < rows ? seen_by(row0 + kQueries - 1 < last_row ? row0 + kQueries - 1 : last_row) : 0;
+    const int block_end = (block + 1) * kBlockRows - 1, block_most = seen_by(block_end < last_row ? block_end : last_row);
+    const int block_fewest = seen_by(block * kBlockRows);
     const int tiles = (block_most + kKeys - 1) / kKeys;
 
     // With a width that is no multiple of eight the last two pieces that K has change places with the last two that LDS has, so that the
@@ -128,10 +138,75 @@ __global__ __launch_bounds__(64 * GROUPS * SPLIT, LOAD == kThrough ? 1 : 2) void
     auto moved = [&](int pair) __attribute__((always_inline)) {
         return LOAD == kTail ? (pair == kSteps - 1 ? tail_pair : (pair == tail_pair ? kSteps - 1 : pair)) : pair;
     };
+    bool careful = false;
+    const float unit = a.scale * 1.4426950408889634f;  // positive: a negative scale has turned q
+
+    const half_t* const k_base = a.k + (int64_t)r.k_first * a.k_row + (int64_t)kv_head * a.k_head;
+    const half_t* const v_base = a.v + (int64_t)r.k_first * a.v_row + (int64_t)kv_head * a.v_head;
+    // this lane's part of an access: a row of the tile and a piece of it
+    const int part_row = wave * kRowsAtOnce + lane / kPieces, part = lane % kPieces;
+    // Rows behind the sequence lie beyond the descriptor and come as zeros, and so do pieces behind the width.
+    auto fetch = [&](const half_t* tile, unsigned stride, int width, bool keys, int left, char* to) __attribute__((always_inline)) {
+        auto piece_of = [&](int row) __attribute__((always_inline)) {
+            if (!keys) return part ^ (2 * (row & 3));
+            const int piece = part ^ (row & (kPieces - 1));
+            return 2 * moved(piece >> 1) + (piece & 1);
+        };
+        if constexpr (LOAD == kThrough) {
+            // (value by value in the last piece of a row; these layouts are for other callers than the fused projection)
+#pragma unroll 1
+            for (int row = part_row; row < kKeys; row += kRowsAtOnce * kWaves) {
+                const int piece = piece_of(row);
+                h8 v = {};
+                if (row < left) {
+                    const half_t* const from = tile + (int64_t)row * (keys ? a.k_row : a.v_row) + 8 * piece;
+                    if (8 * piece + 8 <= width) v = whole_piece(from);
+                    else
+                        for (int j = 0; 8 * piece + j < width; ++j) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (e == j) v[e] = from[j];
+                        }
+                }
+                *reinterpret_cast<h8*>(to + row * kRowBytes + part * 16) = v;
+            }
+        } else {
+            const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<half_t*>(tile), 0, 2u * ((unsigned)((left < kKeys ? left : kKeys) - 1) * stride + (unsigned)width), 0x00020000);
+            // (at is a multiple of the rows over which pieces change places)
+            const int piece = piece_of(part_row);
+            const unsigned first = piece * 8 < width ? 2u * ((unsigned)part_row * stride) + 16u * piece : 0x80000000u;
+#pragma unroll
+            for (int i = 0; i < kAccesses; ++i) {
+                const int at = i * kRowsAtOnce * kWaves;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(to + (at + wave * kRowsAtOnce) * kRowBytes), 16,
+                                                         first + 2u * (unsigned)at * stride, 0, 0, 0);
+            }
+        }
+    };
+    // The tiles come one after the other, K and V each.
+    const half_t *k_tile = k_base, *v_tile = v_base;
+    auto fetch_k = [&](int t, char* to) __attribute__((always_inline)) {
+        if (t >= tiles) return;
+        fetch(k_tile, (unsigned)a.k_row, a.k_dim, true, r.k_count - t * kKeys, to);
+        k_tile += kKeys * a.k_row;
+    };
+    auto fetch_v = [&](int t, char* to) __attribute__((always_inline)) {
+        if (t >= tiles) return;
+        fetch(v_tile, (unsigned)a.v_row, a.v_dim, false, r.k_count - t * kKeys, to);
+        v_tile += kKeys * a.v_row;
+    };
+    auto fetch_first = [&]() __attribute__((always_inline)) {
+        fetch_k(0, k_even);
+        fetch_v(0, v_even);
+        fetch_k(1, k_odd);
+    };
+    fetch_first();
+
     h8 q[kSteps];
     const bool row_exists = row < rows;
     {
-        const int token = row_exists ? row / a.group : 0, head = kv_head * a.group + (row_exists ? row - token * a.group : 0);
+        const int token = row_exists ? query_of(a, row) : 0, head = kv_head * a.group + (row_exists ? row - token * a.group : 0);
         const half_t* from = a.q + (int64_t)(r.q_first + token) * a.q_row + (int64_t)head * a.q_head;
         // whole pieces, then the one that is not whole
         const int partial = a.k_dim >> 3;
@@ -152,59 +227,7 @@ __global__ __launch_bounds__(64 * GROUPS * SPLIT, LOAD == kThrough ? 1 : 2) void
         }
     }
     f16 out[D];
-#pragma unroll
-    for (int i = 0; i < D; ++i) out[i] = f16{};
-    float m = kLowest, l = 0.f;
-    const float unit = a.scale * 1.4426950408889634f;  // positive: a negative scale has turned q
-
-    const half_t* const k_base = a.k + (int64_t)r.k_first * a.k_row + (int64_t)kv_head * a.k_head;
-    const half_t* const v_base = a.v + (int64_t)r.k_first * a.v_row + (int64_t)kv_head * a.v_head;
-    // this lane's part of an access: a row of the tile and a piece of it
-    const int part_row = wave * kRowsAtOnce + lane / kPieces, part = lane % kPieces;
-    // Rows behind the sequence lie beyond the descriptor and come as zeros, and so do pieces behind the width.
-    auto fetch = [&](const half_t* tile, unsigned stride, int width, bool keys, int left, char* to) __attribute__((always_inline)) {
-        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<half_t*>(tile), 0, 2u * ((unsigned)((left < kKeys ? left : kKeys) - 1) * stride + (unsigned)width), 0x00020000);
-#pragma unroll
-        for (int i = 0; i < kAccesses; ++i) {
-            const int at = i * kRowsAtOnce * GROUPS, row = at + part_row;
-            int piece = keys ? part ^ (row & (kPieces - 1)) : part ^ (2 * (row & 3));
-            if (keys) piece = 2 * moved(piece >> 1) + (piece & 1);
-            if constexpr (LOAD == kThrough) {
-                // (value by value in the last piece of a row; these layouts are for other callers than the fused projection)
-                h8 v = {};
-                if (row < left) {
-                    const half_t* const from = tile + (int64_t)row * (keys ? a.k_row : a.v_row) + 8 * piece;
-                    if (8 * piece + 8 <= width) v = whole_piece(from);
-                    else
-                        for (int j = 0; 8 * piece + j < width; ++j) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                if (e == j) v[e] = from[j];
-                        }
-                }
-                *reinterpret_cast<h8*>(to + row * kRowBytes + part * 16) = v;
-            } else {
-                const unsigned first = piece * 8 < width ? 2u * ((unsigned)part_row * stride) + 16u * piece : 0x80000000u;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr)(to + (at + wave * kRowsAtOnce) * kRowBytes), 16,
-                                                         first + 2u * (unsigned)at * stride, 0, 0, 0);
-            }
-        }
-    };
-    // Tile t of this set.  The tiles come one after the other, K and V each.
-    auto key_of = [&](int t) __attribute__((always_inline)) { return (t * SPLIT + set) * kKeys; };
-    const half_t *k_tile = k_base + (int64_t)key_of(0) * a.k_row, *v_tile = v_base + (int64_t)key_of(0) * a.v_row;
-    const int64_t k_ahead = (int64_t)(SPLIT * kKeys) * a.k_row, v_ahead = (int64_t)(SPLIT * kKeys) * a.v_row;
-    auto fetch_k = [&](int t, char* to) __attribute__((always_inline)) {
-        if (t * SPLIT + set >= tiles) return;
-        fetch(k_tile, (unsigned)a.k_row, a.k_dim, true, r.k_count - key_of(t), to);
-        k_tile += k_ahead;
-    };
-    auto fetch_v = [&](int t, char* to) __attribute__((always_inline)) {
-        if (t * SPLIT + set >= tiles) return;
-        fetch(v_tile, (unsigned)a.v_row, a.v_dim, false, r.k_count - key_of(t), to);
-        v_tile += v_ahead;
-    };
+    float m, l;
     // where the lane reads: K rows col and 32 + col, piece 2 step + half; V rows 4 half + j (+ 8), j = (lane / 4) % 4, four channels
     const int k_read = col * kRowBytes, k_swap = col & (kPieces - 1);
     const int v_j = (lane >> 2) & 3, v_read = (4 * half + v_j) * kRowBytes + (lane & 1) * 8;
@@ -225,25 +248,24 @@ __global__ __launch_bounds__(64 * GROUPS * SPLIT, LOAD == kThrough ? 1 : 2) void
     };
     // A step: the weights of tile t from its scores, which the step before has computed, the next tile's scores, the second product.
     auto step = [&](int t, char* k_lds, char* v_lds, char* next_k_lds, char* next_v_lds, f16 (&score)[2], f16 (&next)[2]) __attribute__((always_inline)) {
-        const int key0 = key_of(t);
+        const int key0 = t * kKeys;
         UNIQL_WAIT_ALL_LOADS();
         __syncthreads();
         fetch_k(t + 2, k_lds);
         fetch_v(t + 1, next_v_lds);
         const bool masked = key0 + kKeys > fewest;
-        // A key that some rows of the tile see and others do not: its weight is zero for those, but zero times an infinity is not.  Where
-        // the workgroup has such keys each lane looks at one; those with such values become zeros in LDS, and what they give to the rows that
-        // see them is added on its own, below.
+        // A key that some rows of the tile see and others do not: its weight is zero for those, but zero times an infinity is not.  In the
+        // careful pass each lane looks at one such key; those with such values become zeros in LDS, and what they give to the rows that see
+        // them is added on its own, below.
         unsigned long long odd_keys = 0;
-        if (a.causal && (t + 1) * SPLIT * kKeys > block_fewest) {  // the same for all waves
+        if (careful && key0 + kKeys > block_fewest) {  // the same for all waves
             uint32_t any = 0;
-#pragma unroll 4
             for (int i = 0; i < kPieces; ++i) {
-                const u32x4 w = *reinterpret_cast<const u32x4*>(v_lds + lane * kRowBytes + ((i + lane) & (kPieces - 1)) * 16);
+                const u32x4 w = *reinterpret_cast<const u32x4*>(v_lds + lane * kRowBytes + i * 16);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) any |= ((w[j] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;  // an exponent of all ones runs over
             }
-            odd_keys = key0 < block_most ? __ballot(any != 0) : 0ull;
+            odd_keys = __ballot(any != 0);
             __syncthreads();
             if ((odd_keys >> lane) & 1)
                 for (int i = 0; i < kPieces; ++i) *reinterpret_cast<u32x4*>(v_lds + lane * kRowBytes + i * 16) = u32x4{0u, 0u, 0u, 0u};
@@ -251,12 +273,13 @@ __global__ __launch_bounds__(64 * GROUPS * SPLIT, LOAD == kThrough ? 1 : 2) void
         const bool active = key0 < most;  // the wave's rows see some of the keys (all waves take part in the barriers)
         if (active) {
             if (masked) {
-                asm volatile("");  // keeps the comparisons out of the other tiles' way
+                int seen_here = seen - key0 - 4 * half;
+                asm volatile("" : "+v"(seen_here));  // keeps the comparisons out of the other tiles' way
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (key0 + 32 * k + 8 * (i / 4) + 4 * half + i % 4 >= seen) score[k][i] = -INFINITY;
+                        if (32 * k + 8 * (i / 4) + i % 4 >= seen_here) score[k][i] = -INFINITY;
             }
             float top = score[0][0];
 #pragma unroll
@@ -267,9 +290,11 @@ __global__ __launch_bounds__(64 * GROUPS * SPLIT, LOAD == kThrough ? 1 : 2) void
                 const float higher = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)) * unit);
                 const float fade = __builtin_amdgcn_exp2f(m - higher);
                 m = higher;
-                l *= fade;
+                if (t > 0) {  // (all zeros so far)
+                    l *= fade;
 #pragma unroll
-                for (int i = 0; i < D; ++i) out[i] *= fade;
+                    for (int i = 0; i < D; ++i) out[i] *= fade;
+                }
             }
         }
         if (!active) return;
@@ -350,96 +375,90 @@ __global__ __launch_bounds__(64 * GROUPS * SPLIT, LOAD == kThrough ? 1 : 2) void
             }
         }
     };
-    const int rounds = (tiles + SPLIT - 1) / SPLIT;
-    if (rounds > 0) {
-        f16 even[2], odd[2];
-        fetch_k(0, k_even);
-        fetch_v(0, v_even);
-        fetch_k(1, k_odd);
-        UNIQL_WAIT_ALL_LOADS();
-        __syncthreads();
-        even[0] = even[1] = f16{};
+    for (int pass = 0;; ++pass) {
+        careful = pass > 0;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i)
+        for (int i = 0; i < D; ++i) out[i] = f16{};
+        m = kLowest, l = 0.f;
+        if (tiles > 0) {
+            f16 even[2], odd[2];
+            UNIQL_WAIT_ALL_LOADS();
+            __syncthreads();
+            h8 keys[4];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) even[k] = product(keys_of(k_even, k, i), i, even[k]);
-        for (int t = 0; t < rounds; t += 2) {
-            step(t, k_even, v_even, k_odd, v_odd, even, odd);
-            if (t + 1 < rounds) step(t + 1, k_odd, v_odd, k_even, v_even, odd, even);
+            for (int i = 0; i < 4; ++i) keys[i] = keys_of(k_even, i & 1, i >> 1);
+            even[0] = even[1] = f16{};
+#pragma unroll
+            for (int i = 0; i < 2 * kSteps; ++i) {
+                even[i & 1] = product(keys[i & 3], i >> 1, even[i & 1]);
+                if (i + 4 < 2 * kSteps) keys[i & 3] = keys_of(k_even, i & 1, (i + 4) >> 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            for (int t = 0; t < tiles; t += 2) {
+                step(t, k_even, v_even, k_odd, v_odd, even, odd);
+                if (t + 1 < tiles) step(t + 1, k_odd, v_odd, k_even, v_even, odd, even);
+            }
         }
-    }
-    l += __shfl_xor(l, 32, 64);
-    if constexpr (SPLIT == 2) {
-        // the second set's results go through LDS, 16 KiB a wave: half of them in each of the two K tiles' and V tiles' places
-        constexpr int kPart = 8 * D;  // values of a lane
-        float* const place[2] = {reinterpret_cast<float*>(k_even_all), reinterpret_cast<float*>(v_even_all)};
-        float* const extra = reinterpret_cast<float*>(k_odd_all);
-        static_assert(GROUPS * kPart * 64 * 4 <= SPLIT * kTileBytes, "the results fit the tiles' places");
-        __syncthreads();
-        if (set == 1) {
-#pragma unroll
-            for (int i = 0; i < D; ++i)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) place[(16 * i + j) / kPart][(wave * kPart + (16 * i + j) % kPart) * 64 + lane] = out[i][j];
-            extra[wave * 128 + lane] = m;
-            extra[wave * 128 + 64 + lane] = l;
-        }
-        __syncthreads();
-        if (set == 1) return;
-        const float other = extra[wave * 128 + lane], other_l = extra[wave * 128 + 64 + lane];
-        const float higher = fmaxf(m, other), keep = __builtin_amdgcn_exp2f(m - higher), add = __builtin_amdgcn_exp2f(other - higher);
-        l = l * keep + other_l * add;
+        if (pass > 0 || !a.causal) break;
+        // Infinities and NaN are rare: where a result shows one, all is done again with care.
+        float zero = 0.f;
 #pragma unroll
         for (int i = 0; i < D; ++i)
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                out[i][j] = out[i][j] * keep + place[(16 * i + j) / kPart][(wave * kPart + (16 * i + j) % kPart) * 64 + lane] * add;
+            for (int j = 0; j < 16; ++j) zero = __builtin_fmaf(out[i][j], 0.f, zero);
+        const bool bad = __any(row < rows && zero != 0.f);
+        if (lane == 0) spoilt[wave] = bad;
+        __syncthreads();
+        int any = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) any |= spoilt[w];
+        if (__builtin_amdgcn_readfirstlane(any) == 0) break;
+        k_tile = k_base, v_tile = v_base;
+        fetch_first();
     }
+    l += __shfl_xor(l, 32, 64);
     int my_row = row;
     asm volatile("" : "+v"(my_row));  // the quotient is not kept over the loop
     if (my_row >= rows) return;
-    const int token = my_row / a.group, head = kv_head * a.group + my_row - token * a.group;
+    const int token = query_of(a, my_row), head = kv_head * a.group + my_row - token * a.group;
     half_t* to = a.out + (int64_t)(r.q_first + token) * a.out_row + (int64_t)head * a.out_head;
+    // A lane has four values of every eight, the lane 32 from it the others: exchanged so that each has whole eights.
     const float inverse = seen > 0 ? 1.0f / l : 0.f;
 #pragma unroll
     for (int i = 0; i < D; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int channel = 32 * i + 8 * j + 4 * half;
-            half_t v[4];
+        for (int j = 0; j < 2; ++j) {
+            uint32_t w[2][2];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = seen > 0 ? (half_t)(out[i][4 * j + e] * inverse) : (half_t)0.f;
-            if (channel + 4 <= a.v_dim) {
-                *reinterpret_cast<h4u*>(to + channel) = h4u{v[0], v[1], v[2], v[3]};
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int f = 0; f < 2; ++f) {
+                    const f2 v = {out[i][8 * j + 4 * e + 2 * f] * inverse, out[i][8 * j + 4 * e + 2 * f + 1] * inverse};
+                    w[e][f] = seen > 0 ? h2_to_bits(__builtin_convertvector(v, h2)) : 0u;
+                }
+            const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+            const h8 v = __builtin_bit_cast(h8, u32x4{x[0], y[0], x[1], y[1]});
+            const int channel = 32 * i + 16 * j + 8 * half;
+            if (channel + 8 <= a.v_dim) {
+                *reinterpret_cast<h8u*>(to + channel) = h8u{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
             } else {
+                for (int e = 0; channel + e < a.v_dim; ++e) {
+                    half_t one = v[0];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (channel + e < a.v_dim) to[channel + e] = v[e];
+                    for (int f = 1; f < 8; ++f) one = e == f ? v[f] : one;
+                    to[channel + e] = one;
+                }
             }
         }
 }
 
-template <int D, int GROUPS, int SPLIT, int LOAD>
-static void go(const PromptArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL((prompt_attention_kernel<D, GROUPS, SPLIT, LOAD>), dim3((unsigned)(a.blocks * (a.heads / a.group))), dim3(64 * GROUPS * SPLIT), 0,
-                       stream, a);
-}
-template <int D, int LOAD>
-static void go(const PromptArgs& a, int shape, hipStream_t stream) {
-    if (shape == 0) go<D, 4, 1, LOAD>(a, stream);
-    else if (shape == 1) go<D, 4, 2, LOAD>(a, stream);
-    else go<D, 2, 2, LOAD>(a, stream);
-}
 template <int D>
-static void go(const PromptArgs& a, int shape, int load, hipStream_t stream) {
-    if (load == kWhole) go<D, kWhole>(a, shape, stream);
-    else if (load == kTail) go<D, kTail>(a, shape, stream);
-    else go<D, 4, 1, kThrough>(a, stream);
-}
-
-static int prompt_shape(const PromptArgs& a) {
-    if (const char* e = getenv("UNIQL_SHAPE")) return atoi(e);
-    return 0;
+static void go(const PromptArgs& a, int load, hipStream_t stream) {
+    const dim3 grid((unsigned)(a.blocks * (a.heads / a.group))), block(64 * kWaves);
+    if (load == kWhole) hipLaunchKernelGGL((prompt_attention_kernel<D, kWhole>), grid, block, 0, stream, a);
+    else if (load == kTail) hipLaunchKernelGGL((prompt_attention_kernel<D, kTail>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((prompt_attention_kernel<D, kThrough>), grid, block, 0, stream, a);
 }
 
 int prompt_attention_launch(const PromptArgs& args, hipStream_t stream) {
@@ -452,15 +471,19 @@ int prompt_attention_launch(const PromptArgs& args, hipStream_t stream) {
     const bool near = a.k_row >= a.k_dim && a.v_row >= a.v_dim && a.k_row <= far && a.v_row <= far;
     const int load = near && (strides & 7) == 0 && (bases & 15) == 0 ? kWhole
                      : near && (strides & 1) == 0 && (bases & 3) == 0 && a.k_row >= 8 && a.v_row >= 8 ? kTail : kThrough;
-    const int shape = load == kThrough ? 0 : prompt_shape(a);
-    const int block_rows = kQueries * (shape == 2 ? 2 : 4);
-    const int64_t rows = (int64_t)a.rows * a.group, blocks = rows / block_rows + (a.sequences < a.rows ? a.sequences : a.rows);
+    const int64_t rows = (int64_t)a.rows * a.group, blocks = rows / kBlockRows + (a.sequences < a.rows ? a.sequences : a.rows);
     if (rows > (1LL << 30) || blocks * (a.heads / a.group) > 0x7fffffffLL) return UNIQL_E_SHAPE;
     a.blocks = (int)blocks;
+    // floor(row / d) = row f >> (31 + s) with f = 2^(31 + s) / d rounded up and s so that d <= 2^s < 2 d: f d - 2^(31 + s) < 2^s, so the
+    // excess stays below 1 / d for rows below 2^31
+    int s = 0;
+    while ((1 << s) < a.group) ++s;
+    a.group_shift = 31 + s;
+    a.group_factor = (unsigned)(((1ULL << a.group_shift) + a.group - 1) / a.group);
     const int width = ((a.k_dim > a.v_dim ? a.k_dim : a.v_dim) + 31) / 32;
-    if (width <= 2) go<2>(a, shape, load, stream);
-    else if (width == 3) go<3>(a, shape, load, stream);
-    else go<4>(a, shape, load, stream);
+    if (width <= 2) go<2>(a, load, stream);
+    else if (width == 3) go<3>(a, load, stream);
+    else go<4>(a, load, stream);
     return hipGetLastError() == hipSuccess ? UNIQL_OK : UNIQL_E_LAUNCH;
 }
 

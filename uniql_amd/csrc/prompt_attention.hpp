@@ -12,7 +12,9 @@ struct PromptArgs {
     half_t* out;
     int rows, k_rows, sequences, heads, group, k_dim, v_dim, causal;
     float scale;
-    int q_sign, blocks;  // set by the launch: the scale's sign, and blocks of rows in all sequences at most
+    // set by the launch: the scale's sign, blocks of rows in all sequences at most, factor and shift for quotients by `group`
+    int q_sign, blocks, group_shift;
+    unsigned group_factor;
 };
 
 }  // namespace uniql
