@@ -24,11 +24,12 @@ typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
 constexpr int kTile = 64;              // positions a wave takes at a time
 constexpr int kRows = 16;              // rows of a workgroup
 constexpr int kWaves = 4;
-constexpr int kSlotFloats = 16 * 132;  // a workgroup's partial result: 16 rows of 128 channels, m and sum p
+constexpr int kSlotFloats = 16 * 130;  // a workgroup's partial result: 16 rows of 128 channels, then (m, sum p) of each
+constexpr int kDeviceScope = 16;       // cache policy bit sc1: as relaxed device-scope loads and stores compile to
 constexpr int kOutStride = 132;
 constexpr float kNoMaximum = -3.0e38f;
 constexpr float kSlack = 8.0f;         // weights may grow to 2^8 before the maximum follows
-constexpr int kWorkgroups = 1024;      // that a call is shared out to, four a compute unit
+constexpr int kWorkgroups = 512;       // that a call is shared out to, two a compute unit
 
 template <int S>
 struct Words;
@@ -78,63 +79,97 @@ __device__ __forceinline__ Request request_of(const KvAttentionArgs& a, int r) {
     q.length = n < 0 ? 0 : (n > room ? (int)room : n);
     return q;
 }
+// row / a.group for rows below 2^31 (see the launch)
+__device__ __forceinline__ int query_of(const KvAttentionArgs& a, int row) { return (int)(((uint64_t)(unsigned)row * a.group_factor) >> a.group_shift); }
 __device__ __forceinline__ int row_tiles(const KvAttentionArgs& a, const Request& q) { return (int)(((int64_t)q.count * a.group + kRows - 1) / kRows); }
 __device__ __forceinline__ int position_tiles(const Request& q) { return (q.length + kTile - 1) / kTile; }
+
+// Sums over the lanes up to and including each.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned from_below(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false); }
+template <typename Add>
+__device__ __forceinline__ unsigned sums_upto(unsigned v, Add add) {
+    v = add(v, from_below<0x111, 0xf>(v));  // one, two, four, eight lanes below, within sixteen
+    v = add(v, from_below<0x112, 0xf>(v));
+    v = add(v, from_below<0x114, 0xf>(v));
+    v = add(v, from_below<0x118, 0xf>(v));
+    v = add(v, from_below<0x142, 0xa>(v));  // the last of the sixteen below, for the second and fourth sixteen
+    return add(v, from_below<0x143, 0xc>(v));  // lane 31, for the upper half
+}
+__device__ __forceinline__ unsigned lane_value(unsigned v, int lane) { return (unsigned)__builtin_amdgcn_readlane((int)v, lane); }
 
 // A workgroup's share: `run` position tiles from tile `run * chunk` on, for row tile `rows` of request `request`; `index0` is the
 // index of the first of the `chunks` workgroups that share these rows.
 struct Share {
+    Request what;
     int request, rows, chunk, chunks, run, index0;
 };
 // Every wave finds it for itself.  Position tiles times row tiles of all requests, over the workgroups there are, give the run's
 // length; requests in order take one workgroup for each run.
 __device__ __forceinline__ bool find_share(const KvAttentionArgs& a, int index, Share& s) {
     const int lane = threadIdx.x & 63;
+    const auto add_f = [](unsigned x, unsigned y) { return __builtin_bit_cast(unsigned, __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y)); };
+    const auto add_u = [](unsigned x, unsigned y) { return x + y; };
+    Request q = {0, 0, 0};
     float total = 0.f;
-    for (int r = lane; r < a.requests; r += 64) {
-        const Request q = request_of(a, r);
-        total += (float)row_tiles(a, q) * (float)position_tiles(q);
+    for (int base = 0; base < a.requests; base += 64) {
+        const int r = base + lane;
+        q = Request{0, 0, 0};
+        if (r < a.requests) q = request_of(a, r);
+        const float mine = (float)row_tiles(a, q) * (float)position_tiles(q);
+        total += __builtin_bit_cast(float, lane_value(sums_upto(__builtin_bit_cast(unsigned, mine), add_f), 63));
     }
-    for (int d = 1; d < 64; d <<= 1) total += __shfl_xor(total, d, 64);
     // (a little more than the quotient: sums in fp32 must not make more runs than there are workgroups for)
     const float run_f = total * 1.0001f / (float)a.shares;
     int run = run_f < 1.0e9f ? (int)run_f + 1 : 1 << 30;
-    run = (run + kWaves - 1) / kWaves * kWaves;
-    int64_t before = 0;
+    run = __builtin_amdgcn_readfirstlane((run + kWaves - 1) / kWaves * kWaves);
+    const float by_run = 1.0f / (float)run;
+    unsigned before = 0;
     for (int base = 0; base < a.requests; base += 64) {
-        const int r = base + lane;
-        int64_t mine = 0;
-        int tiles = 0, chunks = 1;
-        if (r < a.requests) {
-            const Request q = request_of(a, r);
-            tiles = row_tiles(a, q);
-            const int positions = position_tiles(q);
-            chunks = positions > run ? (positions + run - 1) / run : 1;
-            mine = (int64_t)tiles * chunks;
+        if (a.requests > 64) {
+            const int r = base + lane;
+            q = Request{0, 0, 0};
+            if (r < a.requests) q = request_of(a, r);
         }
-        int64_t upto = mine;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t other = __shfl_up(upto, d, 64);
-            if (lane >= d) upto += other;
+        const int tiles = row_tiles(a, q), positions = position_tiles(q);
+        // positions / run rounded up, from the quotient in fp32, which is off by one at most
+        int chunks = 1;
+        if (positions > run) {
+            chunks = (int)((float)positions * by_run);
+            while ((int64_t)chunks * run < positions) ++chunks;
+            while ((int64_t)(chunks - 1) * run >= positions) --chunks;
         }
-        const unsigned long long above = __ballot(before + upto > index);
+        const int64_t want = (int64_t)tiles * chunks;
+        const unsigned mine = want < (1 << 25) ? (unsigned)want : 1u << 25;  // (more than any grid has: offsets that fall and rise again)
+        const unsigned upto = sums_upto(mine, add_u);
+        const unsigned long long above = __ballot((uint64_t)before + upto > (uint64_t)index);
         if (above) {
             const int owner = __builtin_ctzll(above);
-            const int64_t start = before + __shfl(upto - mine, owner, 64);
-            const int c = __shfl(chunks, owner, 64);
-            const int at = (int)(index - start);
-            s.request = __builtin_amdgcn_readfirstlane(base + owner);
-            s.chunks = __builtin_amdgcn_readfirstlane(c);
-            s.rows = __builtin_amdgcn_readfirstlane(at / c);
-            s.chunk = __builtin_amdgcn_readfirstlane(at % c);
+            const int start = (int)(before + lane_value(upto - mine, owner));
+            s.chunks = (int)lane_value((unsigned)chunks, owner);
+            s.what = Request{(int)lane_value((unsigned)q.first, owner), (int)lane_value((unsigned)q.count, owner),
+                             (int)lane_value((unsigned)q.length, owner)};
+            s.request = base + owner;
+            const int at = index - start;
+            s.rows = s.chunks == 1 ? at : at / s.chunks;
+            s.chunk = at - s.rows * s.chunks;
             s.run = run;
             s.index0 = index - s.chunk;
             return true;
         }
-        before += __shfl(upto, 63, 64);
+        before += lane_value(upto, 63);
+        if (before > 0x7fffffffu) return false;
     }
     return false;
 }
+
+// What a wave reads for 64 positions.
+template <int S>
+struct Positions {
+    typename Words<S>::type k[4];
+    u32x4 v[4];
+    uint64_t k_scales[4], v_scales[4];
+};
 
 template <int S>
 __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttentionArgs a) {
@@ -145,17 +180,52 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
     const int heads = c.heads, kv_head = (int)(blockIdx.x % (unsigned)heads), index = (int)(blockIdx.x / (unsigned)heads);
     Share s;
     if (!find_share(a, index, s)) return;
-    const Request rq = request_of(a, s.request);
+    const Request rq = s.what;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quad = lane >> 4;
     const int rows_total = rq.count * a.group, flat = s.rows * kRows + col;
     const bool row_exists = flat < rows_total;
-    const int token = row_exists ? flat / a.group : 0, sub_head = row_exists ? flat - token * a.group : 0;
+    const int token = row_exists ? query_of(a, flat) : 0, sub_head = row_exists ? flat - token * a.group : 0;
     // positions that the lane's row sees; the first and the last row of the tile have the fewest and the most
     const int limit = row_exists ? rq.length - rq.count + token + 1 : 0;
     const int last_flat = rows_total - 1 < s.rows * kRows + kRows - 1 ? rows_total - 1 : s.rows * kRows + kRows - 1;
-    const int seen_by_all = rq.length - rq.count + s.rows * kRows / a.group + 1, seen_by_any = rq.length - rq.count + last_flat / a.group + 1;
+    const int seen_by_all = rq.length - rq.count + query_of(a, s.rows * kRows) + 1, seen_by_any = rq.length - rq.count + query_of(a, last_flat) + 1;
     const int tiles = (seen_by_any + kTile - 1) / kTile;
     const int end = (s.chunk + 1) * s.run < tiles ? (s.chunk + 1) * s.run : tiles;
+
+    const int32_t* table = a.table + (int64_t)s.request * a.columns;
+    const int last_column = rq.length > 0 ? (rq.length - 1) >> c.page_shift : 0;
+    const int n_word = col < c.v_words ? col : 0;
+    const uint32_t mask_low = 0x000f000fu, mask_high = 0x00f000f0u;
+    struct Pages {
+        int page[4];
+    };
+    auto pages_of = [&](int t) __attribute__((always_inline)) {
+        Pages p;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int column = (t * kTile + 16 * u) >> c.page_shift;
+            p.page[u] = table[column < last_column ? column : last_column];
+        }
+        return p;
+    };
+    auto load = [&](int t, const Pages& p) __attribute__((always_inline)) {
+        Positions<S> x;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const bool there = (unsigned)p.page[u] < (unsigned)c.pages;
+            const int64_t at = (((int64_t)(there ? p.page[u] : 0) * heads + kv_head) << c.page_shift) + ((t * kTile + 16 * u) & ((1 << c.page_shift) - 1));
+            x.k[u] = *reinterpret_cast<const typename Words<S>::type*>(c.k_codes + at * (4 * S) + col * (4 * S) + quad * S);
+            x.k_scales[u] = *reinterpret_cast<const uint64_t*>(c.k_scales + at + 4 * quad);
+            x.v_scales[u] = *reinterpret_cast<const uint64_t*>(c.v_scales + at + 4 * quad);
+            x.v[u] = *reinterpret_cast<const u32x4*>(c.v_codes + at * c.v_words + quad * (4 * c.v_words) + 4 * n_word);
+        }
+        return x;
+    };
+    int t = s.chunk * s.run + wave;
+    Pages pages = pages_of(t);
+    Positions<S> next = {};
+    if (t < end) next = load(t, pages);
+    Pages next_pages = pages_of(t + kWaves);
 
     h8 q[S];
     float q_sum = 0.f;
@@ -177,37 +247,20 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
 #pragma unroll
     for (int i = 0; i < 8; ++i) out[i] = f4{0.f, 0.f, 0.f, 0.f};
     float m = kNoMaximum, l = 0.f, w_sum = 0.f;
-    const int32_t* table = a.table + (int64_t)s.request * a.columns;
-    const int last_column = rq.length > 0 ? (rq.length - 1) >> c.page_shift : 0;
-    const int n_word = col < c.v_words ? col : 0;
-    const uint32_t mask_low = 0x000f000fu, mask_high = 0x00f000f0u;
 
-    for (int t = s.chunk * s.run + wave; t < end; t += kWaves) {
+    for (; t < end; t += kWaves) {
         const int j0 = t * kTile;
         typename Words<S>::type kw[4];
         u32x4 vw[4];
         uint64_t ks[4], vs[4];
-        unsigned bad = 0;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int j = j0 + 16 * u;
-            const int column = j >> c.page_shift;
-            int page = table[column < last_column ? column : last_column];
-            if ((unsigned)page >= (unsigned)c.pages) {
-                page = 0;
-                bad |= 1u << u;
-            }
-            const int64_t at = (((int64_t)page * heads + kv_head) << c.page_shift) + (j & ((1 << c.page_shift) - 1));
-            kw[u] = *reinterpret_cast<const typename Words<S>::type*>(c.k_codes + at * (4 * S) + col * (4 * S) + quad * S);
-            ks[u] = *reinterpret_cast<const uint64_t*>(c.k_scales + at + 4 * quad);
-            vs[u] = *reinterpret_cast<const uint64_t*>(c.v_scales + at + 4 * quad);
-            vw[u] = *reinterpret_cast<const u32x4*>(c.v_codes + at * c.v_words + quad * (4 * c.v_words) + 4 * n_word);
+            kw[u] = next.k[u], vw[u] = next.v[u], ks[u] = next.k_scales[u], vs[u] = next.v_scales[u];
+            if ((unsigned)pages.page[u] >= (unsigned)c.pages) ks[u] = 0x7e007e007e007e00ull;  // no such page: NaN
         }
-        if (bad) {  // pages that do not exist: NaN
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (bad & (1u << u)) ks[u] = 0x7e007e007e007e00ull;
-        }
+        pages = next_pages;
+        if (t + kWaves < end) next = load(t + kWaves, pages);
+        next_pages = pages_of(t + 2 * kWaves);
         float score[16];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -312,7 +365,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
     }
     __syncthreads();
     // a thread: eight channels of a row
-    const int my_row = tid >> 4, my_channel = 8 * (tid & 15);
+    int my_row = tid >> 4;
+    const int my_channel = 8 * (tid & 15);
     float top = kNoMaximum, sum = 0.f, o[8] = {};
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, merge_m[w * 16 + my_row]);
@@ -324,19 +378,20 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] += from[i] * part;
     }
-    const int my_flat = s.rows * kRows + my_row;
+    int my_flat = s.rows * kRows + my_row;
     const bool mine = my_flat < rows_total;
     if (s.chunks > 1) {
         // The exchange: relaxed stores at device scope, which pass the local L2; a wait until they have been acknowledged; the
         // barrier; the count.  The last to arrive reads with relaxed loads at device scope.
-        float* slot = a.temp + (int64_t)blockIdx.x * kSlotFloats;
+        const __amdgpu_buffer_rsrc_t slot =
+            __builtin_amdgcn_make_buffer_rsrc(a.temp + (int64_t)blockIdx.x * kSlotFloats, 0, (unsigned)kSlotFloats * 4u, 0x00020000);
         if (mine) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) __hip_atomic_store(slot + my_row * kOutStride + my_channel + i, o[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if ((tid & 15) == 0) {
-                __hip_atomic_store(slot + my_row * kOutStride + 128, top, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                __hip_atomic_store(slot + my_row * kOutStride + 129, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
+            const uint32_t at = 4u * (uint32_t)(my_row * 128 + my_channel);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f4{o[0], o[1], o[2], o[3]}), slot, at, 0, kDeviceScope);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f4{o[4], o[5], o[6], o[7]}), slot, at + 16u, 0, kDeviceScope);
+            if ((tid & 15) == 0)
+                __builtin_amdgcn_raw_buffer_store_b64(u32x2{__builtin_bit_cast(uint32_t, top), __builtin_bit_cast(uint32_t, sum)}, slot,
+                                                      8192u + 8u * (uint32_t)my_row, 0, kDeviceScope);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
@@ -345,26 +400,68 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
         __syncthreads();
         if (!last_flag) return;
         if (tid == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (!mine) return;
+        asm volatile("" ::: "memory");
+        // Rows of the tile that exist, times slices of the partial results: all threads read, four results on their way at a time.
+        const int rows_here = rows_total - s.rows * kRows < kRows ? rows_total - s.rows * kRows : kRows;
+        int shift = 0;
+        while ((1 << shift) < rows_here) ++shift;
+        const int slices = kRows >> shift, slice = (tid >> 4) >> shift;
+        my_row = (tid >> 4) & ((1 << shift) - 1);
         top = kNoMaximum, sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = 0.f;
-        for (int k = 0; k < s.chunks; ++k) {
-            const float* from = a.temp + ((int64_t)(s.index0 + k) * heads + kv_head) * kSlotFloats + my_row * kOutStride;
-            const float other = __hip_atomic_load(from + 128, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const float other_sum = __hip_atomic_load(from + 129, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            float v[8];
+        for (int first = slice; first < s.chunks; first += 4 * slices) {
+            u32x4 lo[4], hi[4];
+            u32x2 ml[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __hip_atomic_load(from + my_channel + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const float next = fmaxf(top, other), keep = __builtin_amdgcn_exp2f(top - next), add = __builtin_amdgcn_exp2f(other - next);
-            top = next;
-            sum = sum * keep + other_sum * add;
+            for (int k = 0; k < 4; ++k) {
+                const int from = first + k * slices < s.chunks ? first + k * slices : first;
+                const __amdgpu_buffer_rsrc_t part = __builtin_amdgcn_make_buffer_rsrc(a.temp + ((int64_t)s.index0 * heads + kv_head) * kSlotFloats, 0,
+                                                                                      0xffffffffu, 0x00020000);
+                const uint32_t at = 4u * (uint32_t)from * (uint32_t)(heads * kSlotFloats);
+                lo[k] = __builtin_amdgcn_raw_buffer_load_b128(part, at + 4u * (uint32_t)(my_row * 128 + my_channel), 0, kDeviceScope);
+                hi[k] = __builtin_amdgcn_raw_buffer_load_b128(part, at + 4u * (uint32_t)(my_row * 128 + my_channel) + 16u, 0, kDeviceScope);
+                ml[k] = __builtin_amdgcn_raw_buffer_load_b64(part, at + 8192u + 8u * (uint32_t)my_row, 0, kDeviceScope);
+            }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = o[i] * keep + v[i] * add;
+            for (int k = 0; k < 4; ++k) {
+                if (first + k * slices >= s.chunks) break;
+                const uint32_t m_bits = ml[k][0], l_bits = ml[k][1];  // (a bit cast of an element takes the vector's first one)
+                const float other = __builtin_bit_cast(float, m_bits), other_sum = __builtin_bit_cast(float, l_bits);
+                const float higher = fmaxf(top, other), keep = __builtin_amdgcn_exp2f(top - higher), add = __builtin_amdgcn_exp2f(other - higher);
+                top = higher;
+                sum = sum * keep + other_sum * add;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[i] = o[i] * keep + __builtin_bit_cast(f4, lo[k])[i] * add;
+                    o[4 + i] = o[4 + i] * keep + __builtin_bit_cast(f4, hi[k])[i] * add;
+                }
+            }
         }
+        if (slices > 1) {
+            float* const to = merge + (tid >> 4) * kOutStride + my_channel;
+            *reinterpret_cast<f4*>(to) = f4{o[0], o[1], o[2], o[3]};
+            *reinterpret_cast<f4*>(to + 4) = f4{o[4], o[5], o[6], o[7]};
+            merge_m[tid >> 4] = top;
+            merge_l[tid >> 4] = sum;
+            __syncthreads();
+            if (slice > 0) return;
+            for (int k = 1; k < slices; ++k) {
+                const int at = my_row + (k << shift);
+                const float other = merge_m[at], higher = fmaxf(top, other);
+                const float keep = __builtin_amdgcn_exp2f(top - higher), add = __builtin_amdgcn_exp2f(other - higher);
+                top = higher;
+                sum = sum * keep + merge_l[at] * add;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o[i] = o[i] * keep + merge[at * kOutStride + my_channel + i] * add;
+            }
+        }
+        my_flat = s.rows * kRows + my_row;
+        if (my_row >= rows_here) return;
+    } else if (!mine) {
+        return;
     }
-    if (!mine) return;
-    const int my_token = my_flat / a.group, my_head = kv_head * a.group + my_flat - my_token * a.group;
+    const int my_token = query_of(a, my_flat), my_head = kv_head * a.group + my_flat - my_token * a.group;
     const bool empty = rq.length - rq.count + my_token + 1 <= 0;
     half_t* to = a.out + (int64_t)(rq.first + my_token) * a.out_row + (int64_t)my_head * a.out_head + my_channel;
     h8u result;
@@ -399,6 +496,11 @@ void kv4_attention_needs(int rows, int requests, int q_heads, const KvCache& cac
 int kv4_attention_launch(const KvAttentionArgs& args, hipStream_t stream) {
     KvAttentionArgs a = args;
     a.shares = (int)shares_of(a.cache.heads);
+    // floor(row / d) = row f >> (31 + s) with f = 2^(31 + s) / d rounded up and s so that d <= 2^s < 2 d
+    int shift = 0;
+    while ((1 << shift) < a.group) ++shift;
+    a.group_shift = 31 + shift;
+    a.group_factor = (unsigned)(((1ULL << a.group_shift) + a.group - 1) / a.group);
     const int64_t workgroups = workgroups_of(a.rows, a.requests, a.group, a.cache.heads, a.cu_q == nullptr) * a.cache.heads;
     if (workgroups > 0x7fffffffLL) return UNIQL_E_SHAPE;
     const dim3 grid((unsigned)workgroups), block(64 * kWaves);

@@ -17,6 +17,8 @@ struct KvAttentionArgs {
     int rows, requests, columns, group;  // group: query heads of a key / value head
     int shares;                          // runs of positions that a head's work is shared out to
     float scale;
+    int group_shift;                     // for quotients by `group`, set by the launch, as `shares` is
+    unsigned group_factor;
 };
 
 }  // namespace uniql
