@@ -98,16 +98,35 @@ __device__ __forceinline__ unsigned sums_upto(unsigned v, Add add) {
 }
 __device__ __forceinline__ unsigned lane_value(unsigned v, int lane) { return (unsigned)__builtin_amdgcn_readlane((int)v, lane); }
 
-// A workgroup's share: `run` position tiles from tile `run * chunk` on, for row tile `rows` of request `request`; `index0` is the
-// index of the first of the `chunks` workgroups that share these rows.
+// A workgroup's share of a request's row tile `rows`.  Either the position tiles from `run * chunk` on, `run` of them, for one key /
+// value head, a tile a wave in turn; `chunks` workgroups share these rows, and their partial results lie in the places `place - chunk`
+// and on.  Or, `alone`, all of its positions, a head a wave: requests too short to keep four waves busy.
 struct Share {
     Request what;
-    int request, rows, chunk, chunks, run, index0;
+    int request, rows, chunk, chunks, run, place, head;
+    bool alone;
 };
+// How a request is taken apart: whole runs, and a rest or not; or alone.
+struct Parts {
+    int runs, rest, alone;
+};
+__device__ __forceinline__ Parts parts_of(int positions, int run, float by_run) {
+    Parts p = {0, 0, 0};
+    if (positions * kWaves <= run) {  // (rows that see nothing are among them)
+        p.alone = 1;
+        return p;
+    }
+    // positions / run from the quotient in fp32, which is off by one at most
+    p.runs = (int)((float)positions * by_run);
+    while ((int64_t)(p.runs + 1) * run <= positions) ++p.runs;
+    while ((int64_t)p.runs * run > positions) --p.runs;
+    p.rest = p.runs * run < positions;
+    return p;
+}
 // Every wave finds it for itself.  Position tiles times row tiles of all requests, over the workgroups there are, give the run's
-// length; requests in order take one workgroup for each run.
-__device__ __forceinline__ bool find_share(const KvAttentionArgs& a, int index, Share& s) {
-    const int lane = threadIdx.x & 63;
+// length.  Whole runs come first, request after request, then the rests, then what is done alone: what takes longest starts first.
+__device__ __forceinline__ bool find_share(const KvAttentionArgs& a, Share& s) {
+    const int lane = threadIdx.x & 63, heads = a.cache.heads;
     const auto add_f = [](unsigned x, unsigned y) { return __builtin_bit_cast(unsigned, __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y)); };
     const auto add_u = [](unsigned x, unsigned y) { return x + y; };
     Request q = {0, 0, 0};
@@ -124,41 +143,67 @@ __device__ __forceinline__ bool find_share(const KvAttentionArgs& a, int index, 
     int run = run_f < 1.0e9f ? (int)run_f + 1 : 1 << 30;
     run = __builtin_amdgcn_readfirstlane((run + kWaves - 1) / kWaves * kWaves);
     const float by_run = 1.0f / (float)run;
-    unsigned before = 0;
-    for (int base = 0; base < a.requests; base += 64) {
-        if (a.requests > 64) {
-            const int r = base + lane;
-            q = Request{0, 0, 0};
-            if (r < a.requests) q = request_of(a, r);
+    const unsigned index = blockIdx.x / (unsigned)heads;
+    s.run = run;
+    s.head = (int)(blockIdx.x - index * (unsigned)heads);
+    // The first round over the requests looks for `index` among the whole runs, the second among the rests and what is done alone; the
+    // sums up to a request tell where its places begin.
+    unsigned all_runs = 0, all_rests = 0, alone_index = 0;
+    bool alone = false;
+    for (int round = 0; round < 2; ++round) {
+        unsigned runs = 0, rests = 0, alones = 0;
+        for (int base = 0; base < a.requests; base += 64) {
+            if (a.requests > 64) {
+                const int r = base + lane;
+                q = Request{0, 0, 0};
+                if (r < a.requests) q = request_of(a, r);
+            }
+            const int tiles = row_tiles(a, q);
+            const Parts p = parts_of(position_tiles(q), run, by_run);
+            const int64_t want = (int64_t)tiles * p.runs;
+            const unsigned some = tiles < (1 << 24) ? (unsigned)tiles : 1u << 24;  // (more than any grid has: offsets that fall and rise again)
+            const unsigned my_runs = want < (1 << 24) ? (unsigned)want : 1u << 24, my_rests = some * (unsigned)p.rest, my_alones = some * (unsigned)p.alone;
+            const unsigned upto_runs = runs + sums_upto(my_runs, add_u), upto_rests = rests + sums_upto(my_rests, add_u);
+            unsigned upto = upto_runs, looked_for = index;
+            if (round == 1) {
+                const unsigned upto_alones = alones + sums_upto(my_alones, add_u);
+                upto = alone ? upto_alones : all_runs + upto_rests;
+                looked_for = alone ? alone_index : index;
+                alones = lane_value(upto_alones, 63);
+            }
+            const unsigned long long above = __ballot(upto > looked_for);
+            if (above) {
+                const int owner = __builtin_ctzll(above);
+                s.what = Request{(int)lane_value((unsigned)q.first, owner), (int)lane_value((unsigned)q.count, owner),
+                                 (int)lane_value((unsigned)q.length, owner)};
+                s.request = base + owner;
+                s.alone = alone;
+                const int r = (int)lane_value((unsigned)p.runs, owner);
+                s.chunks = alone ? 1 : r + (int)lane_value((unsigned)p.rest, owner);
+                const unsigned before_runs = lane_value(upto_runs - my_runs, owner), before_rests = lane_value(upto_rests - my_rests, owner);
+                if (round == 0) {
+                    const int at = (int)(index - before_runs);
+                    s.rows = r == 1 ? at : at / r;
+                    s.chunk = at - s.rows * r;
+                } else {
+                    s.rows = (int)(looked_for - lane_value(upto - (alone ? my_alones : my_rests), owner));
+                    s.chunk = alone ? 0 : r;
+                }
+                s.place = (int)(before_runs + before_rests) + s.rows * s.chunks + s.chunk;
+                return true;
+            }
+            runs = lane_value(upto_runs, 63);
+            rests = lane_value(upto_rests, 63);
+            if ((runs | rests | alones) > 0x1fffffffu) return false;
         }
-        const int tiles = row_tiles(a, q), positions = position_tiles(q);
-        // positions / run rounded up, from the quotient in fp32, which is off by one at most
-        int chunks = 1;
-        if (positions > run) {
-            chunks = (int)((float)positions * by_run);
-            while ((int64_t)chunks * run < positions) ++chunks;
-            while ((int64_t)(chunks - 1) * run >= positions) --chunks;
+        all_runs = runs;
+        all_rests = rests;
+        if (round == 0 && index >= all_runs + all_rests) {
+            alone = true;
+            const unsigned groups = (unsigned)(heads + kWaves - 1) / kWaves, at = blockIdx.x - (all_runs + all_rests) * (unsigned)heads;
+            alone_index = at / groups;
+            s.head = (int)(at - alone_index * groups) * kWaves + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
         }
-        const int64_t want = (int64_t)tiles * chunks;
-        const unsigned mine = want < (1 << 25) ? (unsigned)want : 1u << 25;  // (more than any grid has: offsets that fall and rise again)
-        const unsigned upto = sums_upto(mine, add_u);
-        const unsigned long long above = __ballot((uint64_t)before + upto > (uint64_t)index);
-        if (above) {
-            const int owner = __builtin_ctzll(above);
-            const int start = (int)(before + lane_value(upto - mine, owner));
-            s.chunks = (int)lane_value((unsigned)chunks, owner);
-            s.what = Request{(int)lane_value((unsigned)q.first, owner), (int)lane_value((unsigned)q.count, owner),
-                             (int)lane_value((unsigned)q.length, owner)};
-            s.request = base + owner;
-            const int at = index - start;
-            s.rows = s.chunks == 1 ? at : at / s.chunks;
-            s.chunk = at - s.rows * s.chunks;
-            s.run = run;
-            s.index0 = index - s.chunk;
-            return true;
-        }
-        before += lane_value(upto, 63);
-        if (before > 0x7fffffffu) return false;
     }
     return false;
 }
@@ -177,20 +222,23 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
     __shared__ float merge_m[kWaves * 16], merge_l[kWaves * 16];
     __shared__ int last_flag;
     const KvCache& c = a.cache;
-    const int heads = c.heads, kv_head = (int)(blockIdx.x % (unsigned)heads), index = (int)(blockIdx.x / (unsigned)heads);
+    const int heads = c.heads;
     Share s;
-    if (!find_share(a, index, s)) return;
+    if (!find_share(a, s)) return;
+    const bool head_exists = s.head < heads;  // (of four heads that are done alone some may not)
+    const int kv_head = head_exists ? s.head : heads - 1;
     const Request rq = s.what;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, quad = lane >> 4;
     const int rows_total = rq.count * a.group, flat = s.rows * kRows + col;
-    const bool row_exists = flat < rows_total;
+    const bool row_exists = flat < rows_total && head_exists;
     const int token = row_exists ? query_of(a, flat) : 0, sub_head = row_exists ? flat - token * a.group : 0;
     // positions that the lane's row sees; the first and the last row of the tile have the fewest and the most
     const int limit = row_exists ? rq.length - rq.count + token + 1 : 0;
     const int last_flat = rows_total - 1 < s.rows * kRows + kRows - 1 ? rows_total - 1 : s.rows * kRows + kRows - 1;
     const int seen_by_all = rq.length - rq.count + query_of(a, s.rows * kRows) + 1, seen_by_any = rq.length - rq.count + query_of(a, last_flat) + 1;
     const int tiles = (seen_by_any + kTile - 1) / kTile;
-    const int end = (s.chunk + 1) * s.run < tiles ? (s.chunk + 1) * s.run : tiles;
+    const int end = s.alone ? (head_exists ? tiles : 0) : ((s.chunk + 1) * s.run < tiles ? (s.chunk + 1) * s.run : tiles);
+    const int step = s.alone ? 1 : kWaves;
 
     const int32_t* table = a.table + (int64_t)s.request * a.columns;
     const int last_column = rq.length > 0 ? (rq.length - 1) >> c.page_shift : 0;
@@ -221,24 +269,26 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
         }
         return x;
     };
-    int t = s.chunk * s.run + wave;
+    int t = s.alone ? 0 : s.chunk * s.run + wave;
     Pages pages = pages_of(t);
-    Positions<S> next = {};
-    if (t < end) next = load(t, pages);
-    Pages next_pages = pages_of(t + kWaves);
-
     h8 q[S];
-    float q_sum = 0.f;
     {
         const half_t* row = a.q + (int64_t)(rq.first + token) * a.q_row + (int64_t)(kv_head * a.group + sub_head) * a.q_head;
 #pragma unroll
         for (int i = 0; i < S; ++i) {
             q[i] = h8{};
             if (row_exists) q[i] = load_eight_of(row, 8 * (S * quad + i), c.k_dim);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) q_sum += (float)q[i][j];
         }
     }
+    Positions<S> next = {};
+    if (t < end) next = load(t, pages);
+    Pages next_pages = pages_of(t + step);
+
+    float q_sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q_sum += (float)q[i][j];
     q_sum = quad_sum(q_sum);
     const float log2e = 1.4426950408889634f;
     const float by_code = a.scale * log2e * 16777216.0f, by_sum = -8.0f * q_sum * a.scale * log2e;
@@ -248,7 +298,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
     for (int i = 0; i < 8; ++i) out[i] = f4{0.f, 0.f, 0.f, 0.f};
     float m = kNoMaximum, l = 0.f, w_sum = 0.f;
 
-    for (; t < end; t += kWaves) {
+    for (; t < end; t += step) {
         const int j0 = t * kTile;
         typename Words<S>::type kw[4];
         u32x4 vw[4];
@@ -259,8 +309,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
             if ((unsigned)pages.page[u] >= (unsigned)c.pages) ks[u] = 0x7e007e007e007e00ull;  // no such page: NaN
         }
         pages = next_pages;
-        if (t + kWaves < end) next = load(t + kWaves, pages);
-        next_pages = pages_of(t + 2 * kWaves);
+        if (t + step < end) next = load(t + step, pages);
+        next_pages = pages_of(t + 2 * step);
         float score[16];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -364,7 +414,33 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
         merge_l[wave * 16 + col] = l;
     }
     __syncthreads();
-    // a thread: eight channels of a row
+    // eight channels of a row
+    auto finish = [&](int row, int head, int channel, const float (&o)[8], float sum) __attribute__((always_inline)) {
+        const int of_token = query_of(a, row), q_head = head * a.group + row - of_token * a.group;
+        const bool empty = rq.length - rq.count + of_token + 1 <= 0;
+        half_t* to = a.out + (int64_t)(rq.first + of_token) * a.out_row + (int64_t)q_head * a.out_head + channel;
+        h8u result;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) result[i] = empty ? (half_t)0.f : (half_t)(o[i] / sum);
+        if (channel + 8 <= c.v_dim) {
+            *reinterpret_cast<h8u*>(to) = result;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (channel + i < c.v_dim) to[i] = result[i];
+        }
+    };
+    if (s.alone) {
+        for (int i = 0; i < 4; ++i) {
+            const int row = 4 * i + quad, flat_row = s.rows * kRows + row;
+            if (flat_row >= rows_total || !head_exists) break;
+            const float* from = merge + (wave * 16 + row) * kOutStride + 8 * col;
+            const float mine[8] = {from[0], from[1], from[2], from[3], from[4], from[5], from[6], from[7]};
+            finish(flat_row, kv_head, 8 * col, mine, merge_l[wave * 16 + row]);
+        }
+        return;
+    }
+    // a thread: eight channels of a row, of all four waves' positions
     int my_row = tid >> 4;
     const int my_channel = 8 * (tid & 15);
     float top = kNoMaximum, sum = 0.f, o[8] = {};
@@ -384,7 +460,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
         // The exchange: relaxed stores at device scope, which pass the local L2; a wait until they have been acknowledged; the
         // barrier; the count.  The last to arrive reads with relaxed loads at device scope.
         const __amdgpu_buffer_rsrc_t slot =
-            __builtin_amdgcn_make_buffer_rsrc(a.temp + (int64_t)blockIdx.x * kSlotFloats, 0, (unsigned)kSlotFloats * 4u, 0x00020000);
+            __builtin_amdgcn_make_buffer_rsrc(a.temp + ((int64_t)s.place * heads + kv_head) * kSlotFloats, 0, (unsigned)kSlotFloats * 4u, 0x00020000);
         if (mine) {
             const uint32_t at = 4u * (uint32_t)(my_row * 128 + my_channel);
             __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f4{o[0], o[1], o[2], o[3]}), slot, at, 0, kDeviceScope);
@@ -395,7 +471,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        unsigned* count = reinterpret_cast<unsigned*>(a.accum) + (int64_t)s.index0 * heads + kv_head;
+        unsigned* count = reinterpret_cast<unsigned*>(a.accum) + (int64_t)(s.place - s.chunk) * heads + kv_head;
         if (tid == 0) last_flag = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)s.chunks - 1;
         __syncthreads();
         if (!last_flag) return;
@@ -416,7 +492,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int from = first + k * slices < s.chunks ? first + k * slices : first;
-                const __amdgpu_buffer_rsrc_t part = __builtin_amdgcn_make_buffer_rsrc(a.temp + ((int64_t)s.index0 * heads + kv_head) * kSlotFloats, 0,
+                const __amdgpu_buffer_rsrc_t part = __builtin_amdgcn_make_buffer_rsrc(a.temp + ((int64_t)(s.place - s.chunk) * heads + kv_head) * kSlotFloats, 0,
                                                                                       0xffffffffu, 0x00020000);
                 const uint32_t at = 4u * (uint32_t)from * (uint32_t)(heads * kSlotFloats);
                 lo[k] = __builtin_amdgcn_raw_buffer_load_b128(part, at + 4u * (uint32_t)(my_row * 128 + my_channel), 0, kDeviceScope);
@@ -461,19 +537,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
     } else if (!mine) {
         return;
     }
-    const int my_token = query_of(a, my_flat), my_head = kv_head * a.group + my_flat - my_token * a.group;
-    const bool empty = rq.length - rq.count + my_token + 1 <= 0;
-    half_t* to = a.out + (int64_t)(rq.first + my_token) * a.out_row + (int64_t)my_head * a.out_head + my_channel;
-    h8u result;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) result[i] = empty ? (half_t)0.f : (half_t)(o[i] / sum);
-    if (my_channel + 8 <= c.v_dim) {
-        *reinterpret_cast<h8u*>(to) = result;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (my_channel + i < c.v_dim) to[i] = result[i];
-    }
+    finish(my_flat, kv_head, my_channel, o, sum);
 }
 
 // Workgroups for each key / value head: one for each run, and one more for each row tile whose last run is not whole.
