@@ -258,3 +258,27 @@ def test_store_captured_and_replayed(gpu):
                     assert torch.equal(a[s // 16, :, s % 16 // 4, :, s % 4], b[s // 16, :, s % 16 // 4, :, s % 4])
                 else:
                     assert torch.equal(a[s // 16, :, s % 16], b[s // 16, :, s % 16])
+
+
+def test_a_cache_whose_tensors_are_replaced_or_copied(gpu):
+    """calls follow the module's own tensors: after an assignment, a move, a copy"""
+    import copy
+    import pickle
+    x = torch.randn(20, 2, 40, generator=torch.Generator().manual_seed(1)).half()
+    slots, table = torch.arange(20, device=gpu), torch.arange(2, dtype=torch.int32, device=gpu)[None]
+    cu = torch.tensor([0, 20], dtype=torch.int32, device=gpu)
+    want = as_held(x)[0].half()
+    cache = new_cache(gpu, 2, 16, 2, 40, 40)
+    cache.store(x.to(gpu), x.to(gpu), slots)
+    other = copy.deepcopy(cache)
+    third = pickle.loads(pickle.dumps(cache))
+    old = cache.k_scales
+    cache.k_scales = torch.zeros_like(old)
+    assert (cache.load(table, cu, 20)[0] == 0).all() and torch.equal(cache.load(table, cu, 20)[1].cpu(), want)
+    cache.k_scales = old
+    moved = cache.cpu().to(gpu)
+    for c in (cache, other, third, moved):
+        k, v = c.load(table, cu, 20)
+        assert torch.equal(k.cpu(), want) and torch.equal(v.cpu(), want)
+    other.store(torch.zeros_like(x).to(gpu), torch.zeros_like(x).to(gpu), slots)
+    assert (other.load(table, cu, 20)[0] == 0).all() and torch.equal(cache.load(table, cu, 20)[0].cpu(), want)

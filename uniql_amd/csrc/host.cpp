@@ -12,6 +12,7 @@
 // strided rows, allocations and launches may all wait for the device - but for that map and the accumulator's lookup.
 #include <torch/extension.h>
 
+#include <cmath>
 #include <map>
 #include <optional>
 #include <stdexcept>
@@ -346,4 +347,11 @@ PYBIND11_MODULE(_host, module) {
     module.def("kv4_load", &kv4_load);
     module.def("kv4_attention", &kv4_attention);
     module.def("prompt_attention", &prompt_attention);
+    py::class_<KvPool>(module, "KvPool")
+        .def(py::init([](Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, int64_t k_dim, int64_t v_dim) {
+            return KvPool{std::move(k_codes), std::move(k_scales), std::move(v_codes), std::move(v_scales), k_dim, v_dim};
+        }))
+        .def("store", &pool_store)
+        .def("load", &pool_load)
+        .def("attend", &pool_attend);
 }

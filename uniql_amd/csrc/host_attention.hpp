@@ -230,3 +230,28 @@ Tensor prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
           "uniql_prompt_attention");
     return out;
 }
+
+// The tensors of a module's cache, so that a call does not hand them over one by one (1 us for the four and 1.2 for a module to look
+// its buffers up); every call checks them as it would the caller's.
+struct KvPool {
+    Tensor k_codes, k_scales, v_codes, v_scales;
+    int64_t k_dim, v_dim;
+};
+void require_width(const Tensor& t, const char* name, int64_t width) {
+    if (t.dim() == 3 && t.size(2) != width) fail(std::string(name) + " must be " + std::to_string(width) + " wide");
+}
+void pool_store(const KvPool& p, const Tensor& k, const Tensor& v, const Tensor& slots, uintptr_t stream) {
+    require_width(k, "k", p.k_dim);
+    require_width(v, "v", p.v_dim);
+    kv4_store(k, v, slots, p.k_codes, p.k_scales, p.v_codes, p.v_scales, stream);
+}
+std::pair<Tensor, Tensor> pool_load(const KvPool& p, const Tensor& table, const Tensor& cu, int64_t rows, const std::optional<Tensor>& starts,
+                                    const std::optional<Tensor>& k_out, const std::optional<Tensor>& v_out, uintptr_t stream) {
+    return kv4_load(p.k_codes, p.k_scales, p.v_codes, p.v_scales, table, cu, rows, p.k_dim, p.v_dim, starts, k_out, v_out, stream);
+}
+Tensor pool_attend(const KvPool& p, const Tensor& q, const Tensor& table, const Tensor& lengths, const std::optional<Tensor>& cu_q,
+                   std::optional<double> scale, const std::optional<Tensor>& out, uintptr_t stream, const py::object& accumulator) {
+    require_width(q, "q", p.k_dim);
+    return kv4_attention(q, p.k_codes, p.k_scales, p.v_codes, p.v_scales, table, lengths, p.v_dim, cu_q,
+                         scale ? *scale : 1.0 / std::sqrt((double)p.k_dim), out, stream, accumulator);
+}

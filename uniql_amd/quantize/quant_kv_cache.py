@@ -19,7 +19,7 @@ from typing import NamedTuple
 import torch
 import torch.nn as nn
 
-from .. import ops
+from .. import _capi, ops
 
 
 class KVStep(NamedTuple):
@@ -83,29 +83,45 @@ class W4KVCache(nn.Module):
         self.register_buffer("v_codes", pool(torch.int32, page_size // 4, (self.v_head_dim + 31) // 32 * 4, 4), persistent=False)
         self.register_buffer("v_scales", pool(torch.float16, page_size), persistent=False)
 
+    # The native handle of the four tensors: made at the first call, and anew when one of them has been replaced or moved.
+    def _native(self):
+        handle = self.__dict__.get("_handle")
+        if handle is None:
+            handle = _capi.host().KvPool(self.k_codes, self.k_scales, self.v_codes, self.v_scales, self.head_dim, self.v_head_dim)
+            self.__dict__["_handle"] = handle
+        return handle
+
+    def __setattr__(self, name, value):
+        if name in ("k_codes", "k_scales", "v_codes", "v_scales", "head_dim", "v_head_dim"):
+            self.__dict__.pop("_handle", None)
+        super().__setattr__(name, value)
+
+    def _apply(self, fn, recurse=True):
+        self.__dict__.pop("_handle", None)
+        return super()._apply(fn, recurse)
+
+    def __getstate__(self):
+        state = self.__dict__.copy()
+        state.pop("_handle", None)
+        return state
+
     def store(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Quantises k [tokens, kv heads, head_dim] and v [tokens, kv heads, v_head_dim] into the places `slots` (int64 [tokens]; -1
         is left out, none may occur twice)."""
-        if k.dim() == 3 and v.dim() == 3 and (k.shape[2] != self.head_dim or v.shape[2] != self.v_head_dim):
-            raise RuntimeError(f"k and v must be {self.head_dim} and {self.v_head_dim} wide")
-        ops.kv4_store(k, v, slots, self.k_codes, self.k_scales, self.v_codes, self.v_scales)
+        self._native().store(k, v, slots, ops._stream_of(k, "k"))
 
     def load(self, table: torch.Tensor, cu: torch.Tensor, rows: int, starts: torch.Tensor | None = None,
              k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None):
         """(k, v) in fp16, packed by request: rows cu[r] .. cu[r + 1] are the positions from starts[r] (0 when None) on.  For
         prompts taken in pieces: prompt_attention(q, *load(..), cu_q, cu) sees what attend would."""
-        return ops.kv4_load(self.k_codes, self.k_scales, self.v_codes, self.v_scales, table, cu, rows, self.head_dim, self.v_head_dim,
-                            starts=starts, k_out=k_out, v_out=v_out)
+        return self._native().load(table, cu, rows, starts, k_out, v_out, ops._stream_of(table, "table"))
 
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, cu_q: torch.Tensor | None = None,
                scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of each request's newest tokens, q [rows, q heads, head_dim], over its pages; the tokens' own keys and values
         have been stored and count in `lengths`.  cu_q int32 [requests + 1]: rows of each request (None: one each).
         Returns [rows, q heads, v_head_dim]."""
-        if q.dim() == 3 and q.shape[2] != self.head_dim:
-            raise RuntimeError(f"q must be {self.head_dim} wide")
-        return ops.kv4_attention(q, self.k_codes, self.k_scales, self.v_codes, self.v_scales, table, lengths, self.v_head_dim, cu_q=cu_q,
-                                 scale=scale, out=out)
+        return self._native().attend(q, table, lengths, cu_q, scale, out, ops._stream_of(q, "q"), ops._accumulator)
 
     def __repr__(self):
         return (f"W4KVCache(num_pages={self.num_pages}, page_size={self.page_size}, num_kv_heads={self.num_kv_heads}, "
