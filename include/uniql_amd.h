@@ -410,7 +410,7 @@ typedef struct uniql_kv4_cache {
  *   slots        device out, int64 [max_tokens]: each token's place; -1 for tokens of refused requests and behind the last
  *   positions    device out, int32 [max_tokens]: each token's position in its request; 0 where slots is -1
  *   refused      device out, int32 [rows]: 1 where a request with new tokens was refused
- * columns <= 2^20, columns * page_size <= 2^30, rows * columns < 2^31, max_tokens <= 2^30.  Nothing outside these arrays is touched
+ * columns <= 2^20, columns * page_size <= 2^30, rows * columns < 2^31, max_tokens <= 2^24.  Nothing outside these arrays is touched
  * whatever they hold; lengths below 0 count as 0 where a request ends and are refused otherwise.
  */
 int uniql_kv_assign_pages(const int32_t* new_tokens, const int32_t* lengths, int32_t* table, int32_t* free_pages,

@@ -37,7 +37,7 @@ def test_assign(lib):
         return lib.uniql_kv_assign_pages(*{**args, **kw}.values())
 
     for kw, code in [(dict(rows=-1), -2), (dict(columns=0), -2), (dict(columns=(1 << 20) + 1), -2), (dict(pool=-1), -2), (dict(page=15), -2),
-                     (dict(most=-1), -2), (dict(most=(1 << 30) + 1), -2), (dict(columns=1 << 20, rows=4096), -2),
+                     (dict(most=-1), -2), (dict(most=(1 << 24) + 1), -2), (dict(columns=1 << 20, rows=4096), -2),
                      (dict(columns=1 << 20, rows=1, page=256, new=None), -1)]:
         assert call(**kw) == code, kw
     for name in ("new", "lengths", "table", "free", "count", "lengths_out", "count_out", "slots", "positions", "cu", "refused"):

@@ -58,7 +58,7 @@ extern "C" {
 int uniql_kv_assign_pages(const int32_t* new_tokens, const int32_t* lengths, int32_t* table, int32_t* free_pages,
                           const int32_t* free_count, int32_t* lengths_out, int32_t* free_count_out, int64_t* slots, int32_t* positions,
                           int32_t* cu, int32_t* refused, int rows, int columns, int pool, int page_size, int max_tokens, void* stream) {
-    if (rows < 0 || pool < 0 || max_tokens < 0 || max_tokens > (1 << 30) || !page_size_ok(page_size) ||
+    if (rows < 0 || pool < 0 || max_tokens < 0 || max_tokens > (1 << 24) || !page_size_ok(page_size) ||
         !columns_ok(rows, columns, page_size))
         return UNIQL_E_SHAPE;
     if (!free_count || !free_count_out || !cu) return UNIQL_E_NULL;

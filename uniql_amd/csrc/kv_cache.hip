@@ -19,22 +19,27 @@ struct AssignArgs {
 };
 constexpr int kAssignThreads = 1024;
 
-// Sums over the workgroup's threads up to and including each; `total` is the whole sum.
-template <typename T>
-__device__ __forceinline__ T scan_inclusive(T v, T* wave_sums, T& total) {
+// Sums over the workgroup's threads up to and including each, and the whole sum; within a wave in 32 bits.  wave_sums is the scan's own:
+// between two uses of it all threads have met.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned add_from(unsigned v) {
+    return v + (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int64_t scan_inclusive(unsigned v, unsigned* wave_sums, int64_t& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const T other = __shfl_up(v, d, 64);
-        if (lane >= d) v += other;
-    }
-    __syncthreads();  // the sums of an earlier scan have been read
+    v = add_from<0x111, 0xf>(v);  // one, two, four, eight lanes below, within sixteen
+    v = add_from<0x112, 0xf>(v);
+    v = add_from<0x114, 0xf>(v);
+    v = add_from<0x118, 0xf>(v);
+    v = add_from<0x142, 0xa>(v);  // the last of the sixteen below, for the second and fourth sixteen
+    v = add_from<0x143, 0xc>(v);  // lane 31, for the upper half
     if (lane == 63) wave_sums[wave] = v;
     __syncthreads();
-    T before = 0;
+    int64_t before = 0;
     total = 0;
+#pragma unroll
     for (int w = 0; w < kAssignThreads / 64; ++w) {
-        const T s = wave_sums[w];
+        const unsigned s = wave_sums[w];
         if (w < wave) before += s;
         total += s;
     }
@@ -70,60 +75,65 @@ __device__ __forceinline__ void place_token(const AssignArgs& a, int t, int requ
 // PLACE: it also places the tokens (a small batch: no second launch).
 template <bool PLACE>
 __global__ __launch_bounds__(kAssignThreads) void kv_assign_kernel(const AssignArgs a) {
-    __shared__ int64_t sums64[kAssignThreads / 64];
-    __shared__ int sums[kAssignThreads / 64], upto[kAssignThreads], upto_tokens[kAssignThreads], held_by[kAssignThreads], used;
+    __shared__ unsigned sums[3][kAssignThreads / 64];
+    __shared__ int upto[kAssignThreads], upto_tokens[kAssignThreads], held_by[kAssignThreads], used;
     const int tid = threadIdx.x;
     const int page = 1 << a.page_shift;
     const int64_t capacity = (int64_t)a.columns << a.page_shift;
     if (tid == 0) used = 0;
+    // what the first rows ask for and hold is read once, with the count
+    const int first_asked = tid < a.rows ? a.new_tokens[tid] : 0, first_held = tid < a.rows ? a.lengths[tid] : 0;
     int count = *a.free_count;
     count = count < 0 ? 0 : (count > a.pool ? a.pool : count);
     for (int base = 0; base < a.rows; base += kAssignThreads) {
         const int r = base + tid;
         int pages = 0;
-        if (r < a.rows && a.new_tokens[r] < 0) {
-            int64_t n = a.lengths[r];
+        if (r < a.rows && (base == 0 ? first_asked : a.new_tokens[r]) < 0) {
+            int64_t n = base == 0 ? first_held : a.lengths[r];
             n = n < 0 ? 0 : (n > capacity ? capacity : n);
             pages = (int)((n + page - 1) >> a.page_shift);
         }
-        int total;
-        const int sum = scan_inclusive(pages, sums, total);
-        if (total == 0) continue;  // uniform
-        upto[tid] = sum;
-        held_by[tid] = pages;
-        __syncthreads();
-        for (int i = tid; i < total; i += kAssignThreads) {
-            const int row = first_above(upto, kAssignThreads, i), j = i - (upto[row] - held_by[row]);
-            if (count + i < a.pool) a.free_pages[count + i] = a.table[(int64_t)(base + row) * a.columns + j];
+        int64_t released;
+        const int sum = (int)scan_inclusive((unsigned)pages, sums[0], released);
+        const int total = (int)released;  // at most 2^30
+        if (total > 0) {
+            upto[tid] = sum;
+            held_by[tid] = pages;
+            __syncthreads();
+            for (int i = tid; i < total; i += kAssignThreads) {
+                const int row = first_above(upto, kAssignThreads, i), j = i - (upto[row] - held_by[row]);
+                if (count + i < a.pool) a.free_pages[count + i] = a.table[(int64_t)(base + row) * a.columns + j];
+            }
+            count = total > a.pool - count ? a.pool : count + total;
         }
-        count = total > a.pool - count ? a.pool : count + total;
+        __syncthreads();  // (the sums have been read; released pages are on the list)
     }
-    __syncthreads();  // released pages are on the list
     int64_t tokens_before = 0;
     int64_t pages_before = 0;
     for (int base = 0; base < a.rows; base += kAssignThreads) {
         const int r = base + tid;
         const bool exists = r < a.rows;
-        const int asked = exists ? a.new_tokens[r] : 0, n = asked > 0 ? asked : 0;
-        const int64_t old = exists ? a.lengths[r] : 0;
+        const int asked = base == 0 ? first_asked : (exists ? a.new_tokens[r] : 0), n = asked > 0 ? asked : 0;
+        const int64_t old = base == 0 ? first_held : (exists ? a.lengths[r] : 0);
         int64_t tokens, pages_total;
-        const int64_t sum_tokens = tokens_before + scan_inclusive((int64_t)n, sums64, tokens);
+        // (more than max_tokens count as one more)
+        const int64_t sum_tokens = tokens_before + scan_inclusive((unsigned)(n <= a.max_tokens ? n : a.max_tokens + 1), sums[1], tokens);
         const bool fits = n > 0 && old >= 0 && old + n <= capacity && sum_tokens <= a.max_tokens;
         const int held = (int)((old + page - 1) >> a.page_shift);
         const int need = fits ? (int)((old + n + page - 1) >> a.page_shift) - held : 0;
-        const int64_t sum_pages = pages_before + scan_inclusive((int64_t)need, sums64, pages_total);
+        const int64_t sum_pages = pages_before + scan_inclusive((unsigned)need, sums[2], pages_total);
         const bool served = fits && (need == 0 || sum_pages <= count);
+        const int end = sum_tokens < a.max_tokens ? (int)sum_tokens : a.max_tokens;
+        if (PLACE) upto_tokens[tid] = end;
         if (exists) {
-            a.cu[r + 1] = sum_tokens < a.max_tokens ? (int)sum_tokens : a.max_tokens;
+            a.cu[r + 1] = end;
             a.refused[r] = n > 0 && !served;
             a.lengths_out[r] = asked < 0 ? 0 : (int)(served ? old + n : old);
         }
         // those that are served and need pages come before all that are refused for want of them
-        __syncthreads();
         const int64_t mine = sum_pages - pages_before;
         upto[tid] = (int)(mine < 0x7fffffff ? mine : 0x7fffffff);
-        held_by[tid] = (int)(need != 0 ? need : 0) ;
-        if (PLACE) upto_tokens[tid] = exists ? a.cu[r + 1] : a.max_tokens;
+        held_by[tid] = need;
         __shared__ int first_page[kAssignThreads], old_or_none[kAssignThreads];
         first_page[tid] = held;
         old_or_none[tid] = served ? (int)old : -1;
@@ -145,6 +155,7 @@ __global__ __launch_bounds__(kAssignThreads) void kv_assign_kernel(const AssignA
         }
         tokens_before += tokens;
         pages_before += pages_total;
+        __syncthreads();
     }
     if (PLACE && a.rows == 0)
         for (int t = tid; t < a.max_tokens; t += kAssignThreads) place_token(a, t, 0, 0, -1);
