@@ -4,9 +4,11 @@
 // A workgroup takes 16 rows (query heads of one key / value head, of one or several tokens) of a request over a run of positions;
 // its four waves take 64 positions in turn.  Both products are matrix instructions of 16 x 16 x 32 on fp16 with the codes as they are: a code
 // c in an fp16 number's low bits is the subnormal c 2^-24 (c 2^-20 four bits higher), which the instruction multiplies exactly, so that a
-// pair of codes costs one mask.  The 8 that belongs off the codes and the scales come in around the products:
+// pair of codes costs one mask.  Scales and, of the keys, the 8 that belongs off the codes come in around the products:
 //   scores   scale s_j (2^24 (q . c_j 2^-24) - 8 sum q)      positions along the rows of the first product, so that
-//   output   2^24 sum_j w_j (c'_j 2^-24) - 8 sum_j w_j       its results are the second one's operand in the lanes where they are
+//   output   2^24 sum_j w_j ((c'_j - 8) 2^-24)               its results are the second one's operand in the lanes where they are
+// (The values' 8 is taken off in front of the product, one more instruction a pair: behind it, over 65536 positions, the difference of two sums
+// 80 times as large as itself was four times as far from the exact result.)
 // with w_j = fp16(p_j s'_j).  For w_j to use fp16's range whatever the values' sizes, m is the running maximum of the scores plus
 // the exponent of s'_j: w_j <= 1 at the maximum, and it moves only when some w_j would pass 2^8.
 // The rounding of w_j (2^-11) is what a matrix instruction on fp16 asks for; sums, maxima and the output stay in fp32.
@@ -55,7 +57,12 @@ __device__ __forceinline__ float quad_sum(float v) {
     v += __shfl_xor(v, 16, 64);
     return v + __shfl_xor(v, 32, 64);
 }
+// Codes of two positions a word, less eight: exact, subnormal numbers and sums of them.
+__device__ __forceinline__ uint32_t less_eight(uint32_t codes, uint32_t eight) { return h2_to_bits(bits_to_h2(codes) + bits_to_h2(eight)); }
 __device__ __forceinline__ h8 halves(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __builtin_bit_cast(h8, u32x4{a, b, c, d}); }
+__device__ __forceinline__ h8 values_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t mask, uint32_t eight) {
+    return halves(less_eight(a & mask, eight), less_eight(b & mask, eight), less_eight(c & mask, eight), less_eight(d & mask, eight));
+}
 
 // What a request asks for: its rows [first, first + count) and the positions in the cache.
 struct Request {
@@ -244,6 +251,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
     const int last_column = rq.length > 0 ? (rq.length - 1) >> c.page_shift : 0;
     const int n_word = col < c.v_words ? col : 0;
     const uint32_t mask_low = 0x000f000fu, mask_high = 0x00f000f0u;
+    const uint32_t eight_low = 0x80088008u, eight_high = 0x80808080u;  // -8 2^-24 and -8 2^-20, twice
     struct Pages {
         int page[4];
     };
@@ -296,7 +304,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
     f4 out[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) out[i] = f4{0.f, 0.f, 0.f, 0.f};
-    float m = kNoMaximum, l = 0.f, w_sum = 0.f;
+    float m = kNoMaximum, l = 0.f;
 
     for (; t < end; t += step) {
         const int j0 = t * kTile;
@@ -359,7 +367,6 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
             const float fade = __builtin_amdgcn_exp2f(m - next);
             m = next;
             l *= fade;
-            w_sum *= fade;
 #pragma unroll
             for (int i = 0; i < 8; ++i) out[i] *= fade;
         }
@@ -375,9 +382,6 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
                     l += p;
                     weight[4 * h + i] = (half_t)(p * (float)__builtin_bit_cast(half_t, (uint16_t)(vs[u] >> (16 * i))));
                 }
-            const h2 one = {(half_t)1.f, (half_t)1.f};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w_sum = __builtin_amdgcn_fdot2(h2{weight[2 * i], weight[2 * i + 1]}, one, w_sum, false);
             const u32x4 first = vw[2 * k], second = vw[2 * k + 1];
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
@@ -386,15 +390,12 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
                 const uint32_t x0 = __builtin_amdgcn_perm(first[1], first[0], pick), x1 = __builtin_amdgcn_perm(first[3], first[2], pick);
                 const uint32_t x2 = __builtin_amdgcn_perm(second[1], second[0], pick), x3 = __builtin_amdgcn_perm(second[3], second[2], pick);
                 const int low = 4 * (b & 1) + (b >> 1), high = low + 2;
-                out[low] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(x0 & mask_low, x1 & mask_low, x2 & mask_low, x3 & mask_low), weight,
-                                                                  out[low], 0, 0, 0);
-                out[high] = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(x0 & mask_high, x1 & mask_high, x2 & mask_high, x3 & mask_high),
-                                                                   weight, out[high], 0, 0, 0);
+                out[low] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values_of(x0, x1, x2, x3, mask_low, eight_low), weight, out[low], 0, 0, 0);
+                out[high] = __builtin_amdgcn_mfma_f32_16x16x32_f16(values_of(x0, x1, x2, x3, mask_high, eight_high), weight, out[high], 0, 0, 0);
             }
         }
     }
     l = quad_sum(l);
-    w_sum = quad_sum(w_sum);
     // the lane's row: channels 32 quad + 8 i + (0 .. 7); value index 2, 3, 6, 7 came from the high nibbles
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -403,8 +404,8 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float unit = (j & 2) ? 1048576.0f : 16777216.0f;
-            lo[j] = out[j][i] * unit - 8.f * w_sum;
-            hi[j] = out[4 + j][i] * unit - 8.f * w_sum;
+            lo[j] = out[j][i] * unit;
+            hi[j] = out[4 + j][i] * unit;
         }
         *reinterpret_cast<f4*>(to) = lo;
         *reinterpret_cast<f4*>(to + 4) = hi;
