@@ -443,10 +443,10 @@ int uniql_kv4_load(const uniql_kv4_cache* cache, const int32_t* table, const int
  *   q        device, fp16 [rows, n_q_heads, k_dim], unit stride along the last axis, q_row and q_head elements between rows and heads
  *   table    device, int32 [requests, columns];  lengths  device, int32 [requests]: tokens in the cache, the new ones among them
  *   cu_q     device, int32 [requests + 1]: the rows of each request; NULL: one row each (rows == requests)
- *   out      device out, fp16 [rows, n_q_heads, v_dim], strides likewise
+ *   out      device out, fp16 [rows, n_q_heads, v_dim], strides likewise; must not overlap q
  * Row i of a request with t rows sees the positions 0 .. length - t + i.  A row that sees none is 0; rows in front of cu_q[0] and
  * from cu_q[requests] on are left as they were.  What lies in the pages behind a request's length does not matter; a page number
- * outside the pool within it makes the rows that see it NaN.
+ * outside the pool within it makes the rows that see it NaN.  (Offsets that fall count as ones that stay.)
  *   accum, temp   as for uniql_w4a16_gemm: accum all zero on entry and on exit, temp of any contents, neither shared by calls that may
  *                 run at the same time; sizes from uniql_kv4_attention_workspace (bounds that follow from the arguments alone)
  */

@@ -274,3 +274,44 @@ def test_refusals(gpu):
     for bad in ((4, 24, 2, 64), (4, 16, 2, 129), (4, 16, 0, 64), (0, 16, 2, 64)):
         with pytest.raises(ValueError):
             W4KVCache(*bad, device=gpu)
+
+
+def test_offsets_that_fall_leave_no_counts_behind(gpu):
+    """requests whose rows are shared by several workgroups, with offsets that fall and rise again: the words that workgroups count their
+    arrivals in are zeros afterwards, as every later call on the stream relies on"""
+    from uniql_amd import ops
+    p = Problem(gpu, [5000, 4000, 3000, 2000], [40, 30, 20, 10], 8, 1, 64, 64, 64)
+    q, table, lengths, _ = p.on_gpu()
+    for cu in ([0, 100, 0, 100, 0], [100, 0, 100, 0, 100], [50, 20, 90, 10, 100], [0, 2 ** 31 - 1, -5, 2 ** 31 - 1, 7]):
+        p.cache.attend(q, table, lengths, cu_q=torch.tensor(cu, dtype=torch.int32, device=gpu))
+        torch.cuda.synchronize()
+        assert all(int(b.count_nonzero()) == 0 for b in ops._accum_cache.values())
+    p.check(p.run(), 0.125)
+
+
+@pytest.mark.parametrize("requests", [63, 64, 65, 130, 300])
+@pytest.mark.parametrize("several", [False, True])
+def test_many_requests(gpu, requests, several):
+    """more requests than a wave has lanes; lengths from none to a few pages, some of them long"""
+    gen = torch.Generator().manual_seed(requests)
+    lengths = torch.randint(0, 60, (requests,), generator=gen).tolist()
+    lengths[requests // 2], lengths[-1] = 900, 350
+    tokens = torch.randint(0, 3, (requests,), generator=gen).tolist() if several else [1] * requests
+    p = Problem(gpu, lengths, tokens, 4, 2, 32, 32, 16, seed=requests)
+    p.check(p.run(), 32 ** -0.5)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(5, 5), (6, 2), (9, 3), (64, 1), (80, 2)])
+def test_heads_that_do_not_fill_four_waves(gpu, heads, kv_heads):
+    p = Problem(gpu, [30, 700, 64, 1], [1, 1, 2, 1], heads, kv_heads, 64, 64, 16)
+    p.check(p.run(), 0.125)
+
+
+def test_a_scale_that_is_no_number_and_an_output_that_is_the_input(gpu):
+    p = Problem(gpu, [64], [1], 4, 2, 64, 64, 16)
+    q, table, lengths, _ = p.on_gpu()
+    for scale in (float("nan"), float("inf"), 1e300):
+        with pytest.raises(RuntimeError):
+            p.cache.attend(q, table, lengths, scale=scale)
+    with pytest.raises(RuntimeError, match="must not be q"):
+        p.cache.attend(q, table, lengths, out=q)

@@ -282,3 +282,12 @@ def test_a_cache_whose_tensors_are_replaced_or_copied(gpu):
         assert torch.equal(k.cpu(), want) and torch.equal(v.cpu(), want)
     other.store(torch.zeros_like(x).to(gpu), torch.zeros_like(x).to(gpu), slots)
     assert (other.load(table, cu, 20)[0] == 0).all() and torch.equal(cache.load(table, cu, 20)[0].cpu(), want)
+
+
+def test_a_request_without_need_behind_one_that_is_refused(gpu):
+    """it is served, and takes nothing: the pages that the refused one asked for in vain stay free"""
+    got = run_assign(gpu, [40, 1, 20, 3], [0, 5, 0, 10], [[-1] * 4, [7, -1, -1, -1], [-1] * 4, [8, -1, -1, -1]], [4, 6], 10, 16, 64, True)
+    slots, positions, refused, cu, after, count, tab, memory = assign_reference(
+        [40, 1, 20, 3], [0, 5, 0, 10], [[-1] * 4, [7, -1, -1, -1], [-1] * 4, [8, -1, -1, -1]], [4, 6], 16, 64)
+    assert refused == [1, 0, 1, 0] and count == 2
+    assert [got[2], got[4], got[5], got[0], got[6]] == [refused, after, [count], slots, tab]

@@ -214,3 +214,52 @@ def test_refusals(gpu):
         with pytest.raises(RuntimeError, match=words):
             prompt_attention(*args, **kw)
     assert prompt_attention(x[:0], x, x, cu).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("count", [63, 64, 65, 200])
+def test_many_sequences(gpu, count):
+    """more sequences than a wave has lanes, most of them shorter than a tile of rows"""
+    lengths = torch.randint(0, 40, (count,), generator=torch.Generator().manual_seed(count)).tolist()
+    lengths[count // 3] = 300
+    q, k, v, cu, _ = problem(lengths, lengths, 6, 2, 32, 40, seed=count, first=1, behind=3)
+    want, tol = reference(q, k, v, cu, cu, 0.2)
+    got = run(gpu, q, k, v, cu, None, scale=0.2).cpu().double()
+    assert ((got - want).abs() <= tol)[1:-3].all()
+
+
+@pytest.mark.parametrize("h,g", [(7, 7), (12, 4), (20, 4), (33, 1), (64, 1), (130, 1)])
+def test_groups_of_every_kind(gpu, h, g):
+    q, k, v, cu, _ = problem([70, 3, 140], [70, 3, 140], h, g, 48, 32, seed=h)
+    want, tol = reference(q, k, v, cu, cu, 0.15)
+    got = run(gpu, q, k, v, cu, None, scale=0.15).cpu().double()
+    assert ((got - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("d,e", [(2, 2), (10, 12), (30, 62), (66, 34), (94, 96), (98, 126), (126, 130 - 2), (64, 66)])
+@pytest.mark.parametrize("neighbour", [float("nan"), float("inf")])
+def test_rows_whose_neighbours_are_no_numbers(gpu, d, e, neighbour):
+    """even widths, pieces of which reach into other columns of the same rows: what those hold does not matter"""
+    n = 150
+    gen = torch.Generator().manual_seed(d + e)
+    row = 2 * d + 2 * e + 8
+    buf = torch.full((n, row), neighbour).half()
+    q = torch.randn(n, 2, d, generator=gen).half()
+    k, v = buf[:, 2:2 + d].view(n, 1, d), buf[:, d + 4:d + 4 + e].view(n, 1, e)
+    k.copy_(torch.randn(n, 1, d, generator=gen))
+    v.copy_(torch.randn(n, 1, e, generator=gen))
+    want, tol = reference(q, k, v, [0, n], [0, n], 0.2)
+    got = run(gpu, q, k, v, [0, n], None, scale=0.2).cpu().double()
+    assert ((got - want).abs() <= tol).all()
+
+
+def test_a_scale_that_is_no_number_and_an_output_that_is_an_input(gpu):
+    from uniql_amd.attention import prompt_attention
+    x = torch.zeros(8, 4, 64, dtype=torch.float16, device=gpu)
+    cu = torch.tensor([0, 8], dtype=torch.int32, device=gpu)
+    for scale in (float("nan"), float("-inf"), 1e300):
+        with pytest.raises(RuntimeError):
+            prompt_attention(x, x, x, cu, scale=scale)
+    with pytest.raises(RuntimeError, match="must not be"):
+        prompt_attention(x, x, x, cu, out=x)
+    with pytest.raises(RuntimeError, match="must not be"):
+        prompt_attention(x.clone(), x, x.clone(), cu, out=x)

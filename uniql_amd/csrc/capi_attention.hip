@@ -72,7 +72,7 @@ int uniql_kv4_store(const void* k, int64_t k_row, int64_t k_head, const void* v,
                     const uniql_kv4_cache* cache, int tokens, void* stream) {
     KvCache c;
     if (const int code = cache_sizes(cache, c)) return code;
-    if (tokens < 0) return UNIQL_E_SHAPE;
+    if (tokens < 0 || tokens > (1 << 27)) return UNIQL_E_SHAPE;
     if (tokens == 0) return UNIQL_OK;
     if (!k || !v || !slots) return UNIQL_E_NULL;
     if (const int code = cache_pointers(c)) return code;
@@ -83,7 +83,7 @@ int uniql_kv4_load(const uniql_kv4_cache* cache, const int32_t* table, const int
                    int64_t k_head, void* v, int64_t v_row, int64_t v_head, int requests, int columns, int rows, void* stream) {
     KvCache c;
     if (const int code = cache_sizes(cache, c)) return code;
-    if (rows < 0 || requests < 0 || !columns_ok(requests, columns, cache->page_size)) return UNIQL_E_SHAPE;
+    if (rows < 0 || rows > (1 << 27) || requests < 0 || !columns_ok(requests, columns, cache->page_size)) return UNIQL_E_SHAPE;
     if (rows == 0 || requests == 0) return UNIQL_OK;
     if (!table || !cu || !k || !v) return UNIQL_E_NULL;
     if (const int code = cache_pointers(c)) return code;

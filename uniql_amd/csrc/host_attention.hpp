@@ -108,6 +108,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> kv_assign_pages(const Tensor& new_tok
         require_plain(*count_out, "count_out", at::kInt, 1, new_tokens);
         if (count_out->size(0) != 1) fail("count_out must have one entry");
     }
+    const auto is = [](const Tensor& x, const Tensor& y) { return x.numel() > 0 && x.data_ptr() == y.data_ptr(); };
+    if (is(new_tokens, lengths_out ? *lengths_out : lengths)) fail("lengths_out must not be new_tokens");
     if (max_tokens < 0 || max_tokens > (1 << 24)) fail("max_tokens must be between 0 and 2^24");
     if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256)
         fail("pages must hold 16, 32, 64, 128 or 256 tokens");
@@ -192,6 +194,7 @@ Tensor kv4_attention(const Tensor& q, const Tensor& k_codes, const Tensor& k_sca
     }
     const c10::DeviceGuard guard(q.device());
     Tensor out = heads_output(out_in, "out", rows, heads, v_dim, q);
+    if (rows > 0 && out.data_ptr() == q.data_ptr()) fail("out must not be q: workgroups that share a row read it at different times");
     size_t need_accum = 0, need_temp = 0;
     check(p_attention_workspace(&cache, (int)rows, (int)requests, (int)table.size(1), (int)heads, &need_accum, &need_temp),
           "uniql_kv4_attention_workspace");
@@ -234,6 +237,8 @@ Tensor prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
     }
     const c10::DeviceGuard guard(q.device());
     Tensor out = heads_output(out_in, "out", rows, heads, v.size(2), q);
+    if (rows > 0 && (out.data_ptr() == q.data_ptr() || out.data_ptr() == k.data_ptr() || out.data_ptr() == v.data_ptr()))
+        fail("out must not be q, k or v");
     check(p_prompt(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
                    cu_q.data_ptr<int>(), cu_k.data_ptr<int>(), out.data_ptr(), out.stride(0), out.stride(1), (int)rows, (int)k_rows,
                    (int)(cu_q.size(0) - 1), (int)heads, (int)kv_heads, (int)q.size(2), (int)v.size(2), causal, (float)scale,

@@ -69,23 +69,6 @@ struct Request {
     int first, count;
     int length;
 };
-__device__ __forceinline__ Request request_of(const KvAttentionArgs& a, int r) {
-    Request q;
-    if (a.cu_q) {
-        int b = a.cu_q[r], e = a.cu_q[r + 1];
-        b = b < 0 ? 0 : (b > a.rows ? a.rows : b);
-        e = e < b ? b : (e > a.rows ? a.rows : e);
-        q.first = b;
-        q.count = e - b;
-    } else {
-        q.first = r;
-        q.count = 1;
-    }
-    const int64_t room = (int64_t)a.columns << a.cache.page_shift;
-    const int n = a.lengths[r];
-    q.length = n < 0 ? 0 : (n > room ? (int)room : n);
-    return q;
-}
 // row / a.group for rows below 2^31 (see the launch)
 __device__ __forceinline__ int query_of(const KvAttentionArgs& a, int row) { return (int)(((uint64_t)(unsigned)row * a.group_factor) >> a.group_shift); }
 __device__ __forceinline__ int row_tiles(const KvAttentionArgs& a, const Request& q) { return (int)(((int64_t)q.count * a.group + kRows - 1) / kRows); }
@@ -104,6 +87,38 @@ __device__ __forceinline__ unsigned sums_upto(unsigned v, Add add) {
     return add(v, from_below<0x143, 0xc>(v));  // lane 31, for the upper half
 }
 __device__ __forceinline__ unsigned lane_value(unsigned v, int lane) { return (unsigned)__builtin_amdgcn_readlane((int)v, lane); }
+
+// The requests from `base` on, one a lane.  `end`: where the rows of those before end; offsets that fall count as ones that stay, so
+// that all requests together have no more rows than there are, and no more workgroups than are launched: were some of those that
+// share a request's rows missing, the others' count of arrivals would stay behind in `accum`.
+__device__ __forceinline__ Request requests_of(const KvAttentionArgs& a, int base, unsigned& end) {
+    const int lane = threadIdx.x & 63, r = base + lane;
+    Request q = {0, 0, 0};
+    if (a.cu_q) {
+        int first = 0, last = 0;
+        if (r < a.requests) {
+            first = a.cu_q[r];
+            last = a.cu_q[r + 1];
+        }
+        first = first < 0 ? 0 : (first > a.rows ? a.rows : first);
+        last = last < 0 ? 0 : (last > a.rows ? a.rows : last);
+        const auto larger = [](unsigned x, unsigned y) { return x > y ? x : y; };
+        const unsigned begin = larger(sums_upto((unsigned)first, larger), end);
+        const unsigned stop = larger(begin, (unsigned)last);
+        q.first = (int)begin;
+        q.count = r < a.requests ? (int)(stop - begin) : 0;
+        end = lane_value(stop, 63);
+    } else {
+        q.first = r;
+        q.count = r < a.requests ? 1 : 0;
+    }
+    if (r < a.requests) {
+        const int64_t room = (int64_t)a.columns << a.cache.page_shift;
+        const int n = a.lengths[r];
+        q.length = n < 0 ? 0 : (n > room ? (int)room : n);
+    }
+    return q;
+}
 
 // A workgroup's share of a request's row tile `rows`.  Either the position tiles from `run * chunk` on, `run` of them, for one key /
 // value head, a tile a wave in turn; `chunks` workgroups share these rows, and their partial results lie in the places `place - chunk`
@@ -133,15 +148,14 @@ __device__ __forceinline__ Parts parts_of(int positions, int run, float by_run) 
 // Every wave finds it for itself.  Position tiles times row tiles of all requests, over the workgroups there are, give the run's
 // length.  Whole runs come first, request after request, then the rests, then what is done alone: what takes longest starts first.
 __device__ __forceinline__ bool find_share(const KvAttentionArgs& a, Share& s) {
-    const int lane = threadIdx.x & 63, heads = a.cache.heads;
+    const int heads = a.cache.heads;
     const auto add_f = [](unsigned x, unsigned y) { return __builtin_bit_cast(unsigned, __builtin_bit_cast(float, x) + __builtin_bit_cast(float, y)); };
     const auto add_u = [](unsigned x, unsigned y) { return x + y; };
     Request q = {0, 0, 0};
     float total = 0.f;
+    unsigned rows_end = 0;
     for (int base = 0; base < a.requests; base += 64) {
-        const int r = base + lane;
-        q = Request{0, 0, 0};
-        if (r < a.requests) q = request_of(a, r);
+        q = requests_of(a, base, rows_end);
         const float mine = (float)row_tiles(a, q) * (float)position_tiles(q);
         total += __builtin_bit_cast(float, lane_value(sums_upto(__builtin_bit_cast(unsigned, mine), add_f), 63));
     }
@@ -159,16 +173,13 @@ __device__ __forceinline__ bool find_share(const KvAttentionArgs& a, Share& s) {
     bool alone = false;
     for (int round = 0; round < 2; ++round) {
         unsigned runs = 0, rests = 0, alones = 0;
+        rows_end = 0;
         for (int base = 0; base < a.requests; base += 64) {
-            if (a.requests > 64) {
-                const int r = base + lane;
-                q = Request{0, 0, 0};
-                if (r < a.requests) q = request_of(a, r);
-            }
+            if (a.requests > 64) q = requests_of(a, base, rows_end);
             const int tiles = row_tiles(a, q);
             const Parts p = parts_of(position_tiles(q), run, by_run);
             const int64_t want = (int64_t)tiles * p.runs;
-            const unsigned some = tiles < (1 << 24) ? (unsigned)tiles : 1u << 24;  // (more than any grid has: offsets that fall and rise again)
+            const unsigned some = tiles < (1 << 24) ? (unsigned)tiles : 1u << 24;  // (more than any grid has)
             const unsigned my_runs = want < (1 << 24) ? (unsigned)want : 1u << 24, my_rests = some * (unsigned)p.rest, my_alones = some * (unsigned)p.alone;
             const unsigned upto_runs = runs + sums_upto(my_runs, add_u), upto_rests = rests + sums_upto(my_rests, add_u);
             unsigned upto = upto_runs, looked_for = index;
@@ -567,7 +578,7 @@ int kv4_attention_launch(const KvAttentionArgs& args, hipStream_t stream) {
     a.group_shift = 31 + shift;
     a.group_factor = (unsigned)(((1ULL << a.group_shift) + a.group - 1) / a.group);
     const int64_t workgroups = workgroups_of(a.rows, a.requests, a.group, a.cache.heads, a.cu_q == nullptr) * a.cache.heads;
-    if (workgroups > 0x7fffffffLL) return UNIQL_E_SHAPE;
+    if (workgroups >= (1LL << 32) / (64 * kWaves)) return UNIQL_E_SHAPE;  // (threads of a grid)
     const dim3 grid((unsigned)workgroups), block(64 * kWaves);
     switch (a.cache.k_words / 4) {
         case 1: hipLaunchKernelGGL(kv4_attention_kernel<1>, grid, block, 0, stream, a); break;

@@ -84,6 +84,7 @@ __device__ __forceinline__ bool find_block(const PromptArgs& a, int index, int b
             return true;
         }
         before += __builtin_amdgcn_readlane(upto, 63);
+        if (before > 0x3fffffff) return false;  // (offsets that fall and rise again)
     }
     return false;
 }
@@ -472,7 +473,7 @@ int prompt_attention_launch(const PromptArgs& args, hipStream_t stream) {
     const int load = near && (strides & 7) == 0 && (bases & 15) == 0 ? kWhole
                      : near && (strides & 1) == 0 && (bases & 3) == 0 && a.k_row >= 8 && a.v_row >= 8 ? kTail : kThrough;
     const int64_t rows = (int64_t)a.rows * a.group, blocks = rows / kBlockRows + (a.sequences < a.rows ? a.sequences : a.rows);
-    if (rows > (1LL << 30) || blocks * (a.heads / a.group) > 0x7fffffffLL) return UNIQL_E_SHAPE;
+    if (rows > (1LL << 30) || blocks * (a.heads / a.group) >= (1LL << 32) / (64 * kWaves)) return UNIQL_E_SHAPE;
     a.blocks = (int)blocks;
     // floor(row / d) = row f >> (31 + s) with f = 2^(31 + s) / d rounded up and s so that d <= 2^s < 2 d: f d - 2^(31 + s) < 2^s, so the
     // excess stays below 1 / d for rows below 2^31
