@@ -1,14 +1,22 @@
 // Causal attention over the prompts of several sequences that lie behind each other: o = sum_j p_j v_j / sum_j p_j,
 // p_j = exp(scale q . k_j - m), row i of a sequence with t queries and n keys over the keys j <= i + n - t.
 //
-// A workgroup takes 32 rows of a head for each of its waves and goes through the keys 64 at a time, in LDS, the next 64 on their way
-// meanwhile (two buffers, straight from memory to LDS).  Matrix instructions of 32 x 32 x 16: the scores come transposed, keys along
+// A workgroup takes 32 rows for each of its four waves (a query's heads that share keys side by side) and goes through the keys 64 at a
+// time, in LDS, the next 64 on their way meanwhile (two buffers, straight from memory to LDS).  Matrix instructions of 32 x 32 x 16: the scores come transposed, keys along
 // the rows, K q^T, because a lane then holds scores of one query and of just those keys that the second product, V^T P^T, wants
 // from it: the weights never leave its registers.  That product takes V transposed, four keys of one channel at a time, which the
 // transposing LDS read gives.  Rows of K and V lie in LDS with their 16-byte pieces exchanged by the row's number, so that neither
 // kind of read meets itself in a bank.
 // The maximum follows the scores only when a weight would pass 2^8 (weights are fp16, sums and outputs fp32): mostly once.
 // The rounding of the weights to fp16 (2^-11) is what a matrix instruction on fp16 asks for; their sum takes the rounded ones.
+//
+// Bound by the matrix and vector instructions together, and by power: 32 + 8 heads of 128, 16384 tokens 2.08 to 2.18 ms, 1.01 to 1.06
+// PFLOP/s, where the library's product of 16384 x 16384 reaches 1.26 at the clock that the GPU holds; 8 prompts of 2048 0.83, 1 of 2048
+// 0.64, 24 of 1 to 1850 tokens 0.66.  A step of 64 keys is 32 matrix instructions of 32 clocks for a wave, and beside the next tile's
+// scores 32 exponentials, as many products, 16 conversions and 16 sums; two workgroups a compute unit fill each other's gaps.  Short
+// prompts are bound by latency (1 token 6.7 us, 333 12): offsets, queries and the first tile follow each other, then 1.2 us a step.
+// Tried and taken out: two sets of four waves that share the keys out (333 tokens 14.3 -> 13.9, 24 prompts 81 -> 107 us: a compute unit
+// then holds one workgroup), blocks of all sequences in order of their length (24 prompts 75 -> 74, 64 of 512 276 -> 299 us).
 #include "prompt_attention.hpp"
 
 namespace uniql {
