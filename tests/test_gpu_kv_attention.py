@@ -315,3 +315,26 @@ def test_a_scale_that_is_no_number_and_an_output_that_is_the_input(gpu):
             p.cache.attend(q, table, lengths, scale=scale)
     with pytest.raises(RuntimeError, match="must not be q"):
         p.cache.attend(q, table, lengths, out=q)
+
+
+@pytest.mark.parametrize("small,large", [(1e-4, 1e3), (1e-5, 6e4), (1.0, 6e4)])
+@pytest.mark.parametrize("seen_first", [False, True])
+def test_small_values_beside_large_ones_without_weight(gpu, small, large, seen_first):
+    """nearly all weight is on one position whose values are tiny; others' are huge, but have no weight.  The result is that
+    position's values to within the rounding of weights and results (half a step each) and of fp16 numbers below 2^-14 (2^-25)."""
+    n, at = 400, 30 if seen_first else 370
+    gen = torch.Generator().manual_seed(2)
+    direction = torch.randn(64, generator=gen)
+    k = torch.zeros(n, 1, 64).half()
+    k[at, 0] = direction.half()
+
+    def values(v):
+        v = v * 0 + large * torch.sign(v)
+        v[at] = (small * torch.randn(1, 64, generator=gen)).half()
+        return v.half()
+
+    p = Problem(gpu, [n], [1], 2, 1, 64, 64, 16, k_of=lambda _: k, v_of=values)
+    p.q = (direction * 3).half().expand(1, 2, 64).contiguous()
+    got = p.run(scale=1.0).cpu().double()[0, 0]      # one score of about 190, the others 0: weights of e^-190 and less
+    want = as_held(p.v[0])[0][at, 0]
+    assert ((got - want).abs() <= 2 ** -10 * want.abs() + 2 ** -25).all(), float((got - want).abs().max())

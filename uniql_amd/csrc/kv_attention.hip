@@ -9,13 +9,14 @@
 //   output   2^24 sum_j w_j ((c'_j - 8) 2^-24)               its results are the second one's operand in the lanes where they are
 // (The values' 8 is taken off in front of the product, one more instruction a pair: behind it, over 65536 positions, the difference of two sums
 // 80 times as large as itself was four times as far from the exact result.)
-// with w_j = fp16(p_j s'_j).  For w_j to use fp16's range whatever the values' sizes, m is the running maximum of the scores plus
-// the exponent of s'_j: w_j <= 1 at the maximum, and it moves only when some w_j would pass 2^8.
+// with w_j = fp16(p_j s'_j).  For w_j to use fp16's range whatever the values' sizes, m is the running maximum of each
+// position's score with the exponent of its s'_j: w_j < 2 at the maximum, and it moves only when some w_j would pass 2^8.  (Largest score
+// and largest exponent apart save 1 % of the time, but lose small values that have the weight beside large ones that have none.)
 // The rounding of w_j (2^-11) is what a matrix instruction on fp16 asks for; sums, maxima and the output stay in fp32.
 //
-// Bound by HBM: 132 bytes for a position of 128 + 128 channels (16 requests of 65536 tokens, 8 heads of 128: 196 us, 5.65 TB/s; a kernel
+// Bound by HBM: 132 bytes for a position of 128 + 128 channels (16 requests of 65536 tokens, 8 heads of 128: 198 us, 5.6 TB/s; a kernel
 // that sums up 2 GB reads 6.1).  Fewer bytes are bound by latency: share, page numbers, positions, sums, exchange follow each other (1 x 4096
-// 10.8 us, 48 requests of 1 to 8192 16.5: finding the share 1 us, the first positions 1.5, 1.5 for each further 64 a wave takes, the
+// 10.9 us, 48 requests of 1 to 8192 17.0: finding the share 1 us, the first positions 1.5, 1.5 for each further 64 a wave takes, the
 // waves' sums 0.4, exchange and adding up 2).  The lengths are on the device, so every workgroup finds its share from them
 // (kPositions x request tiles, shared out evenly): requests of any lengths fill the GPU alike.  Where several workgroups share a
 // request's rows they leave (m, sum p, o) in scratch memory and the last to arrive adds them up in their order.
@@ -365,21 +366,16 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
                 vs[u] &= keep;
             }
         }
-        // the largest score and the largest exponent of a value's scale (fp16 numbers order as their bits do)
-        float top = score[0];
-        uint32_t scale_bits = 0;
-#pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, score[i]);
+        // the largest score with its value's exponent, 14 too large: the scale's bits are its exponent, and 0 for zero and what is masked
+        float top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t b = (uint32_t)(vs[u] >> (16 * i)) & 0xffffu;
-                scale_bits = b > scale_bits ? b : scale_bits;
-            }
-        const float size = (float)(int)(scale_bits >> 10) - 14.f;
-        if (__any(top + size > m + kSlack)) {
-            const float next = fmaxf(m, quad_max(top + size));
+            for (int i = 0; i < 4; ++i)
+                top = fmaxf(top, score[4 * u + i] + (float)(unsigned)((uint32_t)(vs[u] >> (16 * i + 10)) & 31u));
+        top -= 14.f;
+        if (__any(top > m + kSlack)) {
+            const float next = fmaxf(m, quad_max(top));
             const float fade = __builtin_amdgcn_exp2f(m - next);
             m = next;
             l *= fade;
