@@ -371,7 +371,7 @@ int uniql_fwht_columns(const void* x, void* y, int rows, int cols, float scale, 
 
 /*
  * ---- attention: a paged key / value cache held in 4 bits, attention over it and over whole prompts -------------------
- * The reference keeps fp16 keys and values of transformers' cache classes and calls torch's or flash_attn's attention
+ * The reference keeps fp16 keys and values of transformers' cache classes and calls a library's attention
  * (modeling/llama/llama_qblocks.py:104-150); these calls are this library's own and stand between the rotary kernel and
  * the output projection.  fp16 throughout, head widths 1 to 128, query heads a multiple of the key / value heads (query
  * head h uses key / value head h / (n_q_heads / n_kv_heads)).

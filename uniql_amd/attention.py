@@ -1,5 +1,5 @@
 """Attention over whole prompts: what stands between the rotary embedding and the output projection while a prompt is
-taken in.  (The reference calls torch's or flash_attn's there, modeling/llama/llama_qblocks.py:104-150.)  For single tokens, over
+taken in.  (The reference calls a library's attention there, modeling/llama/llama_qblocks.py:104-150.)  For single tokens, over
 the 4-bit cache: quantize.quant_kv_cache."""
 from __future__ import annotations
 
