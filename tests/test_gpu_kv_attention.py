@@ -338,3 +338,40 @@ def test_small_values_beside_large_ones_without_weight(gpu, small, large, seen_f
     got = p.run(scale=1.0).cpu().double()[0, 0]      # one score of about 190, the others 0: weights of e^-190 and less
     want = as_held(p.v[0])[0][at, 0]
     assert ((got - want).abs() <= 2 ** -10 * want.abs() + 2 ** -25).all(), float((got - want).abs().max())
+
+
+def test_graphs_of_one_stream_replayed_beside_each_other(gpu):
+    """two graphs captured on a stream that has run eager calls, replayed on two other streams while that stream runs eager calls:
+    each counts arrivals in words of its own"""
+    from uniql_amd import ops
+    problems = [Problem(gpu, [4000, 900], [1, 1], 8, 2, 128, 128, 64, seed=5 + i) for i in range(3)]
+    inputs = [x.on_gpu()[:3] for x in problems]
+    home = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(home):
+        want = [x.cache.attend(*i) for x, i in zip(problems, inputs)]
+    torch.cuda.synchronize()
+    before = set(ops._accum_in_capture)
+    graphs, outs = [], []
+    for x, i in list(zip(problems, inputs))[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=home):
+            outs.append([x.cache.attend(*i) for _ in range(3)])
+        graphs.append(graph)
+    words = [ops._accum_in_capture[key].data_ptr() for key in set(ops._accum_in_capture) - before]
+    eager = ops._accum_cache[(home.device.index, home.cuda_stream)].data_ptr()
+    assert len({eager, *words}) == 3
+    others = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(10):
+        for out in outs:
+            for o in out:
+                o.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, others):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        with torch.cuda.stream(home):
+            got = [problems[2].cache.attend(*inputs[2]) for _ in range(3)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want[2]) for o in got)
+        assert all(torch.equal(o, want[i]) for i in range(2) for o in outs[i])

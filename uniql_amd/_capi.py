@@ -134,7 +134,8 @@ def host():
             spec.loader.exec_module(module)
             module.bind_attention(*(ctypes.cast(fn, ctypes.c_void_p).value
                                     for fn in (lib.uniql_kv_assign_pages, lib.uniql_kv4_store, lib.uniql_kv4_load,
-                                               lib.uniql_kv4_attention_workspace, lib.uniql_kv4_attention, lib.uniql_prompt_attention)))
+                                               lib.uniql_kv4_attention_workspace, lib.uniql_kv4_attention, lib.uniql_prompt_attention,
+                                               lib.uniql_stream_capture_id)))
             module.bind(*(ctypes.cast(fn, ctypes.c_void_p).value
                           for fn in (lib.uniql_w4a16_linear, lib.uniql_w4a16_linear_workspace, lib.uniql_w4_embedding_lookup,
                                      lib.uniql_fwht, lib.uniql_fwht_composite, lib.uniql_fwht_columns, lib.uniql_w4a16_quantize,

@@ -7,14 +7,17 @@ decltype(&uniql_kv4_load) p_load = nullptr;
 decltype(&uniql_kv4_attention_workspace) p_attention_workspace = nullptr;
 decltype(&uniql_kv4_attention) p_attention = nullptr;
 decltype(&uniql_prompt_attention) p_prompt = nullptr;
+decltype(&uniql_stream_capture_id) p_capture_id = nullptr;
 
-void bind_attention(uintptr_t assign, uintptr_t store, uintptr_t load, uintptr_t workspace, uintptr_t attention, uintptr_t prompt) {
+void bind_attention(uintptr_t assign, uintptr_t store, uintptr_t load, uintptr_t workspace, uintptr_t attention, uintptr_t prompt,
+                    uintptr_t capture_id) {
     p_assign = reinterpret_cast<decltype(p_assign)>(assign);
     p_store = reinterpret_cast<decltype(p_store)>(store);
     p_load = reinterpret_cast<decltype(p_load)>(load);
     p_attention_workspace = reinterpret_cast<decltype(p_attention_workspace)>(workspace);
     p_attention = reinterpret_cast<decltype(p_attention)>(attention);
     p_prompt = reinterpret_cast<decltype(p_prompt)>(prompt);
+    p_capture_id = reinterpret_cast<decltype(p_capture_id)>(capture_id);
 }
 
 void require_device(const Tensor& t, const char* name, const Tensor& like) {
@@ -200,8 +203,11 @@ Tensor kv4_attention(const Tensor& q, const Tensor& k_codes, const Tensor& k_sca
           "uniql_kv4_attention_workspace");
     Tensor accum, temp;
     if (need_accum) {
+        // a capture has counts of its own: its graph may be replayed on any stream, beside eager calls and other graphs
+        unsigned long long capture = 0;
+        check(p_capture_id(reinterpret_cast<void*>(stream), &capture), "uniql_stream_capture_id");
         const py::gil_scoped_acquire lock;
-        accum = accumulator(py::cast(q.device()), need_accum, stream).cast<Tensor>();
+        accum = accumulator(py::cast(q.device()), need_accum, stream, capture != 0).cast<Tensor>();
     }
     if (need_temp) temp = new_output({(int64_t)need_temp}, at::kByte, q);
     check(p_attention(q.data_ptr(), q.stride(0), q.stride(1), &cache, table.data_ptr<int>(), lengths.data_ptr<int>(),

@@ -64,7 +64,7 @@ _accum_retired: list = []
 # reserve, or, where there is none, a buffer whose zero fill is a node of that graph, so that it is
 # only known to be zero when that graph replays.  They serve nothing else and are kept until
 # reset_accumulators() (a capture on a stream that already ran an eager call uses that stream's
-# eager buffer instead).
+# eager buffer instead, but for calls that ask for `own` words).
 _accum_in_capture: dict = {}
 # Per device [words that are zero, how many of them captures have taken].  A graph that takes its
 # words from here records no zero fill: 1.8 to 4.6 us and a gap between kernels on each replay
@@ -88,12 +88,12 @@ def _capture_id(stream_ptr: int) -> int:
     return out.value
 
 
-def _accumulator(device: torch.device, nbytes: int, stream: int | None = None) -> torch.Tensor:
+def _accumulator(device: torch.device, nbytes: int, stream: int | None = None, own: bool = False) -> torch.Tensor:
     if stream is None:
         stream = _stream_ptr(device)
     key = (device.index, stream)
     buf = _accum_cache.get(key)
-    if buf is not None and buf.numel() * 8 >= nbytes:
+    if buf is not None and buf.numel() * 8 >= nbytes and not own:
         return buf
     words = max(nbytes // 8, 1 << 16)
     capture = _capture_id(stream)
