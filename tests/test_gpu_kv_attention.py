@@ -375,3 +375,21 @@ def test_graphs_of_one_stream_replayed_beside_each_other(gpu):
         torch.cuda.synchronize()
         assert all(torch.equal(o, want[2]) for o in got)
         assert all(torch.equal(o, want[i]) for i in range(2) for o in outs[i])
+
+
+def test_many_small_weights_beside_a_large_one(gpu):
+    """one position has the weight 1 and the value -1, 60000 have 2^-24.3 and 1: together 0.0029, each below what is left of an fp16
+    number scaled to 1.  Rounding: of the large weight 2^-11, of the small ones' sum (2^-24 of 2^-19.2) 6e-5, of the result 2^-12."""
+    n = 60001
+    k = torch.zeros(n, 1, 64).half()
+    k[100, 0] = 1.0
+    v = torch.ones(n, 1, 64).half()
+    v[100] = -1.0
+    p = Problem(gpu, [n], [1], 2, 1, 64, 64, 64, k_of=lambda _: k, v_of=lambda _: v)
+    p.q = torch.ones(1, 2, 64).half()
+    held_k, held_v = as_held(p.k[0])[0], as_held(p.v[0])[0]
+    scale = 24.3 * 0.6931471805599453 / float(held_k[100, 0].sum())
+    got = p.run(scale=scale).cpu().double()[0, 0]
+    weight = 2.0 ** -24.3
+    want = (held_v[100, 0] + (held_v[:, 0].sum(0) - held_v[100, 0]) * weight) / (1 + (n - 1) * weight)
+    assert ((got - want).abs() <= 2 ** -10).all(), float((got - want).abs().max())

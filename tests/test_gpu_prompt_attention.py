@@ -263,3 +263,19 @@ def test_a_scale_that_is_no_number_and_an_output_that_is_an_input(gpu):
         prompt_attention(x, x, x, cu, out=x)
     with pytest.raises(RuntimeError, match="must not be"):
         prompt_attention(x.clone(), x, x.clone(), cu, out=x)
+
+
+def test_many_small_weights_beside_a_large_one(gpu):
+    """one key has the weight 1 and the value -1, 60000 have 2^-25.1 and 1: together 0.0017, each below what is left of an fp16 number
+    scaled to 1.  Rounding: of the large weight 2^-11, of the small ones' sum (2^-25 of 2^-19.1) 3e-5, of the result 2^-12."""
+    from uniql_amd.attention import prompt_attention
+    n = 60001
+    k = torch.zeros(n, 1, 64).half()
+    k[100] = 1.0
+    v = torch.ones(n, 1, 64).half()
+    v[100] = -1.0
+    cu = [torch.tensor([0, x], dtype=torch.int32, device=gpu) for x in (1, n)]
+    got = prompt_attention(torch.ones(1, 2, 64, device=gpu).half(), k.to(gpu), v.to(gpu), cu[0], cu[1], scale=25.1 * 0.6931471805599453 / 64)
+    weight = 2.0 ** -25.1
+    want = (-1 + (n - 1) * weight) / (1 + (n - 1) * weight)
+    assert (got.cpu().double() - want).abs().max() <= 2 ** -10, float((got.cpu().double() - want).abs().max())

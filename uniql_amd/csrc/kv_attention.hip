@@ -10,7 +10,7 @@
 // (The values' 8 is taken off in front of the product, one more instruction a pair: behind it, over 65536 positions, the difference of two sums
 // 80 times as large as itself was four times as far from the exact result.)
 // with w_j = fp16(p_j s'_j).  For w_j to use fp16's range whatever the values' sizes, m is the running maximum of each
-// position's score with the exponent of its s'_j: w_j < 2 at the maximum, and it moves only when some w_j would pass 2^8.  (Largest score
+// position's score with the exponent of its s'_j, less 6: w_j < 2^7 at the maximum, and it moves only when some w_j might pass 2^15.  (Largest score
 // and largest exponent apart save 1 % of the time, but lose small values that have the weight beside large ones that have none.)
 // The rounding of w_j (2^-11) is what a matrix instruction on fp16 asks for; sums, maxima and the output stay in fp32.
 //
@@ -34,7 +34,8 @@ constexpr int kSlotFloats = 16 * 130;  // a workgroup's partial result: 16 rows 
 constexpr int kDeviceScope = 16;       // cache policy bit sc1: as relaxed device-scope loads and stores compile to
 constexpr int kOutStride = 132;
 constexpr float kNoMaximum = -3.0e38f;
-constexpr float kSlack = 8.0f;         // weights may grow to 2^8 before the maximum follows
+constexpr float kLift = 6.0f;          // weights at the maximum reach 2^6 to 2^7: ones 2^-24 as large are many in a long cache and keep five bits
+constexpr float kSlack = kLift + 8.0f; // they may grow by 2^8 before the maximum follows
 // Workgroups that a call is shared out to, two a compute unit, as many as its registers allow to run at once: what does not fit waits for a
 // whole one to end (us with 512 / 768 / 1024: 9 x 5 pruned 15.3 / 20.4 / 20.5, 16 x 65536 199 / 200 / 204, 1 x 4096 10.3 for all).
 constexpr int kWorkgroups = 512;
@@ -375,7 +376,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
                 top = fmaxf(top, score[4 * u + i] + (float)(unsigned)((uint32_t)(vs[u] >> (16 * i + 10)) & 31u));
         top -= 14.f;
         if (__any(top > m + kSlack)) {
-            const float next = fmaxf(m, quad_max(top));
+            const float next = fmaxf(m, quad_max(top) - kLift);
             const float fade = __builtin_amdgcn_exp2f(m - next);
             m = next;
             l *= fade;
