@@ -9,6 +9,9 @@
 // kind of read meets itself in a bank.
 // The maximum follows the scores only when a weight would pass 2^14 (weights are fp16, sums and outputs fp32): mostly once.  Weights are
 // 2^6 times as large as they need be, so that many small ones beside a large one are not lost (16384 tokens 2.095 -> 2.108 ms).
+// Scores beyond 2^22 (in powers of two), whose rounding alone is more than that room, are taken relative to the largest in a second pass,
+// as infinities and NaN behind the causal border have a pass of their own (16384 tokens 2.138 -> 2.154 ms; as a branch of every step instead
+// 2.121 -> 2.156).
 // The rounding of the weights to fp16 (2^-11) is what a matrix instruction on fp16 asks for; their sum takes the rounded ones.
 //
 // Bound by the matrix and vector instructions together, and by power: 32 + 8 heads of 128, 16384 tokens 2.08 to 2.18 ms, 1.01 to 1.06
@@ -30,6 +33,7 @@ constexpr int kBlockRows = kWaves * kQueries;
 constexpr float kLowest = -3.0e38f;
 constexpr float kLift = 6.0f;           // the largest weight is 2^6: ones 2^-24 as large are many among long rows of keys and keep five bits
 constexpr float kRoom = 8.0f;           // weights may grow to 2^14 before the maximum follows
+constexpr float kFar = 4194304.0f;      // 2^22: below it a product of a score and the scale is rounded by a quarter at most
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
@@ -138,7 +142,8 @@ __global__ __launch_bounds__(64 * kWaves, LOAD == kThrough ? 1 : 2) void prompt_
     const int row0 = block * kBlockRows + wave * kQueries, row = row0 + col;
     const int seen = seen_by(row);  // keys of the lane's row
     // of the wave's first row and of its last, and of the workgroup's
-    const int last_row = rows - 1, fewest = seen_by(row0);
+    const int last_row = rows - 1;
+    int fewest = seen_by(row0);
     const int most = row0 < rows ? seen_by(row0 + kQueries - 1 < last_row ? row0 + kQueries - 1 : last_row) : 0;
     const int block_end = (block + 1) * kBlockRows - 1, block_most = seen_by(block_end < last_row ? block_end : last_row);
     const int block_fewest = seen_by(block * kBlockRows);
@@ -239,7 +244,8 @@ __global__ __launch_bounds__(64 * kWaves, LOAD == kThrough ? 1 : 2) void prompt_
         }
     }
     f16 out[D];
-    float m, l;
+    float m = kLowest, l, shift = 0.f;  // shift: taken off the row's scores in a careful pass
+    bool searching = false;             // the pass looks for the row's maximum
     // where the lane reads: K rows col and 32 + col, piece 2 step + half; V rows 4 half + j (+ 8), j = (lane / 4) % 4, four channels
     const int k_read = col * kRowBytes, k_swap = col & (kPieces - 1);
     const int v_j = (lane >> 2) & 3, v_read = (4 * half + v_j) * kRowBytes + (lane & 1) * 8;
@@ -285,6 +291,14 @@ __global__ __launch_bounds__(64 * kWaves, LOAD == kThrough ? 1 : 2) void prompt_
         const bool active = key0 < most;  // the wave's rows see some of the keys (all waves take part in the barriers)
         if (active) {
             if (masked) {
+                if (careful) {
+                    float by = shift;
+                    asm volatile("" : "+v"(by));  // (not the scores and then the scale in one go: the difference is rounded first)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) score[k][i] -= by;
+                }
                 int seen_here = seen - key0 - 4 * half;
                 asm volatile("" : "+v"(seen_here));  // keeps the comparisons out of the other tiles' way
 #pragma unroll
@@ -392,7 +406,7 @@ __global__ __launch_bounds__(64 * kWaves, LOAD == kThrough ? 1 : 2) void prompt_
         careful = pass > 0;
 #pragma unroll
         for (int i = 0; i < D; ++i) out[i] = f16{};
-        m = kLowest, l = 0.f;
+        l = 0.f;
         if (tiles > 0) {
             f16 even[2], odd[2];
             UNIQL_WAIT_ALL_LOADS();
@@ -412,20 +426,33 @@ __global__ __launch_bounds__(64 * kWaves, LOAD == kThrough ? 1 : 2) void prompt_
                 if (t + 1 < tiles) step(t + 1, k_odd, v_odd, k_even, v_even, odd, even);
             }
         }
-        if (pass > 0 || !a.causal) break;
-        // Infinities and NaN are rare: where a result shows one, all is done again with care.
-        float zero = 0.f;
+        // Two things ask for all to be done again, with care.  Infinities and NaN, which are rare and show in a result.  And maxima so
+        // large that the products of the scores and the scale, exact in the exponentials, differ from the rounded maximum by more
+        // than the room that weights have: such a row's scores are taken relative to their largest, of which a pass leaves 2^-23,
+        // until the maximum is a near one; a last pass starts from it, as it does for the other rows.
+        const bool row_far = m != kLowest && fabsf(m) >= kFar;
+        bool bad = row_far || searching;
+        searching = row_far;
+        if (row_far) {
+            shift += m / unit;
+            m = kLowest;
+        }
+        if (pass == 0) {
+            float zero = 0.f;
 #pragma unroll
-        for (int i = 0; i < D; ++i)
+            for (int i = 0; i < D; ++i)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) zero = __builtin_fmaf(out[i][j], 0.f, zero);
-        const bool bad = __any(row < rows && zero != 0.f);
+                for (int j = 0; j < 16; ++j) zero = __builtin_fmaf(out[i][j], 0.f, zero);
+            bad |= row < rows && zero != 0.f;
+        }
+        bad = __any(bad);
         if (lane == 0) spoilt[wave] = bad;
         __syncthreads();
         int any = 0;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) any |= spoilt[w];
-        if (__builtin_amdgcn_readfirstlane(any) == 0) break;
+        if (__builtin_amdgcn_readfirstlane(any) == 0 || pass == 3) break;
+        fewest = 0;  // a careful pass treats every tile as one that not all rows see
         k_tile = k_base, v_tile = v_base;
         fetch_first();
     }
