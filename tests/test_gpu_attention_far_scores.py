@@ -3,7 +3,7 @@ give finite results, and where one key's score is beyond all others by more than
 import pytest
 import torch
 
-from tests.attention_reference import attention, bound
+from tests.attention_reference import as_held, attention, bound
 
 pytestmark = pytest.mark.gpu
 SIZES = [2.0 ** e for e in (18, 21, 22, 23, 24, 25, 26, 27, 28, 29, 31, 36)]
@@ -37,6 +37,30 @@ def test_prompts(gpu, score, turned):
         got = prompt_attention(q.to(gpu), k.to(gpu), v.to(gpu), cu, scale=1.1 * score / 2 ** 17).cpu()
         want = v[strongest(size, turned)].expand(n, 2, 48)
         assert torch.equal(got, want), (order, int((got != want).any(-1).any(-1).sum()))
+
+
+@pytest.mark.parametrize("score", SIZES)
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("n,requests", [(50, 2), (700, 1), (700, 600)])
+def test_over_the_cache(gpu, score, turned, n, requests):
+    """As above, with values from 1e-3 to 1e3.  Rounding: of the one weight times its scale and of the result, half a step each."""
+    from uniql_amd.quantize.quant_kv_cache import W4KVCache
+    gen = torch.Generator().manual_seed(2)
+    pages = -(-n // 16)
+    table = torch.randperm(pages, generator=gen).to(torch.int32).expand(requests, pages).contiguous()
+    slots = table[0].long()[torch.arange(n) // 16] * 16 + torch.arange(n) % 16
+    lengths = torch.full((requests,), n, dtype=torch.int32, device=gpu)
+    for order in ("rising", "falling", "mixed"):
+        size = ordered(1000.0 + 8 * torch.arange(n), order)
+        k = size.view(n, 1, 1).expand(n, 1, 64).half().contiguous()
+        v = (torch.randn(n, 1, 40, generator=gen) * 10 ** (6 * torch.rand(n, 1, 1, generator=gen) - 3)).half()
+        cache = W4KVCache(pages, 16, 1, 64, 40, device=gpu)
+        cache.store(k.to(gpu), v.to(gpu), slots.to(gpu))
+        q = torch.full((requests, 2, 64), -1.0 if turned else 1.0, device=gpu).half()
+        got = cache.attend(q, table.to(gpu), lengths, scale=1.1 * score / 2 ** 17).cpu().double()
+        held_k, held_v = as_held(k)[0], as_held(v)[0]
+        want = held_v[int((held_k[:, 0, 0].argmin if turned else held_k[:, 0, 0].argmax)()), 0]
+        assert ((got - want).abs() <= 2 ** -10 * want.abs() + 2 ** -25).all(), (order, float((got - want).abs().max()))
 
 
 NEAR = [0, 3, 70, 130, 199]

@@ -12,6 +12,7 @@
 // with w_j = fp16(p_j s'_j).  For w_j to use fp16's range whatever the values' sizes, m is the running maximum of each
 // position's score with the exponent of its s'_j, less 6: w_j < 2^7 at the maximum, and it moves only when some w_j might pass 2^15.  (Largest score
 // and largest exponent apart save 1 % of the time, but lose small values that have the weight beside large ones that have none.)
+// Beyond 2^22 (in powers of two), where such sums are rounded by as much as the room that weights have, m is the largest score alone.
 // The rounding of w_j (2^-11) is what a matrix instruction on fp16 asks for; sums, maxima and the output stay in fp32.
 //
 // Bound by HBM: 132 bytes for a position of 128 + 128 channels (16 requests of 65536 tokens, 8 heads of 128: 198 us, 5.6 TB/s; a kernel
@@ -36,6 +37,7 @@ constexpr int kOutStride = 132;
 constexpr float kNoMaximum = -3.0e38f;
 constexpr float kLift = 6.0f;          // weights at the maximum reach 2^6 to 2^7: ones 2^-24 as large are many in a long cache and keep five bits
 constexpr float kSlack = kLift + 8.0f; // they may grow by 2^8 before the maximum follows
+constexpr float kFar = 4194304.0f;     // 2^22: below it a score's sum with an exponent is off by a quarter at most
 // Workgroups that a call is shared out to, two a compute unit, as many as its registers allow to run at once: what does not fit waits for a
 // whole one to end (us with 512 / 768 / 1024: 9 x 5 pruned 15.3 / 20.4 / 20.5, 16 x 65536 199 / 200 / 204, 1 x 4096 10.3 for all).
 constexpr int kWorkgroups = 512;
@@ -375,8 +377,20 @@ __global__ __launch_bounds__(256, 2) void kv4_attention_kernel(const KvAttention
             for (int i = 0; i < 4; ++i)
                 top = fmaxf(top, score[4 * u + i] + (float)(unsigned)((uint32_t)(vs[u] >> (16 * i + 10)) & 31u));
         top -= 14.f;
-        if (__any(top > m + kSlack)) {
-            const float next = fmaxf(m, quad_max(top) - kLift);
+        if (__any(top - m > kSlack)) {
+            const float row_top = quad_max(top);
+            const bool far = fabsf(row_top) > kFar;
+            float wanted = row_top - kLift;
+            if (__any(far)) {
+                // Sums of scores that large and exponents are rounded by more than the room: the scores alone, which are exact
+                // beside each other; weights then reach the scales themselves, 2^14 at most.
+                float highest = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) highest = fmaxf(highest, score[i]);
+                highest = quad_max(highest);
+                wanted = far ? highest : wanted;
+            }
+            const float next = fmaxf(m, wanted);
             const float fade = __builtin_amdgcn_exp2f(m - next);
             m = next;
             l *= fade;
