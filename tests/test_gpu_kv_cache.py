@@ -291,3 +291,48 @@ def test_a_request_without_need_behind_one_that_is_refused(gpu):
         [40, 1, 20, 3], [0, 5, 0, 10], [[-1] * 4, [7, -1, -1, -1], [-1] * 4, [8, -1, -1, -1]], [4, 6], 16, 64)
     assert refused == [1, 0, 1, 0] and count == 2
     assert [got[2], got[4], got[5], got[0], got[6]] == [refused, after, [count], slots, tab]
+
+
+def test_a_cache_whose_tensors_are_replaced_past_its_attributes(gpu):
+    """register_buffer, a write to the module's dict of buffers, a functional call: store, load and attend take the tensors that are there"""
+    gen = torch.Generator().manual_seed(3)
+    a, b = torch.randn(20, 2, 40, generator=gen).half(), torch.randn(20, 2, 40, generator=gen).half()
+    slots, table = torch.arange(20, device=gpu), torch.arange(2, dtype=torch.int32, device=gpu)[None]
+    cu, lengths = torch.tensor([0, 20], dtype=torch.int32, device=gpu), torch.tensor([20], dtype=torch.int32, device=gpu)
+    q = torch.randn(1, 4, 40, generator=gen).half().to(gpu)
+    names = ("k_codes", "k_scales", "v_codes", "v_scales")
+    other = new_cache(gpu, 2, 16, 2, 40, 40)
+    other.store(b.to(gpu), b.to(gpu), slots)
+    want = other.attend(q, table, lengths)
+
+    def fresh():
+        cache = new_cache(gpu, 2, 16, 2, 40, 40)
+        cache.store(a.to(gpu), a.to(gpu), slots)
+        return cache
+
+    def is_other(cache):
+        return torch.equal(cache.load(table, cu, 20)[0].cpu(), as_held(b)[0].half()) and torch.equal(cache.attend(q, table, lengths), want)
+
+    cache = fresh()
+    for name in names:
+        cache.register_buffer(name, getattr(other, name).clone(), persistent=False)
+    assert is_other(cache)
+    cache = fresh()
+    mine = [t.clone() for t in cache.buffers()]
+    for name in names:
+        cache._buffers[name] = torch.zeros_like(getattr(other, name))
+    cache.store(b.to(gpu), b.to(gpu), slots)
+    assert is_other(cache)
+
+    class Call(torch.nn.Module):
+        def __init__(self, cache):
+            super().__init__()
+            self.cache = cache
+
+        def forward(self):
+            return is_other(self.cache)
+
+    cache = fresh()
+    assert not Call(cache)()
+    assert torch.func.functional_call(Call(cache), {"cache." + name: getattr(other, name) for name in names}, ())
+    assert not Call(cache)() and all(torch.equal(x, y) for x, y in zip(mine, cache.buffers()))
