@@ -432,7 +432,7 @@ int uniql_kv4_store(const void* k, int64_t k_row, int64_t k_head, const void* v,
  * cu[r] <= t < cu[r + 1].  Rows in front of cu[0] and from cu[requests] on are left as they were; positions without a page in the
  * pool give NaN.
  *   table    device, int32 [requests, columns];  cu  device, int32 [requests + 1];  starts  device, int32 [requests], or NULL: 0
- *   k, v     device out, fp16 [rows, heads, k_dim] and [rows, heads, v_dim], strides as above
+ *   k, v     device out, fp16 [rows, heads, k_dim] and [rows, heads, v_dim], strides as above; must not overlap
  */
 int uniql_kv4_load(const uniql_kv4_cache* cache, const int32_t* table, const int32_t* cu, const int32_t* starts,
                    void* k, int64_t k_row, int64_t k_head, void* v, int64_t v_row, int64_t v_head,

@@ -12,6 +12,7 @@
 // strided rows, allocations and launches may all wait for the device - but for that map and the accumulator's lookup.
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 #include <map>
 #include <optional>
@@ -347,6 +348,8 @@ PYBIND11_MODULE(_host, module) {
     module.def("kv4_load", &kv4_load);
     module.def("kv4_attention", &kv4_attention);
     module.def("prompt_attention", &prompt_attention);
+    module.def("share_memory", &share_memory);
+    module.def("overlaps_itself", &overlaps_itself);
     py::class_<KvPool>(module, "KvPool")
         .def(py::init([](Tensor k_codes, Tensor k_scales, Tensor v_codes, Tensor v_scales, int64_t k_dim, int64_t v_dim) {
             return KvPool{std::move(k_codes), std::move(k_scales), std::move(v_codes), std::move(v_scales), k_dim, v_dim};

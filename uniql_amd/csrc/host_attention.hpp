@@ -38,6 +38,57 @@ void require_heads(const Tensor& t, const char* name) {
     if (t.size(0) > 0x7fffffff || t.size(1) > 0x7fffffff || t.size(2) > 0x7fffffff) fail(std::string(name) + " is larger than a call can take");
     if (t.size(1) == 0 || t.size(2) == 0) fail(std::string(name) + " has no heads or no width");
 }
+// Where the elements of [rows, heads, width] with unit inner stride lie, in elements; heads and rows that follow each other count as
+// one wider head.
+struct Lattice {
+    int64_t first, rows, row, heads, head, width;
+    int64_t span() const { return (rows - 1) * row + (heads - 1) * head + width; }
+};
+Lattice lattice_of(const Tensor& t) {
+    Lattice l = {(int64_t)(reinterpret_cast<uintptr_t>(t.data_ptr()) / t.element_size()), t.size(0), t.stride(0), t.size(1), t.stride(1), t.size(2)};
+    if (l.heads == 1 || l.head == l.width) l.width *= l.heads, l.heads = 1, l.head = 0;
+    if (l.heads == 1 && (l.rows == 1 || l.row == l.width)) l.width *= l.rows, l.rows = 1, l.row = 0;
+    return l;
+}
+int64_t quotient_down(int64_t a, int64_t b) { return a / b - (a % b < 0); }  // b > 0
+// Whether t step lies strictly between `low` and `high` for a whole t from `least` to `most`.
+bool hits(int64_t step, int64_t least, int64_t most, int64_t low, int64_t high) {
+    if (step == 0) return low < 0 && 0 < high;
+    const int64_t t = std::max(least, quotient_down(low, step) + 1);
+    return t <= most && t * step < high && t * step > low;
+}
+// Whether two tensors of heads have an element in common.  Mostly they lie apart; otherwise each pair of heads is looked at, for all
+// rows at once where both have the same distance between rows.
+bool share_memory(const Tensor& x, const Tensor& y) {
+    if (x.numel() == 0 || y.numel() == 0) return false;
+    Lattice a = lattice_of(x), b = lattice_of(y);
+    if (a.first + a.span() <= b.first || b.first + b.span() <= a.first) return false;
+    if (a.rows == 1) a.row = b.row;
+    if (b.rows == 1) b.row = a.row;
+    if (a.row != b.row && a.rows > b.rows) std::swap(a, b);
+    for (int64_t i = 0; i < a.heads; ++i)
+        for (int64_t j = 0; j < b.heads; ++j) {
+            const int64_t apart = a.first + i * a.head - b.first - j * b.head;
+            if (a.row == b.row) {
+                if (hits(a.row, 1 - b.rows, a.rows - 1, -a.width - apart, b.width - apart)) return true;
+                continue;
+            }
+            for (int64_t r = 0; r < a.rows; ++r) {
+                const int64_t at = apart + r * a.row;   // less a row of b
+                if (hits(b.row, 0, b.rows - 1, at - b.width, at + a.width)) return true;
+            }
+        }
+    return false;
+}
+bool overlaps_itself(const Tensor& t) {
+    if (t.numel() == 0) return false;
+    const Lattice l = lattice_of(t);
+    if (l.head >= l.width && l.row >= (l.heads - 1) * l.head + l.width) return false;
+    if (l.rows > 1 && l.row < l.width) return true;
+    for (int64_t i = 1; i < l.heads; ++i)
+        if (hits(l.row, 1 - l.rows, l.rows - 1, -l.width - i * l.head, l.width - i * l.head)) return true;
+    return false;
+}
 // The tensor that a call writes: the caller's, of exactly this shape, or a new one.
 Tensor heads_output(const std::optional<Tensor>& out, const char* name, int64_t rows, int64_t heads, int64_t width, const Tensor& like) {
     if (!out) return new_output({rows, heads, width}, at::kHalf, like);
@@ -45,7 +96,7 @@ Tensor heads_output(const std::optional<Tensor>& out, const char* name, int64_t 
     require_heads(*out, name);
     if (out->size(0) != rows || out->size(1) != heads || out->size(2) != width)
         fail(std::string(name) + " must be [" + std::to_string(rows) + ", " + std::to_string(heads) + ", " + std::to_string(width) + "]");
-    if ((rows > 1 && out->stride(0) < width) || (heads > 1 && out->stride(1) < width)) fail(std::string(name) + " overlaps itself");
+    if (overlaps_itself(*out)) fail(std::string(name) + " overlaps itself");
     return *out;
 }
 // Row r of a table of requests, entry p: the page of positions p page_size ..
@@ -168,6 +219,7 @@ std::pair<Tensor, Tensor> kv4_load(const Tensor& k_codes, const Tensor& k_scales
     if (rows < 0 || rows > 0x7fffffff) fail("rows must be between 0 and 2^31 - 1");
     const c10::DeviceGuard guard(k_codes.device());
     Tensor k = heads_output(k_out, "k_out", rows, cache.heads, k_dim, k_codes), v = heads_output(v_out, "v_out", rows, cache.heads, v_dim, k_codes);
+    if (k_out && v_out && share_memory(k, v)) fail("k_out and v_out must not share memory");
     check(p_load(&cache, table.data_ptr<int>(), cu.data_ptr<int>(), starts ? starts->data_ptr<int>() : nullptr, k.data_ptr(), k.stride(0),
                  k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), (int)requests, (int)table.size(1), (int)rows,
                  reinterpret_cast<void*>(stream)),
@@ -197,7 +249,7 @@ Tensor kv4_attention(const Tensor& q, const Tensor& k_codes, const Tensor& k_sca
     }
     const c10::DeviceGuard guard(q.device());
     Tensor out = heads_output(out_in, "out", rows, heads, v_dim, q);
-    if (rows > 0 && out.data_ptr() == q.data_ptr()) fail("out must not be q: workgroups that share a row read it at different times");
+    if (out_in && share_memory(out, q)) fail("out must not be q or share memory with it: workgroups that share a row read it at different times");
     size_t need_accum = 0, need_temp = 0;
     check(p_attention_workspace(&cache, (int)rows, (int)requests, (int)table.size(1), (int)heads, &need_accum, &need_temp),
           "uniql_kv4_attention_workspace");
@@ -243,8 +295,8 @@ Tensor prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
     }
     const c10::DeviceGuard guard(q.device());
     Tensor out = heads_output(out_in, "out", rows, heads, v.size(2), q);
-    if (rows > 0 && (out.data_ptr() == q.data_ptr() || out.data_ptr() == k.data_ptr() || out.data_ptr() == v.data_ptr()))
-        fail("out must not be q, k or v");
+    if (out_in && (share_memory(out, q) || share_memory(out, k) || share_memory(out, v)))
+        fail("out must not be q, k or v or share memory with them");
     check(p_prompt(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
                    cu_q.data_ptr<int>(), cu_k.data_ptr<int>(), out.data_ptr(), out.stride(0), out.stride(1), (int)rows, (int)k_rows,
                    (int)(cu_q.size(0) - 1), (int)heads, (int)kv_heads, (int)q.size(2), (int)v.size(2), causal, (float)scale,
