@@ -336,3 +336,16 @@ def test_a_cache_whose_tensors_are_replaced_past_its_attributes(gpu):
     assert not Call(cache)()
     assert torch.func.functional_call(Call(cache), {"cache." + name: getattr(other, name) for name in names}, ())
     assert not Call(cache)() and all(torch.equal(x, y) for x, y in zip(mine, cache.buffers()))
+
+
+def test_a_full_list_of_as_many_pages_as_numbers_go(gpu):
+    """2^31 - 1 free pages, as many as the list has room for, and a request that gives back another hundred: nothing is written"""
+    from uniql_amd import ops
+    pool = 2 ** 31 - 1
+    t = lambda v: torch.tensor(v, dtype=torch.int32, device=gpu)
+    free = torch.full((pool,), -7, dtype=torch.int32, device=gpu)
+    for count, kept in ((pool, 0), (pool - 60, 60)):
+        n = t([count])
+        ops.kv_assign_pages(t([-1]), t([1600]), torch.arange(100, dtype=torch.int32, device=gpu)[None], free, n, 16, 4)
+        assert n.tolist() == [pool] and free[count:].tolist() == list(range(kept))
+        assert int(free[:count].amax()) == -7 and int(free[:count].amin()) == -7

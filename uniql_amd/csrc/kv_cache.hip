@@ -103,7 +103,7 @@ __global__ __launch_bounds__(kAssignThreads) void kv_assign_kernel(const AssignA
             __syncthreads();
             for (int i = tid; i < total; i += kAssignThreads) {
                 const int row = first_above(upto, kAssignThreads, i), j = i - (upto[row] - held_by[row]);
-                if (count + i < a.pool) a.free_pages[count + i] = a.table[(int64_t)(base + row) * a.columns + j];
+                if (i < a.pool - count) a.free_pages[count + i] = a.table[(int64_t)(base + row) * a.columns + j];
             }
             count = total > a.pool - count ? a.pool : count + total;
         }
