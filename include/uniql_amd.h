@@ -400,6 +400,7 @@ typedef struct uniql_kv4_cache {
  *                p page_size ..; modified (entries behind a request's last page are not meaningful)
  *   free_pages   device, int32 [pool]: a stack of *free_count free pages; modified
  *   lengths_out, free_count_out   device: lengths and count after the step; may be `lengths` and `free_count` themselves
+ * (otherwise no two of the arrays may overlap)
  * First the pages of ending requests go on top of the stack, in the order of the rows and of their pages; their lengths
  * become 0.  Then the others take ceil((length + new) / page_size) - ceil(length / page_size) pages from the top, in the
  * order of the rows.  A request is refused, and changes nothing, when it would have more tokens than its row has room for, when

@@ -349,3 +349,26 @@ def test_a_full_list_of_as_many_pages_as_numbers_go(gpu):
         ops.kv_assign_pages(t([-1]), t([1600]), torch.arange(100, dtype=torch.int32, device=gpu)[None], free, n, 16, 4)
         assert n.tolist() == [pool] and free[count:].tolist() == list(range(kept))
         assert int(free[:count].amax()) == -7 and int(free[:count].amin()) == -7
+
+
+def test_assign_refuses_arrays_that_share_memory(gpu):
+    """what the call writes is no part of what it reads or writes otherwise; lengths and the count may be replaced in place"""
+    from uniql_amd import ops
+    words = torch.zeros(200, dtype=torch.int32, device=gpu)
+    new, lengths, count, table, free = words[:4], words[4:8], words[8:9], words[9:49].view(4, 10), words[49:69]
+    spare, one = words[69:73], words[73:74]
+
+    def call(**kw):
+        a = {**dict(new=new, lengths=lengths, table=table, free=free, count=count, lengths_out=spare, count_out=one), **kw}
+        return ops.kv_assign_pages(a["new"], a["lengths"], a["table"], a["free"], a["count"], 16, 8, lengths_out=a["lengths_out"],
+                                   count_out=a["count_out"])
+
+    call(), call(lengths_out=None, count_out=None), call(lengths_out=lengths, count_out=count), call(lengths=words[1:5])
+    for kw in (dict(lengths_out=new), dict(lengths_out=words[2:6]), dict(lengths_out=words[5:9]), dict(lengths_out=words[6:10]),
+               dict(lengths_out=words[40:44]), dict(lengths_out=words[66:70]), dict(count_out=words[3:4]), dict(count_out=words[5:6]),
+               dict(count_out=words[70:71]), dict(count_out=words[30:31]), dict(count_out=words[60:61]), dict(free=words[48:60]),
+               dict(free=words[5:20]), dict(table=words[2:42].view(4, 10)), dict(table=words[30:70].view(4, 10)), dict(new=words[45:49]),
+               dict(lengths=words[50:54]), dict(count=words[50:51]), dict(new=lengths, lengths_out=None), dict(count=words[5:6], lengths_out=None)):
+        with pytest.raises(RuntimeError, match="share memory"):
+            call(**kw)
+    assert int(words.count_nonzero()) == 0

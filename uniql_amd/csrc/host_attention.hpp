@@ -162,8 +162,28 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> kv_assign_pages(const Tensor& new_tok
         require_plain(*count_out, "count_out", at::kInt, 1, new_tokens);
         if (count_out->size(0) != 1) fail("count_out must have one entry");
     }
-    const auto is = [](const Tensor& x, const Tensor& y) { return x.numel() > 0 && x.data_ptr() == y.data_ptr(); };
-    if (is(new_tokens, lengths_out ? *lengths_out : lengths)) fail("lengths_out must not be new_tokens");
+    // what is written is read by other threads of the call at other times
+    const Tensor &new_lengths = lengths_out ? *lengths_out : lengths, &new_count = count_out ? *count_out : free_count;
+    const auto apart = [](const Tensor& x, const char* x_name, const Tensor& y, const char* y_name, bool may_be_one) {
+        const char *a = static_cast<const char*>(x.data_ptr()), *b = static_cast<const char*>(y.data_ptr());
+        if (x.numel() == 0 || y.numel() == 0 || a + x.nbytes() <= b || b + y.nbytes() <= a || (may_be_one && a == b)) return;
+        fail(std::string(x_name) + " must not be " + y_name + " or share memory with it");
+    };
+    apart(new_lengths, "lengths_out", new_tokens, "new_tokens", false);
+    apart(new_lengths, "lengths_out", lengths, "lengths", true);
+    apart(new_lengths, "lengths_out", free_count, "free_count", false);
+    apart(new_count, "count_out", new_tokens, "new_tokens", false);
+    apart(new_count, "count_out", lengths, "lengths", false);
+    apart(new_count, "count_out", new_lengths, "lengths_out", false);
+    apart(new_count, "count_out", free_count, "free_count", true);
+    for (const auto& [x, name] : {std::pair<const Tensor&, const char*>{table, "table"}, {free_pages, "free_pages"}}) {
+        apart(x, name, new_tokens, "new_tokens", false);
+        apart(x, name, lengths, "lengths", false);
+        apart(x, name, new_lengths, "lengths_out", false);
+        apart(x, name, free_count, "free_count", false);
+        apart(x, name, new_count, "count_out", false);
+    }
+    apart(table, "table", free_pages, "free_pages", false);
     if (max_tokens < 0 || max_tokens > (1 << 24)) fail("max_tokens must be between 0 and 2^24");
     if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256)
         fail("pages must hold 16, 32, 64, 128 or 256 tokens");
@@ -173,8 +193,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> kv_assign_pages(const Tensor& new_tok
     Tensor slots = part_of(buffer, 0, max_tokens, at::kLong), positions = part_of(buffer, 8 * max_tokens, max_tokens, at::kInt);
     Tensor cu = part_of(buffer, 12 * max_tokens, rows + 1, at::kInt), refused = part_of(buffer, 12 * max_tokens + 4 * (rows + 1), rows, at::kInt);
     check(p_assign(new_tokens.data_ptr<int>(), lengths.data_ptr<int>(), table.data_ptr<int>(), free_pages.data_ptr<int>(),
-                   free_count.data_ptr<int>(), (lengths_out ? *lengths_out : lengths).data_ptr<int>(),
-                   (count_out ? *count_out : free_count).data_ptr<int>(), slots.data_ptr<int64_t>(), positions.data_ptr<int>(),
+                   free_count.data_ptr<int>(), new_lengths.data_ptr<int>(), new_count.data_ptr<int>(), slots.data_ptr<int64_t>(), positions.data_ptr<int>(),
                    cu.data_ptr<int>(), refused.data_ptr<int>(), (int)rows, (int)columns, (int)free_pages.size(0), (int)page_size,
                    (int)max_tokens, reinterpret_cast<void*>(stream)),
           "uniql_kv_assign_pages");
