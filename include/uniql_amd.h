@@ -447,7 +447,7 @@ int uniql_kv4_load(const uniql_kv4_cache* cache, const int32_t* table, const int
  *   out      device out, fp16 [rows, n_q_heads, v_dim], strides likewise; must not overlap q
  * Row i of a request with t rows sees the positions 0 .. length - t + i.  A row that sees none is 0; rows in front of cu_q[0] and
  * from cu_q[requests] on are left as they were.  What lies in the pages behind a request's length does not matter; a page number
- * outside the pool within it makes the rows that see it NaN.  (Offsets that fall count as ones that stay.)
+ * outside the pool within it makes the rows that see it NaN.  (Offsets that fall count as ones that stay.)  |scale| <= 2^64.
  *   accum, temp   as for uniql_w4a16_gemm: accum all zero on entry and on exit, temp of any contents, neither shared by calls that may
  *                 run at the same time; sizes from uniql_kv4_attention_workspace (bounds that follow from the arguments alone)
  */
@@ -467,7 +467,7 @@ int uniql_kv4_attention(const void* q, int64_t q_row, int64_t q_head, const uniq
  *   out      device out, fp16 [rows, n_q_heads, v_dim], strides likewise; must not overlap q, k or v
  * With `causal`, row i of a sequence with t rows and n keys sees the keys 0 .. i + n - t, all of them otherwise.  A row that sees
  * none is 0; rows in front of cu_q[0] and from cu_q[sequences] on are left as they were.  Other sequences' keys and values do
- * not matter, whatever they hold.
+ * not matter, whatever they hold.  |scale| <= 2^64.
  */
 int uniql_prompt_attention(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                            const void* v, int64_t v_row, int64_t v_head, const int32_t* cu_q, const int32_t* cu_k,

@@ -98,3 +98,17 @@ def test_prompt_attention(lib):
     assert call(rows=-1) == -2 and call(k_rows=-1) == -2 and call(sequences=-1) == -2 and call(heads=3) == -2 and call(kv=0) == -2
     assert call(kd=0) == -2 and call(vd=0) == -2 and call(kd=129) == -5 and call(vd=160) == -5 and call(heads=8192) == -2
     assert call(rows=0, q=None) == 0 and call(sequences=0, q=None) == 0
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf"), 1.9e19, -1.9e19, 3e38])
+def test_scales_with_which_finite_inputs_have_no_finite_scores(lib, scale):
+    """2^64 = 1.845e19: times 128 products of fp16 numbers (2^39) and what the kernels fold in (2^25 and less) it stays below 2^128"""
+    p = ctypes.byref(cache())
+    args = [FAKE, 1, 1, p, FAKE, FAKE, FAKE, FAKE, 1, 1, FAKE, 1 << 40, FAKE, 1 << 40, 1, 1, 1, 4]
+    assert lib.uniql_kv4_attention(*args, scale, None) == -5
+    prompt = [FAKE, 1, 1, FAKE, 1, 1, FAKE, 1, 1, FAKE, FAKE, FAKE, 1, 1, 4, 4, 1, 4, 2, 64, 64, 1]
+    assert lib.uniql_prompt_attention(*prompt, scale, None) == -5
+    # no rows: what is left of the checks passes with the largest scales
+    args[14], prompt[14] = 0, 0
+    for most in (2.0 ** 64, -2.0 ** 64, 1.0):
+        assert lib.uniql_kv4_attention(*args, most, None) == 0 and lib.uniql_prompt_attention(*prompt, most, None) == 0

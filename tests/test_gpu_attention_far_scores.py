@@ -121,3 +121,26 @@ def test_near_rows_beside_far_ones(gpu):
                 assert got[i, h].isnan().all()
             elif i == 0 or s[0] - s[1] > 200:
                 assert torch.equal(got[i, h], v[at[0], h])
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 64, -2.0 ** 64])
+@pytest.mark.parametrize("largest", [3.0, 65504.0])
+def test_the_largest_scale(gpu, scale, largest):
+    """finite scores of up to 2^104, each further from the next than any weight reaches"""
+    from uniql_amd.attention import prompt_attention
+    from uniql_amd.quantize.quant_kv_cache import W4KVCache
+    gen = torch.Generator().manual_seed(3)
+    size = ordered(largest * (1 + torch.arange(100)) / 100, "mixed")
+    k = size.view(100, 1, 1).expand(100, 1, 128).half().contiguous()
+    v = torch.randn(100, 1, 40, generator=gen).half()
+    q = torch.full((1, 2, 128), largest).half().to(gpu)
+    at = int(k[:, 0, 0].argmax() if scale > 0 else k[:, 0, 0].argmin())
+    cu = [torch.tensor([0, n], dtype=torch.int32, device=gpu) for n in (1, 100)]
+    for causal in (True, False):
+        got = prompt_attention(q, k.to(gpu), v.to(gpu), *cu, causal=causal, scale=scale).cpu()
+        assert torch.equal(got, v[at].expand(1, 2, 40))
+    cache = W4KVCache(7, 16, 1, 128, 40, device=gpu)
+    cache.store(k.to(gpu), v.to(gpu), torch.arange(100, device=gpu))
+    got = cache.attend(q, torch.arange(7, dtype=torch.int32, device=gpu)[None], cu[1][1:], scale=scale).cpu().double()
+    want = as_held(v)[0][at, 0]
+    assert ((got - want).abs() <= 2 ** -10 * want.abs() + 2 ** -25).all()

@@ -20,7 +20,9 @@ using namespace uniql;
 
 static constexpr int kMaxHeads = 4096, kMaxWidth = 128;
 
-static bool finite(float v) { return v - v == 0.f; }
+// Scales up to 2^64: finite queries and keys (128 products of 2^32) then have finite scores, also with the factors that the
+// kernels fold into the scale.
+static bool scale_ok(float v) { return v >= -18446744073709551616.0f && v <= 18446744073709551616.0f; }
 static bool page_size_ok(int n) { return n == 16 || n == 32 || n == 64 || n == 128 || n == 256; }
 // columns of a table, and the tokens that a row of it has room for
 static bool columns_ok(int64_t rows, int64_t columns, int64_t page_size) {
@@ -114,7 +116,7 @@ int uniql_kv4_attention(const void* q, int64_t q_row, int64_t q_head, const uniq
                         float scale, void* stream) {
     KvAttentionArgs a;
     if (const int code = attention_sizes(cache, a.cache, rows, requests, columns, n_q_heads)) return code;
-    if (!finite(scale)) return UNIQL_E_UNSUPPORTED;
+    if (!scale_ok(scale)) return UNIQL_E_UNSUPPORTED;
     if (!cu_q && rows != requests) return UNIQL_E_SHAPE;
     if (rows == 0 || requests == 0) return UNIQL_OK;
     if (!q || !table || !lengths || !out) return UNIQL_E_NULL;
@@ -149,7 +151,7 @@ int uniql_prompt_attention(const void* q, int64_t q_row, int64_t q_head, const v
     if (rows < 0 || k_rows < 0 || sequences < 0 || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads > kMaxHeads ||
         n_q_heads % n_kv_heads != 0 || k_dim <= 0 || v_dim <= 0)
         return UNIQL_E_SHAPE;
-    if (k_dim > kMaxWidth || v_dim > kMaxWidth || !finite(scale)) return UNIQL_E_UNSUPPORTED;
+    if (k_dim > kMaxWidth || v_dim > kMaxWidth || !scale_ok(scale)) return UNIQL_E_UNSUPPORTED;
     if (rows == 0 || sequences == 0) return UNIQL_OK;
     if (!q || !cu_q || !cu_k || !out || (k_rows > 0 && (!k || !v))) return UNIQL_E_NULL;
     PromptArgs a;
