@@ -411,8 +411,9 @@ typedef struct uniql_kv4_cache {
  *   slots        device out, int64 [max_tokens]: each token's place; -1 for tokens of refused requests and behind the last
  *   positions    device out, int32 [max_tokens]: each token's position in its request; 0 where slots is -1
  *   refused      device out, int32 [rows]: 1 where a request with new tokens was refused
- * columns <= 2^20, columns * page_size <= 2^30, rows * columns < 2^31, max_tokens <= 2^24.  Nothing outside these arrays is touched
- * whatever they hold; lengths below 0 count as 0 where a request ends and are refused otherwise.
+ * Of this and every other table: rows <= 2^30, columns <= 2^20, columns * page_size <= 2^30, rows * columns < 2^31.
+ * max_tokens <= 2^24.  Nothing outside these arrays is touched whatever they hold; lengths below 0 count as 0 where a request
+ * ends and are refused otherwise.
  */
 int uniql_kv_assign_pages(const int32_t* new_tokens, const int32_t* lengths, int32_t* table, int32_t* free_pages,
                           const int32_t* free_count, int32_t* lengths_out, int32_t* free_count_out,
@@ -467,7 +468,7 @@ int uniql_kv4_attention(const void* q, int64_t q_row, int64_t q_head, const uniq
  *   out      device out, fp16 [rows, n_q_heads, v_dim], strides likewise; must not overlap q, k or v
  * With `causal`, row i of a sequence with t rows and n keys sees the keys 0 .. i + n - t, all of them otherwise.  A row that sees
  * none is 0; rows in front of cu_q[0] and from cu_q[sequences] on are left as they were.  Other sequences' keys and values do
- * not matter, whatever they hold.  |scale| <= 2^64.
+ * not matter, whatever they hold.  |scale| <= 2^64, sequences <= 2^30.
  */
 int uniql_prompt_attention(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                            const void* v, int64_t v_row, int64_t v_head, const int32_t* cu_q, const int32_t* cu_k,

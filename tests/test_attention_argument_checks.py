@@ -112,3 +112,14 @@ def test_scales_with_which_finite_inputs_have_no_finite_scores(lib, scale):
     args[14], prompt[14] = 0, 0
     for most in (2.0 ** 64, -2.0 ** 64, 1.0):
         assert lib.uniql_kv4_attention(*args, most, None) == 0 and lib.uniql_prompt_attention(*prompt, most, None) == 0
+
+
+@pytest.mark.parametrize("count", [(1 << 30) + 1, (1 << 31) - 64, (1 << 31) - 1])
+def test_more_requests_than_sums_of_their_numbers_allow(lib, count):
+    p = ctypes.byref(cache())
+    assert lib.uniql_kv_assign_pages(*[FAKE] * 11, count, 1, 4, 16, 5, None) == -2
+    assert lib.uniql_kv4_load(p, FAKE, FAKE, None, FAKE, 1, 1, FAKE, 1, 1, count, 1, 1, None) == -2
+    acc, tmp = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    assert lib.uniql_kv4_attention_workspace(p, 1, count, 1, 4, ctypes.byref(acc), ctypes.byref(tmp)) == -2
+    assert lib.uniql_kv4_attention(FAKE, 1, 1, p, FAKE, FAKE, FAKE, FAKE, 1, 1, FAKE, 1 << 40, FAKE, 1 << 40, 1, count, 1, 4, 1.0, None) == -2
+    assert lib.uniql_prompt_attention(FAKE, 1, 1, FAKE, 1, 1, FAKE, 1, 1, FAKE, FAKE, FAKE, 1, 1, 4, 4, count, 4, 2, 64, 64, 1, 1.0, None) == -2

@@ -57,3 +57,11 @@ def test_attention_over_the_cache_and_loading(gpu):
     assert (buffer == 0).all()
     cache.load(table, rows, 52, k_out=buffer[:52, :2], v_out=buffer[1:, 2:])
     assert torch.equal(buffer[:52, :2], k) and torch.equal(buffer[1:, 2:], v)
+
+
+def test_offsets_of_more_sequences_than_a_call_takes(gpu):
+    from uniql_amd.attention import prompt_attention
+    x = torch.zeros(8, 4, 64, dtype=torch.float16, device=gpu)
+    for count, words in ((2 ** 32 + 2, "larger than a call"), (2 ** 30 + 2, "sizes")):
+        with pytest.raises(RuntimeError, match=words):
+            prompt_attention(x, x, x, torch.empty(count, dtype=torch.int32, device=gpu))

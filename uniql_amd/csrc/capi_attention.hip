@@ -19,14 +19,16 @@ int prompt_attention_launch(const PromptArgs& a, hipStream_t stream);
 using namespace uniql;
 
 static constexpr int kMaxHeads = 4096, kMaxWidth = 128;
+// requests or sequences: sums of two of their numbers, and steps beyond the last, stay below 2^31
+static constexpr int kMaxRequests = 1 << 30;
 
 // Scales up to 2^64: finite queries and keys (128 products of 2^32) then have finite scores, also with the factors that the
 // kernels fold into the scale.
 static bool scale_ok(float v) { return v >= -18446744073709551616.0f && v <= 18446744073709551616.0f; }
 static bool page_size_ok(int n) { return n == 16 || n == 32 || n == 64 || n == 128 || n == 256; }
-// columns of a table, and the tokens that a row of it has room for
+// rows and columns of a table, and the tokens that a row of it has room for
 static bool columns_ok(int64_t rows, int64_t columns, int64_t page_size) {
-    return columns > 0 && columns <= (1 << 20) && columns * page_size <= (1LL << 30) && rows * columns <= 0x7fffffffLL;
+    return rows <= kMaxRequests && columns > 0 && columns <= (1 << 20) && columns * page_size <= (1LL << 30) && rows * columns <= 0x7fffffffLL;
 }
 
 // Sizes first, then (when there is work to do) pointers.
@@ -149,7 +151,7 @@ int uniql_prompt_attention(const void* q, int64_t q_row, int64_t q_head, const v
                            int64_t out_head, int rows, int k_rows, int sequences, int n_q_heads, int n_kv_heads, int k_dim, int v_dim,
                            int causal, float scale, void* stream) {
     if (rows < 0 || k_rows < 0 || sequences < 0 || n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads > kMaxHeads ||
-        n_q_heads % n_kv_heads != 0 || k_dim <= 0 || v_dim <= 0)
+        n_q_heads % n_kv_heads != 0 || k_dim <= 0 || v_dim <= 0 || sequences > kMaxRequests)
         return UNIQL_E_SHAPE;
     if (k_dim > kMaxWidth || v_dim > kMaxWidth || !scale_ok(scale)) return UNIQL_E_UNSUPPORTED;
     if (rows == 0 || sequences == 0) return UNIQL_OK;

@@ -307,6 +307,7 @@ Tensor prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
     if (q.size(2) > 128 || v.size(2) > 128) fail("heads must be 1 to 128 wide");
     require_plain(cu_q, "cu_q", at::kInt, 1, q);
     if (cu_q.size(0) < 1) fail("cu_q must have at least one entry");
+    if (cu_q.size(0) > 0x7fffffff) fail("cu_q is larger than a call can take");
     const Tensor& cu_k = cu_k_in ? *cu_k_in : cu_q;
     if (cu_k_in) {
         require_plain(cu_k, "cu_k", at::kInt, 1, q);
