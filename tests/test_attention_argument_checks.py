@@ -123,3 +123,17 @@ def test_more_requests_than_sums_of_their_numbers_allow(lib, count):
     assert lib.uniql_kv4_attention_workspace(p, 1, count, 1, 4, ctypes.byref(acc), ctypes.byref(tmp)) == -2
     assert lib.uniql_kv4_attention(FAKE, 1, 1, p, FAKE, FAKE, FAKE, FAKE, 1, 1, FAKE, 1 << 40, FAKE, 1 << 40, 1, count, 1, 4, 1.0, None) == -2
     assert lib.uniql_prompt_attention(FAKE, 1, 1, FAKE, 1, 1, FAKE, 1, 1, FAKE, FAKE, FAKE, 1, 1, 4, 4, count, 4, 2, 64, 64, 1, 1.0, None) == -2
+
+
+@pytest.mark.parametrize("heads,q_heads", [(1, 4), (8, 32), (32, 32), (600, 600)])
+def test_scratch_does_not_grow_with_the_rows(lib, heads, q_heads):
+    """only rows that several workgroups share need some, and those are at most two for each of the 512 workgroups that a call is shared
+    out to (rounded up to whole ones a head): 8320 bytes and a word each"""
+    p = ctypes.byref(cache(heads=heads))
+    most = 2 * -(-512 // heads) * heads
+    for rows, requests in ((1, 1), (64, 64), (500, 500), (500, 3), (16384, 1), (16384, 300), (131072, 5)):
+        acc, tmp = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        assert lib.uniql_kv4_attention_workspace(p, rows, requests, 64, q_heads, ctypes.byref(acc), ctypes.byref(tmp)) == 0
+        assert 0 < tmp.value <= most * 8320 and 0 < acc.value <= 4 * most + 7
+        if rows == 1:
+            assert tmp.value < most * 8320 or heads >= 512

@@ -393,3 +393,49 @@ def test_many_small_weights_beside_a_large_one(gpu):
     weight = 2.0 ** -24.3
     want = (held_v[100, 0] + (held_v[:, 0].sum(0) - held_v[100, 0]) * weight) / (1 + (n - 1) * weight)
     assert ((got - want).abs() <= 2 ** -10).all(), float((got - want).abs().max())
+
+
+@pytest.mark.parametrize("lengths,tokens,h,g", [
+    ([5000, 4000, 900, 300, 3000], [3000, 1, 700, 90, 2500], 2, 1),      # rows of two workgroups, of one, of a wave
+    ([700] * 40 + [9000], [150] * 40 + [30], 4, 2), ([20000, 20000, 17], [1, 33, 5], 8, 1), ([12000], [12], 4, 4),
+])
+def test_scratch_of_just_the_size_asked_for(gpu, lengths, tokens, h, g):
+    """many rows and few, shared and not: nothing in front of the scratch memory and behind it is written, the counts are zeros afterwards"""
+    import ctypes
+    from uniql_amd import _capi
+    p = Problem(gpu, lengths, tokens, h, g, 32, 32, 64, seed=len(lengths))
+    q, table, n, cu = p.on_gpu()
+    c, lib, rows = p.cache, _capi.load(), p.q.shape[0]
+
+    class Cache(ctypes.Structure):
+        _fields_ = [(name, ctypes.c_void_p) for name in ("k_codes", "k_scales", "v_codes", "v_scales")] + \
+                   [(name, ctypes.c_int) for name in ("pages", "page_size", "heads", "k_dim", "v_dim")]
+
+    cache = Cache(c.k_codes.data_ptr(), c.k_scales.data_ptr(), c.v_codes.data_ptr(), c.v_scales.data_ptr(), c.num_pages, 64, g, 32, 32)
+    acc, tmp = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    assert lib.uniql_kv4_attention_workspace(ctypes.byref(cache), rows, len(lengths), table.shape[1], h, ctypes.byref(acc), ctypes.byref(tmp)) == 0
+    guard = 1 << 16
+    accum = torch.full((acc.value + 2 * guard,), 77, dtype=torch.uint8, device=gpu)
+    accum[guard:-guard] = 0
+    temp = torch.full((tmp.value + 2 * guard,), 77, dtype=torch.uint8, device=gpu)
+    out = torch.full((rows, h, 32), 9.0, device=gpu).half()
+    torch.cuda.synchronize()
+    for _ in range(2):
+        code = lib.uniql_kv4_attention(q.data_ptr(), h * 32, 32, ctypes.byref(cache), table.data_ptr(), n.data_ptr(),
+                                       None if cu is None else cu.data_ptr(), out.data_ptr(), h * 32, 32, accum[guard:].data_ptr(), acc.value,
+                                       temp[guard:].data_ptr(), tmp.value, rows, len(lengths), table.shape[1], h, 32 ** -0.5,
+                                       torch.cuda.current_stream().cuda_stream)
+        assert code == 0
+        torch.cuda.synchronize()
+    assert (accum[guard:-guard] == 0).all()
+    for t in (accum, temp):
+        assert (t[:guard] == 77).all() and (t[-guard:] == 77).all()
+    assert torch.equal(out, p.run())
+    for r, (size, count) in enumerate(zip(lengths, tokens)):      # some rows of each request against 64 bits
+        k, v = as_held(p.k[r])[0], as_held(p.v[r])
+        for first in sorted({0, count // 2, max(0, count - 20)}):
+            some = slice(p.cu[r] + first, p.cu[r] + min(count, first + 20))
+            seen = size - count + first + 1
+            o, mean_abs, spread = attention(p.q[some], k, v[0], 32 ** -0.5, seen)
+            held = attention(p.q[some], k, v[1].unsqueeze(-1), 32 ** -0.5, seen)[0]
+            assert ((out[some].cpu().double() - o).abs() <= bound(o, mean_abs, spread, size, held)).all(), (r, first)

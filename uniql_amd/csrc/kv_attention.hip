@@ -21,6 +21,8 @@
 // waves' sums 0.4, exchange and adding up 2).  The lengths are on the device, so every workgroup finds its share from them
 // (kPositions x request tiles, shared out evenly): requests of any lengths fill the GPU alike.  Where several workgroups share a
 // request's rows they leave (m, sum p, o) in scratch memory and the last to arrive adds them up in their order.
+#include <algorithm>
+
 #include "kv_attention.hpp"
 
 namespace uniql {
@@ -131,7 +133,8 @@ __device__ __forceinline__ Request requests_of(const KvAttentionArgs& a, int bas
 
 // A workgroup's share of a request's row tile `rows`.  Either the position tiles from `run * chunk` on, `run` of them, for one key /
 // value head, a tile a wave in turn; `chunks` workgroups share these rows, and their partial results lie in the places `place - chunk`
-// and on.  Or, `alone`, all of its positions, a head a wave: requests too short to keep four waves busy.
+// and on (rows of one workgroup need none: places are counted over those with whole runs, so there are at most twice as many as shares).
+// Or, `alone`, all of its positions, a head a wave: requests too short to keep four waves busy.
 struct Share {
     Request what;
     int request, rows, chunk, chunks, run, place, head;
@@ -178,10 +181,11 @@ __device__ __forceinline__ bool find_share(const KvAttentionArgs& a, Share& s) {
     s.head = (int)(blockIdx.x - index * (unsigned)heads);
     // The first round over the requests looks for `index` among the whole runs, the second among the rests and what is done alone; the
     // sums up to a request tell where its places begin.
+    // Whole runs, of which there are no more than shares, and the rests beside them go through one sum, sixteen bits each.
     unsigned all_runs = 0, all_rests = 0, alone_index = 0;
     bool alone = false;
     for (int round = 0; round < 2; ++round) {
-        unsigned runs = 0, rests = 0, alones = 0;
+        unsigned shared = 0, rests = 0, alones = 0;
         rows_end = 0;
         for (int base = 0; base < a.requests; base += 64) {
             if (a.requests > 64) q = requests_of(a, base, rows_end);
@@ -189,8 +193,10 @@ __device__ __forceinline__ bool find_share(const KvAttentionArgs& a, Share& s) {
             const Parts p = parts_of(position_tiles(q), run, by_run);
             const int64_t want = (int64_t)tiles * p.runs;
             const unsigned some = tiles < (1 << 24) ? (unsigned)tiles : 1u << 24;  // (more than any grid has)
-            const unsigned my_runs = want < (1 << 24) ? (unsigned)want : 1u << 24, my_rests = some * (unsigned)p.rest, my_alones = some * (unsigned)p.alone;
-            const unsigned upto_runs = runs + sums_upto(my_runs, add_u), upto_rests = rests + sums_upto(my_rests, add_u);
+            const unsigned my_runs = want < 0x7fff ? (unsigned)want : 0x7fffu, my_rests = some * (unsigned)p.rest, my_alones = some * (unsigned)p.alone;
+            const unsigned my_shared = my_runs | (p.runs > 0 ? my_rests << 16 : 0u);
+            const unsigned upto_shared = shared + sums_upto(my_shared, add_u), upto_rests = rests + sums_upto(my_rests, add_u);
+            const unsigned upto_runs = upto_shared & 0xffffu;
             unsigned upto = upto_runs, looked_for = index;
             if (round == 1) {
                 const unsigned upto_alones = alones + sums_upto(my_alones, add_u);
@@ -207,23 +213,23 @@ __device__ __forceinline__ bool find_share(const KvAttentionArgs& a, Share& s) {
                 s.alone = alone;
                 const int r = (int)lane_value((unsigned)p.runs, owner);
                 s.chunks = alone ? 1 : r + (int)lane_value((unsigned)p.rest, owner);
-                const unsigned before_runs = lane_value(upto_runs - my_runs, owner), before_rests = lane_value(upto_rests - my_rests, owner);
+                const unsigned before = lane_value(upto_shared - my_shared, owner);
                 if (round == 0) {
-                    const int at = (int)(index - before_runs);
+                    const int at = (int)(index - (before & 0xffffu));
                     s.rows = r == 1 ? at : at / r;
                     s.chunk = at - s.rows * r;
                 } else {
                     s.rows = (int)(looked_for - lane_value(upto - (alone ? my_alones : my_rests), owner));
                     s.chunk = alone ? 0 : r;
                 }
-                s.place = (int)(before_runs + before_rests) + s.rows * s.chunks + s.chunk;
+                s.place = (int)((before & 0xffffu) + (before >> 16)) + s.rows * s.chunks + s.chunk;
                 return true;
             }
-            runs = lane_value(upto_runs, 63);
+            shared = lane_value(upto_shared, 63);
             rests = lane_value(upto_rests, 63);
-            if ((runs | rests | alones) > 0x1fffffffu) return false;
+            if ((rests | alones) > 0x1fffffffu) return false;
         }
-        all_runs = runs;
+        all_runs = shared & 0xffffu;
         all_rests = rests;
         if (round == 0 && index >= all_runs + all_rests) {
             alone = true;
@@ -580,9 +586,11 @@ void kv4_attention_needs(int rows, int requests, int q_heads, const KvCache& cac
     // (with and without cu_q alike: the larger of the two)
     const int group = q_heads / cache.heads;
     const int64_t one = workgroups_of(rows, requests, group, cache.heads, true), many = workgroups_of(rows, requests, group, cache.heads, false);
-    const int64_t workgroups = (rows == requests && one > many ? one : many) * cache.heads;
-    *accum_bytes = (size_t)(workgroups * 4 + 7) / 8 * 8;
-    *temp_bytes = (size_t)workgroups * kSlotFloats * 4;
+    const int64_t workgroups = rows == requests && one > many ? one : many;
+    // rows that several workgroups share have a whole run at least, and one rest: two places for a share
+    const int64_t places = std::min(workgroups, 2 * shares_of(cache.heads)) * cache.heads;
+    *accum_bytes = (size_t)(places * 4 + 7) / 8 * 8;
+    *temp_bytes = (size_t)places * kSlotFloats * 4;
 }
 
 int kv4_attention_launch(const KvAttentionArgs& args, hipStream_t stream) {
