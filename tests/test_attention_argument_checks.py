@@ -137,3 +137,15 @@ def test_scratch_does_not_grow_with_the_rows(lib, heads, q_heads):
         assert 0 < tmp.value <= most * 8320 and 0 < acc.value <= 4 * most + 7
         if rows == 1:
             assert tmp.value < most * 8320 or heads >= 512
+
+
+def test_heads_without_width_are_refused_as_anything_else(lib):
+    """also where the scale is left to the width"""
+    import torch
+    from uniql_amd import ops
+    x = torch.zeros(3, 2, 0, dtype=torch.float16)
+    i = torch.zeros(2, dtype=torch.int32)
+    for call in (lambda: ops.prompt_attention(x, x, x, i), lambda: ops.kv4_attention(x, i, x, i, x, i, i, 64),
+                 lambda: ops.prompt_attention(x[0, 0, 0:].sum(), x, x, i)):
+        with pytest.raises(RuntimeError, match="GPU"):
+            call()

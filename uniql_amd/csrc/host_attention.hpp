@@ -38,6 +38,8 @@ void require_heads(const Tensor& t, const char* name) {
     if (t.size(0) > 0x7fffffff || t.size(1) > 0x7fffffff || t.size(2) > 0x7fffffff) fail(std::string(name) + " is larger than a call can take");
     if (t.size(1) == 0 || t.size(2) == 0) fail(std::string(name) + " has no heads or no width");
 }
+// The caller's scale, or that of the heads' width.
+float scale_of(const std::optional<double>& scale, const Tensor& q) { return (float)(scale ? *scale : 1.0 / std::sqrt((double)q.size(2))); }
 // Where the elements of [rows, heads, width] with unit inner stride lie, in elements; heads and rows that follow each other count as
 // one wider head.
 struct Lattice {
@@ -247,7 +249,7 @@ std::pair<Tensor, Tensor> kv4_load(const Tensor& k_codes, const Tensor& k_scales
 }
 
 Tensor kv4_attention(const Tensor& q, const Tensor& k_codes, const Tensor& k_scales, const Tensor& v_codes, const Tensor& v_scales,
-                     const Tensor& table, const Tensor& lengths, int64_t v_dim, const std::optional<Tensor>& cu_q, double scale,
+                     const Tensor& table, const Tensor& lengths, int64_t v_dim, const std::optional<Tensor>& cu_q, std::optional<double> scale,
                      const std::optional<Tensor>& out_in, uintptr_t stream, const py::object& accumulator) {
     const py::gil_scoped_release release;
     const at::NoGradGuard no_grad;
@@ -285,13 +287,13 @@ Tensor kv4_attention(const Tensor& q, const Tensor& k_codes, const Tensor& k_sca
                       cu_q ? cu_q->data_ptr<int>() : nullptr, out.data_ptr(), out.stride(0), out.stride(1),
                       need_accum ? accum.data_ptr() : nullptr, need_accum ? (size_t)accum.numel() * 8 : 0,
                       need_temp ? temp.data_ptr() : nullptr, need_temp, (int)rows, (int)requests, (int)table.size(1), (int)heads,
-                      (float)scale, reinterpret_cast<void*>(stream)),
+                      scale_of(scale, q), reinterpret_cast<void*>(stream)),
           "uniql_kv4_attention");
     return out;
 }
 
 Tensor prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const std::optional<Tensor>& cu_k_in,
-                        bool causal, double scale, const std::optional<Tensor>& out_in, uintptr_t stream) {
+                        bool causal, std::optional<double> scale, const std::optional<Tensor>& out_in, uintptr_t stream) {
     const py::gil_scoped_release release;
     const at::NoGradGuard no_grad;
     require_gpu(q, "q");
@@ -319,7 +321,7 @@ Tensor prompt_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
         fail("out must not be q, k or v or share memory with them");
     check(p_prompt(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
                    cu_q.data_ptr<int>(), cu_k.data_ptr<int>(), out.data_ptr(), out.stride(0), out.stride(1), (int)rows, (int)k_rows,
-                   (int)(cu_q.size(0) - 1), (int)heads, (int)kv_heads, (int)q.size(2), (int)v.size(2), causal, (float)scale,
+                   (int)(cu_q.size(0) - 1), (int)heads, (int)kv_heads, (int)q.size(2), (int)v.size(2), causal, scale_of(scale, q),
                    reinterpret_cast<void*>(stream)),
           "uniql_prompt_attention");
     return out;
@@ -346,6 +348,5 @@ std::pair<Tensor, Tensor> pool_load(const KvPool& p, const Tensor& table, const 
 Tensor pool_attend(const KvPool& p, const Tensor& q, const Tensor& table, const Tensor& lengths, const std::optional<Tensor>& cu_q,
                    std::optional<double> scale, const std::optional<Tensor>& out, uintptr_t stream, const py::object& accumulator) {
     require_width(q, "q", p.k_dim);
-    return kv4_attention(q, p.k_codes, p.k_scales, p.v_codes, p.v_scales, table, lengths, p.v_dim, cu_q,
-                         scale ? *scale : 1.0 / std::sqrt((double)p.k_dim), out, stream, accumulator);
+    return kv4_attention(q, p.k_codes, p.k_scales, p.v_codes, p.v_scales, table, lengths, p.v_dim, cu_q, scale, out, stream, accumulator);
 }

@@ -650,8 +650,8 @@ def kv4_attention(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor
     columns]; lengths int32 [requests], the new tokens among them; cu_q int32 [requests + 1]: each request's rows (None: one
     each).  scale: 1 / sqrt(k_dim) when None.  Returns fp16 [rows, q heads, v_dim]; rows outside every request are left as they
     were (in out) or as allocated."""
-    return _capi.host().kv4_attention(q, k_codes, k_scales, v_codes, v_scales, table, lengths, v_dim, cu_q,
-                                      q.shape[-1] ** -0.5 if scale is None else scale, out, _stream_of(q, "q"), _accumulator)
+    return _capi.host().kv4_attention(q, k_codes, k_scales, v_codes, v_scales, table, lengths, v_dim, cu_q, scale, out,
+                                      _stream_of(q, "q"), _accumulator)
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor | None = None, *,
@@ -660,5 +660,4 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     [rows, kv heads, ..] (ranges of the fused projection's output too), cu_q / cu_k int32 [sequences + 1].  Causal masks are aligned
     at the sequences' ends.  scale: 1 / sqrt(width) when None.  Returns fp16 [rows, q heads, v width]; rows outside every sequence
     are left as they were (in out) or as allocated."""
-    return _capi.host().prompt_attention(q, k, v, cu_q, cu_k, causal, q.shape[-1] ** -0.5 if scale is None else scale, out,
-                                         _stream_of(q, "q"))
+    return _capi.host().prompt_attention(q, k, v, cu_q, cu_k, causal, scale, out, _stream_of(q, "q"))
