@@ -48,3 +48,13 @@ def bound(o, a, spread, keys, held=None):
     if held is not None:
         tol = tol + 16 * sums * held
     return tol
+
+
+def close_bound(o, a, keys, score_error, smallest):
+    """How far the kernels' arithmetic may be from 64 bits, without room for another: the result's rounding (half a step); the
+    weights' rounding to fp16 in front of the second product, half a step of each term and, where the sum of weights takes the rounded ones, of
+    the sum (a = sum p |v|); below fp16's normal range `smallest` for each key, half of 2^-24 over what the largest weight is lifted to;
+    scores off by score_error [t, h] (absolute), in numerator and denominator; fp32 sums over the keys, a lane's quarter of them one
+    after the other (an error of 2^-24 each) and some 64 steps to join them; the exponentials (2^-22)."""
+    sums = 2.0 ** -24 * (keys / 4 + 64) + 2.0 ** -22
+    return HALF_STEP * o.abs() + (HALF_STEP + 2 * score_error.unsqueeze(-1) + 2 * sums) * (a + o.abs()) + keys * smallest.unsqueeze(-1)
