@@ -10,16 +10,16 @@
 // (The values' 8 is taken off in front of the product, one more instruction a pair: behind it, over 65536 positions, the difference of two sums
 // 80 times as large as itself was four times as far from the exact result.)
 // with w_j = fp16(p_j s'_j).  For w_j to use fp16's range whatever the values' sizes, m is the running maximum of each
-// position's score with the exponent of its s'_j, less 6: w_j < 2^7 at the maximum, and it moves only when some w_j might pass 2^15.  (Largest score
+// position's score with the exponent of its s'_j, less 6: w_j is 2^5 to 2^6 at the maximum, and it moves only when some w_j might pass 2^14.  (Largest score
 // and largest exponent apart save 1 % of the time, but lose small values that have the weight beside large ones that have none.)
 // Beyond 2^22 (in powers of two), where such sums are rounded by as much as the room that weights have, m is the largest score alone.
 // The rounding of w_j (2^-11) is what a matrix instruction on fp16 asks for; sums, maxima and the output stay in fp32.
 //
 // Bound by HBM: 132 bytes for a position of 128 + 128 channels (16 requests of 65536 tokens, 8 heads of 128: 198 us, 5.6 TB/s; a kernel
 // that sums up 2 GB reads 6.1).  Fewer bytes are bound by latency: share, page numbers, positions, sums, exchange follow each other (1 x 4096
-// 10.9 us, 48 requests of 1 to 8192 17.0: finding the share 1 us, the first positions 1.5, 1.5 for each further 64 a wave takes, the
+// 10.9 us, 48 requests of 1 to 8192 16.9: finding the share 1 us, the first positions 1.5, 1.5 for each further 64 a wave takes, the
 // waves' sums 0.4, exchange and adding up 2).  The lengths are on the device, so every workgroup finds its share from them
-// (kPositions x request tiles, shared out evenly): requests of any lengths fill the GPU alike.  Where several workgroups share a
+// (tiles of 64 positions x tiles of 16 rows, shared out evenly): requests of any lengths fill the GPU alike.  Where several workgroups share a
 // request's rows they leave (m, sum p, o) in scratch memory and the last to arrive adds them up in their order.
 #include <algorithm>
 
@@ -37,11 +37,12 @@ constexpr int kSlotFloats = 16 * 130;  // a workgroup's partial result: 16 rows 
 constexpr int kDeviceScope = 16;       // cache policy bit sc1: as relaxed device-scope loads and stores compile to
 constexpr int kOutStride = 132;
 constexpr float kNoMaximum = -3.0e38f;
-constexpr float kLift = 6.0f;          // weights at the maximum reach 2^6 to 2^7: ones 2^-24 as large are many in a long cache and keep five bits
+constexpr float kLift = 6.0f;          // weights at the maximum are 2^5 to 2^6: ones 2^-24 as large are many in a long cache and keep five bits
 constexpr float kSlack = kLift + 8.0f; // they may grow by 2^8 before the maximum follows
 constexpr float kFar = 4194304.0f;     // 2^22: below it a score's sum with an exponent is off by a quarter at most
 // Workgroups that a call is shared out to, two a compute unit, as many as its registers allow to run at once: what does not fit waits for a
-// whole one to end (us with 512 / 768 / 1024: 9 x 5 pruned 15.3 / 20.4 / 20.5, 16 x 65536 199 / 200 / 204, 1 x 4096 10.3 for all).
+// whole one to end (us with 512 / 768 / 1024: 9 x 5 pruned 15 / 21 / 21, 48 requests 17 / 19 / 19, 16 x 65536 198 / 199 / 202, 1 x 4096 10.9
+// for all).
 constexpr int kWorkgroups = 512;
 
 template <int S>

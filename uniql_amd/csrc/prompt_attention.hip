@@ -14,11 +14,11 @@
 // 2.121 -> 2.156).
 // The rounding of the weights to fp16 (2^-11) is what a matrix instruction on fp16 asks for; their sum takes the rounded ones.
 //
-// Bound by the matrix and vector instructions together, and by power: 32 + 8 heads of 128, 16384 tokens 2.08 to 2.18 ms, 1.01 to 1.06
-// PFLOP/s, where the library's product of 16384 x 16384 reaches 1.26 at the clock that the GPU holds; 8 prompts of 2048 0.83, 1 of 2048
-// 0.64, 24 of 1 to 1850 tokens 0.66.  A step of 64 keys is 32 matrix instructions of 32 clocks for a wave, and beside the next tile's
+// Bound by the matrix and vector instructions together, and by power: 32 + 8 heads of 128, 16384 tokens 2.11 to 2.19 ms, 1.00 to 1.04
+// PFLOP/s, where the library's product of 16384 x 16384 reaches 1.26 at the clock that the GPU holds; 8 prompts of 2048 0.82, 1 of 2048
+// 0.66, 24 of 1 to 1850 tokens 0.60 to 0.65.  A step of 64 keys is 32 matrix instructions of 32 clocks for a wave, and beside the next tile's
 // scores 32 exponentials, as many products, 16 conversions and 16 sums; two workgroups a compute unit fill each other's gaps.  Short
-// prompts are bound by latency (1 token 6.7 us, 333 12): offsets, queries and the first tile follow each other, then 1.2 us a step.
+// prompts are bound by latency (1 token 6.8 us, 333 12): offsets, queries and the first tile follow each other, then 1.2 us a step.
 // Tried and taken out: two sets of four waves that share the keys out (333 tokens 14.3 -> 13.9, 24 prompts 81 -> 107 us: a compute unit
 // then holds one workgroup), blocks of all sequences in order of their length (24 prompts 75 -> 74, 64 of 512 276 -> 299 us), V's pieces
 // exchanged so that no read meets another in a bank (a third of the LDS cycles less, 333 tokens 12.7 -> 12.55, 16384 2.115 -> 2.135 ms).
