@@ -476,6 +476,69 @@ int uniql_prompt_attention(const void* q, int64_t q_row, int64_t q_head, const v
                            int n_q_heads, int n_kv_heads, int k_dim, int v_dim, int causal, float scale, void* stream);
 
 
+/*
+ * ---- between the projections of a state-space layer: causal convolution, scan, gated norm --------------------------------
+ * The reference calls third-party kernels there (modeling/mamba/mamba2_qblocks.py: causal_conv1d_fn / _update,
+ * mamba_chunk_scan_combined, selective_state_update, a gated RMS norm), none of which are in its tree; these calls are
+ * this library's own.  fp16 rows, states of the convolution in fp16, of the scan in fp32.
+ *
+ * Which rows belong to which sequence (request), and where its states lie in a pool of `pool` places:
+ *   cu       device, int32 [count + 1]: the rows cu[s] .. cu[s + 1] are sequence s's (ascending); NULL: a row each (count == rows)
+ *   starts   device, int32 [count]: tokens that a sequence has had before; where it is 0 (or less) the sequence begins with an empty state, whatever
+ *            its place holds; NULL: all are continued
+ *   places   device, int32 [count]: a sequence's place in the pool; NULL: place s.  Sequences whose place is outside the pool (-1) are
+ *            left out: their rows of the output stay as they were.  A place must not occur twice among sequences that have rows
+ * Rows in no sequence stay as they were, and so do the places of sequences without rows.  count <= 2^24, rows <= 2^27.
+ * Where `state` is NULL all sequences begin with an empty state; where `state_out` is NULL the new states are dropped; where both are,
+ * `pool` is not looked at and any place >= 0 counts.  `state_out` may be `state`, and must not overlap it otherwise.
+ */
+typedef struct uniql_sequences {
+    const int32_t *cu, *starts, *places;
+    int count, pool;
+} uniql_sequences;
+
+/*
+ * out[t, c] = f(bias[c] + sum_k weight[c, k] x[t - width + 1 + k, c]) along each sequence, f(u) = u / (1 + exp(-u)) with `activation`,
+ * u otherwise; fp32, rounded once.  Inputs in front of a sequence's first row come from its state, the last width - 1 of before.
+ *   x        device, fp16 [rows, channels], unit stride along the channels, x_row elements between rows
+ *   weight   device, fp16 [channels, width], width 2 to 4;  bias  device, fp16 [channels], or NULL
+ *   state, state_out   device, fp16 [pool, width - 1, channels], the latest input last
+ *   out      device out, fp16 [rows, channels], out_row elements between rows; must not overlap x
+ */
+int uniql_causal_conv(const void* x, int64_t x_row, const void* weight, const void* bias, const void* state, void* state_out,
+                      const uniql_sequences* sequences, void* out, int64_t out_row, int rows, int channels, int width, int activation,
+                      void* stream);
+
+/*
+ * Linear attention with a decay for each head: with s = dt + dt_bias (then log(1 + exp(s)) with `softplus`, then held between dt_min and dt_max, 0 <= dt_min),
+ *   S' = exp(s decay) S + s x b^T,  y = S' c + skip x     for each head's state S [head_dim, states] and each row in turn.
+ *   x        device, fp16 [rows, heads, head_dim];  b, c  device, fp16 [rows, groups, states], head h uses group h / (heads / groups);
+ *            unit stride along the last axis, *_row, *_head and *_group elements between rows, heads and groups
+ *   dt       device, fp16 [rows, heads], unit stride along the heads, dt_row elements between rows
+ *   decay    device, float [heads]: negative rates;  skip, dt_bias  device, float [heads], or NULL: 0
+ *   state, state_out   device, float [pool, heads, head_dim, states], 16-byte aligned
+ *   y        device out, fp16 [rows, heads, head_dim], strides likewise; must not overlap the inputs
+ *   temp     scratch memory of any contents, 16-byte aligned, not shared by calls that may run at the same time; its size from
+ *            uniql_state_space_scan_workspace (0 without cu)
+ * head_dim 1 to 128, states 1 to 256, heads <= 2^15.  A row's output depends on its sequence's rows up to it alone, whatever the others hold.
+ */
+int uniql_state_space_scan_workspace(int rows, int count, int heads, int groups, int head_dim, int states, size_t* temp_bytes);
+int uniql_state_space_scan(const void* x, int64_t x_row, int64_t x_head, const void* dt, int64_t dt_row, const float* decay, const void* b,
+                           int64_t b_row, int64_t b_group, const void* c, int64_t c_row, int64_t c_group, const float* skip,
+                           const float* dt_bias, int softplus, float dt_min, float dt_max, const float* state, float* state_out,
+                           const uniql_sequences* sequences, void* y, int64_t y_row, int64_t y_head, void* temp, size_t temp_bytes,
+                           int rows, int heads, int groups, int head_dim, int states, void* stream);
+
+/*
+ * u = x z / (1 + exp(-z)), out = u / sqrt(mean(u^2) + eps) weight, the mean over each of `groups` equal ranges of a row's channels; fp32,
+ * rounded once.
+ *   x, z     device, fp16 [rows, channels], unit stride along the channels, *_row elements between rows;  weight  device, fp16 [channels]
+ *   out      device out, fp16 [rows, channels], out_row elements between rows; may be x or z itself, must not overlap them otherwise
+ */
+int uniql_gated_group_norm(const void* x, int64_t x_row, const void* z, int64_t z_row, const void* weight, void* out, int64_t out_row,
+                           int rows, int channels, int groups, float eps, void* stream);
+
+
 #ifdef __cplusplus
 }
 #endif

@@ -75,6 +75,15 @@ SIGNATURES = {
     "uniql_prompt_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
                                        c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int, c_int, c_int,
                                        c_int, c_int, c_int, c_int, c_int, c_float, c_void_p]),
+    "uniql_causal_conv": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                  c_int, c_int, c_int, c_int, c_void_p]),
+    "uniql_state_space_scan_workspace": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, ctypes.POINTER(c_size_t)]),
+    "uniql_state_space_scan": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64,
+                                       c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_float, c_float, c_void_p, c_void_p,
+                                       c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_size_t,
+                                       c_int, c_int, c_int, c_int, c_int, c_void_p]),
+    "uniql_gated_group_norm": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                                       c_int, c_int, c_int, c_float, c_void_p]),
 }
 
 _lib = None
@@ -136,6 +145,9 @@ def host():
                                     for fn in (lib.uniql_kv_assign_pages, lib.uniql_kv4_store, lib.uniql_kv4_load,
                                                lib.uniql_kv4_attention_workspace, lib.uniql_kv4_attention, lib.uniql_prompt_attention,
                                                lib.uniql_stream_capture_id)))
+            module.bind_state_space(*(ctypes.cast(fn, ctypes.c_void_p).value
+                                      for fn in (lib.uniql_causal_conv, lib.uniql_state_space_scan, lib.uniql_state_space_scan_workspace,
+                                                 lib.uniql_gated_group_norm)))
             module.bind(*(ctypes.cast(fn, ctypes.c_void_p).value
                           for fn in (lib.uniql_w4a16_linear, lib.uniql_w4a16_linear_workspace, lib.uniql_w4_embedding_lookup,
                                      lib.uniql_fwht, lib.uniql_fwht_composite, lib.uniql_fwht_columns, lib.uniql_w4a16_quantize,

@@ -1,0 +1,150 @@
+// The causal convolution of a state-space layer: y[t, c] = f(bias[c] + sum_k w[c, k] x[t - W + 1 + k, c]), f SiLU or nothing, inputs in front
+// of a sequence's first row from its state (the last W - 1 inputs of before) or zeros.
+//
+// A thread takes eight channels and a run of rows, of which it reads each once: the last W - 1 stay in registers.  The first W - 1
+// rows of a sequence, and its new state, belong to a workgroup of their own: it has read the state before it writes it, which makes
+// a state that is replaced in place safe, and a batch of single tokens is these workgroups alone.
+//
+// Bound by HBM.
+#include "state_space.hpp"
+
+namespace uniql {
+
+constexpr int kConvThreads = 256;
+constexpr int kConvRows = 32;  // rows of a run
+
+template <int W>
+struct Taps {
+    float w[W][8], bias[8];
+    __device__ __forceinline__ void load(const ConvArgs& a, int c0, int left) {
+        h8 v[W];
+#pragma unroll
+        for (int k = 0; k < W; ++k) v[k] = load_halves(a.weight + (int64_t)c0 * W + 8 * k, left * W - 8 * k);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int k = 0; k < W; ++k) w[k][e] = (float)v[(e * W + k) / 8][(e * W + k) % 8];
+        const h8 b = a.bias ? load_halves(a.bias + c0, left) : h8{};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) bias[e] = (float)b[e];
+    }
+    // x[0 .. W-1]: the inputs of a row, the oldest first
+    __device__ __forceinline__ h8 apply(const h8 (&x)[W], bool activation) const {
+        h8 y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float u = bias[e];
+#pragma unroll
+            for (int k = 0; k < W; ++k) u = __builtin_fmaf((float)x[k][e], w[k][e], u);
+            y[e] = (half_t)(activation ? silu_fast(u) : u);
+        }
+        return y;
+    }
+};
+
+// The largest s in -1 .. count - 1 with cu[s] <= row, for offsets that ascend; all lanes of a wave ask for the same row.
+__device__ __forceinline__ int last_not_behind(const int32_t* cu, int count, int row) {
+    const int lane = threadIdx.x & 63;
+    int below = -1, above = count;  // cu[below] <= row < cu[above]
+    while (above - below > 1) {
+        const int span = above - below - 1, step = (span + 63) / 64;
+        const int at = below + (lane + 1) * step;
+        const bool fits = at < above && cu[at] <= row;
+        const int n = __builtin_popcountll(__ballot(fits));
+        const int upper = below + (n + 1) * step;
+        below += n * step;
+        above = upper < above ? upper : above;
+    }
+    return below;
+}
+
+template <int W>
+__global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(const ConvArgs a) {
+    const int c0 = (blockIdx.y * kConvThreads + threadIdx.x) * 8, left = a.channels - c0;
+    Taps<W> taps;
+    const bool active = left > 0;
+    if ((int)blockIdx.x >= a.tiles) {
+        // a sequence's first rows and its state
+        const Sequence q = sequence_of(a.sequences, blockIdx.x - a.tiles);
+        if (q.rows == 0 || !active) return;
+        h8 x[2 * (W - 1)];  // the state, the first rows
+        const int64_t at = ((int64_t)q.place * (W - 1)) * a.channels + c0;
+        const half_t* from = a.x + (int64_t)q.first * a.x_row + c0;
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) {
+            x[k] = a.state && q.continued ? load_halves(a.state + at + (int64_t)k * a.channels, left) : h8{};
+            x[W - 1 + k] = k < q.rows ? load_halves(from + k * a.x_row, left) : h8{};
+        }
+        taps.load(a, c0, left);
+        if (a.state_out) {
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k) {
+                h8 v = x[W - 2 + 1 + k];
+                if (q.rows >= W - 1) {
+                    v = load_halves(from + (int64_t)(q.rows - (W - 1) + k) * a.x_row, left);
+                } else {
+#pragma unroll
+                    for (int r = 1; r < W - 1; ++r)
+                        if (q.rows == r) v = x[r + k];
+                }
+                store_halves(a.state_out + at + (int64_t)k * a.channels, v, left);
+            }
+        }
+        half_t* to = a.out + (int64_t)q.first * a.out_row + c0;
+#pragma unroll
+        for (int r = 0; r < W - 1; ++r)
+            if (r < q.rows) {
+                h8 row[W];
+#pragma unroll
+                for (int k = 0; k < W; ++k) row[k] = x[r + k];
+                store_halves(to + r * a.out_row, taps.apply(row, a.activation), left);
+            }
+        return;
+    }
+    const int row0 = blockIdx.x * kConvRows, rows = a.sequences.rows - row0 < kConvRows ? a.sequences.rows - row0 : kConvRows;
+    const int32_t* cu = a.sequences.cu;
+    int s = last_not_behind(cu, a.sequences.count, row0);
+    if (!active) return;
+    taps.load(a, c0, left);
+    h8 x[W];
+#pragma unroll
+    for (int k = 1; k < W; ++k) {
+        const int row = row0 - W + k;
+        x[k] = row >= 0 ? load_halves(a.x + (int64_t)row * a.x_row + c0, left) : h8{};
+    }
+    int first = 0, next = 0x7fffffff;  // of the sequence that the row belongs to; `first` passes all rows where it has none
+    auto enter = [&](int row) __attribute__((always_inline)) {
+        while (s + 1 < a.sequences.count && cu[s + 1] <= row) ++s;
+        first = 0x7fffffff;
+        next = s < a.sequences.count ? cu[s + 1] : 0x7fffffff;
+        if (s < 0) return;
+        const Sequence q = sequence_of(a.sequences, s);
+        if (row < q.first + q.rows) first = q.first;
+        else if (next <= row) next = 0x7fffffff;  // behind the last
+    };
+    enter(row0);
+    const half_t* from = a.x + (int64_t)row0 * a.x_row + c0;
+    half_t* to = a.out + (int64_t)row0 * a.out_row + c0;
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) x[k] = x[k + 1];
+        x[W - 1] = load_halves(from + (int64_t)r * a.x_row, left);
+        if (row0 + r >= next) enter(row0 + r);
+        if (row0 + r - (W - 1) >= first) store_halves(to + (int64_t)r * a.out_row, taps.apply(x, a.activation), left);
+    }
+}
+
+int causal_conv_launch(const ConvArgs& args, int width, hipStream_t stream) {
+    ConvArgs a = args;
+    a.tiles = a.sequences.cu ? (a.sequences.rows + kConvRows - 1) / kConvRows : 0;
+    const int64_t across = (int64_t)a.tiles + a.sequences.count, down = (a.channels + 8 * kConvThreads - 1) / (8 * kConvThreads);
+    if (across * kConvThreads >= (1LL << 32) || down > 65535) return UNIQL_E_SHAPE;
+    const dim3 grid((unsigned)across, (unsigned)down), block(kConvThreads);
+    if (width == 2) hipLaunchKernelGGL(causal_conv_kernel<2>, grid, block, 0, stream, a);
+    else if (width == 3) hipLaunchKernelGGL(causal_conv_kernel<3>, grid, block, 0, stream, a);
+    else hipLaunchKernelGGL(causal_conv_kernel<4>, grid, block, 0, stream, a);
+    return hipGetLastError() == hipSuccess ? UNIQL_OK : UNIQL_E_LAUNCH;
+}
+
+}  // namespace uniql

@@ -311,6 +311,7 @@ std::pair<Tensor, Tensor> cut_rows(const Tensor& B, const Tensor& s, int n, int 
 }
 
 #include "host_attention.hpp"
+#include "host_state_space.hpp"
 
 }  // namespace
 
@@ -348,6 +349,10 @@ PYBIND11_MODULE(_host, module) {
     module.def("kv4_load", &kv4_load);
     module.def("kv4_attention", &kv4_attention);
     module.def("prompt_attention", &prompt_attention);
+    module.def("bind_state_space", &bind_state_space);
+    module.def("causal_conv", &causal_conv);
+    module.def("state_space_scan", &state_space_scan);
+    module.def("gated_group_norm", &gated_group_norm);
     module.def("share_memory", &share_memory);
     module.def("overlaps_itself", &overlaps_itself);
     py::class_<KvPool>(module, "KvPool")

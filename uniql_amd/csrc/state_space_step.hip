@@ -1,0 +1,114 @@
+// One more token of every request through a state-space layer: S' = exp(s a) S + s x b^T, y = S' c + d x, with the time step
+// s = softplus(dt + bias), for each head's matrix S [head_dim][states] of fp32.
+//
+// Lanes lie along the states, four to a lane, so that rows of S come and go in whole lines; a wave takes 64 / LANES rows of the head at
+// once, and a thread ROWS of them, all on their way before the first is used.  The products with c are summed over the lanes.
+//
+// Bound by HBM: the state is read and written once.
+#include "state_space.hpp"
+
+namespace uniql {
+
+constexpr int kStepThreads = 256;
+
+// LANES: of a row; EACH: neighbouring states of a lane, PARTS: how often the lanes go over the row.
+template <int LANES, int EACH, int PARTS, int ROWS>
+__global__ __launch_bounds__(kStepThreads) void state_space_step_kernel(const ScanArgs a) {
+    constexpr int kAtOnce = kStepThreads / LANES;  // rows that the workgroup covers in one go
+    const unsigned per_sequence = (unsigned)(a.heads * a.head_blocks);
+    const unsigned s = blockIdx.x / per_sequence, rest = blockIdx.x % per_sequence;
+    const int head = rest / a.head_blocks, block = rest % a.head_blocks;
+    const Sequence q = sequence_of(a.sequences, (int)s);
+    if (q.rows == 0) return;
+    const int lane = threadIdx.x % LANES, p0 = block * kAtOnce * ROWS + threadIdx.x / LANES;
+    const int64_t size = (int64_t)a.head_dim * a.states;
+    const int64_t at = ((int64_t)q.place * a.heads + head) * size;
+    float S[ROWS][PARTS][EACH];
+    typedef float vec __attribute__((ext_vector_type(EACH)));
+    const bool from_state = a.state && q.continued;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+            const int p = p0 + r * kAtOnce, n = (i * LANES + lane) * EACH;
+            vec v = {};
+            if (from_state && p < a.head_dim && n < a.states) v = *reinterpret_cast<const vec*>(a.state + at + (int64_t)p * a.states + n);
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) S[r][i][e] = v[e];
+        }
+    const int group = head / a.share;
+    const half_t* const b_from = a.b + (int64_t)q.first * a.b_row + group * a.b_group;
+    const half_t* const c_from = a.c + (int64_t)q.first * a.c_row + group * a.c_group;
+    const half_t* const x_from = a.x + (int64_t)q.first * a.x_row + head * a.x_head;
+    float b[PARTS][EACH], c[PARTS][EACH], x[ROWS];
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i)
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const int n = (i * LANES + lane) * EACH;
+            b[i][e] = n < a.states ? (float)b_from[n + e] : 0.f;
+            c[i][e] = n < a.states ? (float)c_from[n + e] : 0.f;
+        }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        const int p = p0 + r * kAtOnce;
+        x[r] = p < a.head_dim ? (float)x_from[p] : 0.f;
+    }
+    const float step = time_step(a, (float)a.dt[(int64_t)q.first * a.dt_row + head], a.dt_bias ? a.dt_bias[head] : 0.f);
+    const float decay = expf(step * a.a[head]), skip = a.d ? a.d[head] : 0.f;
+    float y[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        const float in = step * x[r];
+        y[r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i)
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                // (an empty state is not multiplied: a decay that is no number would not leave it empty)
+                S[r][i][e] = from_state ? __builtin_fmaf(S[r][i][e], decay, in * b[i][e]) : in * b[i][e];
+                y[r] = __builtin_fmaf(S[r][i][e], c[i][e], y[r]);
+            }
+    }
+    if (a.state_out) {
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) {
+                const int p = p0 + r * kAtOnce, n = (i * LANES + lane) * EACH;
+                vec v;
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) v[e] = S[r][i][e];
+                if (p < a.head_dim && n < a.states) *reinterpret_cast<vec*>(a.state_out + at + (int64_t)p * a.states + n) = v;
+            }
+    }
+    half_t* const to = a.y + (int64_t)q.first * a.y_row + head * a.y_head;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        const int p = p0 + r * kAtOnce;
+        const float sum = sum_over<LANES>(y[r]);
+        if (lane == 0 && p < a.head_dim) to[p] = (half_t)(a.d ? __builtin_fmaf(skip, x[r], sum) : sum);
+    }
+}
+
+template <int LANES, int EACH, int PARTS, int ROWS>
+static int go(ScanArgs& a, hipStream_t stream) {
+    constexpr int rows = kStepThreads / LANES * ROWS;
+    a.head_blocks = (a.head_dim + rows - 1) / rows;
+    const int64_t blocks = (int64_t)a.sequences.count * a.heads * a.head_blocks;
+    if (blocks * kStepThreads >= (1LL << 32)) return UNIQL_E_SHAPE;
+    hipLaunchKernelGGL((state_space_step_kernel<LANES, EACH, PARTS, ROWS>), dim3((unsigned)blocks), dim3(kStepThreads), 0, stream, a);
+    return hipGetLastError() == hipSuccess ? UNIQL_OK : UNIQL_E_LAUNCH;
+}
+
+int state_space_step_launch(const ScanArgs& args, hipStream_t stream) {
+    ScanArgs a = args;
+    const bool whole = a.states % 4 == 0;
+    if (!whole) return go<64, 1, 4, 2>(a, stream);
+    if (a.states <= 32) return go<8, 4, 1, 2>(a, stream);
+    if (a.states <= 64) return go<16, 4, 1, 4>(a, stream);
+    if (a.states <= 128) return go<32, 4, 1, 8>(a, stream);
+    return go<64, 4, 1, 8>(a, stream);
+}
+
+}  // namespace uniql

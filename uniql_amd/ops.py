@@ -27,6 +27,7 @@ __all__ = [
     "w4a16_read_floor", "w4a16_quantize", "w4a16_pack", "w4a16_unpack", "w4a16_cut_columns",
     "w4a16_cut_rows", "w4_embedding_quantize", "rope_indices_",
     "kv_assign_pages", "kv4_store", "kv4_load", "kv4_attention", "prompt_attention",
+    "causal_conv", "state_space_scan", "gated_group_norm",
 ]
 
 
@@ -661,3 +662,40 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     at the sequences' ends.  scale: 1 / sqrt(width) when None.  Returns fp16 [rows, q heads, v width]; rows outside every sequence
     are left as they were (in out) or as allocated."""
     return _capi.host().prompt_attention(q, k, v, cu_q, cu_k, causal, scale, out, _stream_of(q, "q"))
+
+
+# ---- between the projections of a state-space layer ------------------------------------------------------------------
+# No counterpart in the reference's extensions: its blocks call third-party kernels there.  state_space.StateSpaceMixer puts them together.
+
+def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, state: torch.Tensor | None = None,
+                cu: torch.Tensor | None = None, places: torch.Tensor | None = None, starts: torch.Tensor | None = None,
+                state_out: torch.Tensor | None = None, activation: bool = True, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Each channel convolved with its own `width` weights along the sequences, then SiLU (uniql_causal_conv): x fp16 [rows, channels] (a
+    range of a projection's output too), weight fp16 [channels, 2 to 4], bias fp16 [channels].  cu int32 [sequences + 1]: the rows of
+    each sequence; without it every row is the next token of a request.  state fp16 [places, width - 1, channels]: the last inputs of each
+    request, replaced by the new ones (those go to state_out when given); places int32 [sequences] (sequence s has place s when None;
+    -1: left out); starts int32 [sequences]: 0 where a sequence begins, whatever its place holds (None: all are continued).
+    Returns fp16 [rows, channels]; rows in no sequence are left as they were (in out) or as allocated."""
+    return _capi.host().causal_conv(x, weight, bias, state, cu, places, starts, state_out, activation, out, _stream_of(x, "x"))
+
+
+def state_space_scan(x: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, *, d: torch.Tensor | None = None,
+                     dt_bias: torch.Tensor | None = None, softplus: bool = True, dt_limit: tuple = (0.0, float("inf")),
+                     state: torch.Tensor | None = None, cu: torch.Tensor | None = None, places: torch.Tensor | None = None,
+                     starts: torch.Tensor | None = None, state_out: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Linear attention with a decay for each head (uniql_state_space_scan): S' = exp(s a) S + s x b^T, y = S' c + d x for each row in turn,
+    s = softplus(dt + dt_bias) held within dt_limit (from 0 on: a time step
+    cannot be negative).  x fp16 [rows, heads, head_dim], b and c fp16 [rows, groups, states] (ranges
+    of a larger buffer too), dt fp16 [rows, heads], a, d and dt_bias float [heads] (a: negative).  state float [places, heads, head_dim, states];
+    cu, places, starts and state_out as for causal_conv: with cu whole prompts, pieces of prompts and single tokens in one batch,
+    without it one more token of every request.  Returns fp16 [rows, heads, head_dim]; rows in no sequence are left as they were
+    (in out) or as allocated."""
+    return _capi.host().state_space_scan(x, dt, a, b, c, d, dt_bias, softplus, dt_limit[0], dt_limit[1], state, cu, places, starts, state_out,
+                                         out, _stream_of(x, "x"))
+
+
+def gated_group_norm(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, groups: int = 1, eps: float = 1e-5, *,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """u = x silu(z), then u / sqrt(mean(u^2) + eps) weight over each of `groups` ranges of the channels (uniql_gated_group_norm): x and z
+    fp16 [rows, channels] (ranges of a larger buffer too), weight fp16 [channels].  out may be x or z.  Returns fp16 [rows, channels]."""
+    return _capi.host().gated_group_norm(x, z, weight, groups, eps, out, _stream_of(x, "x"))
