@@ -102,9 +102,25 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(const ConvArg
         return;
     }
     const int row0 = blockIdx.x * kConvRows, rows = a.sequences.rows - row0 < kConvRows ? a.sequences.rows - row0 : kConvRows;
-    const int32_t* cu = a.sequences.cu;
-    int s = last_not_behind(cu, a.sequences.count, row0);
-    if (!active) return;
+    // Rows that have W - 1 others of their sequence in front of them, a bit each: 64 sequences at a time, which share no bits.
+    const int lane = threadIdx.x & 63;
+    uint32_t allowed = 0;
+    for (int base = __builtin_amdgcn_readfirstlane(last_not_behind(a.sequences.cu, a.sequences.count, row0)); base < a.sequences.count; base += 64) {
+        const int s = base + lane;
+        int first = kConvRows, last = kConvRows;
+        if (s >= 0 && s < a.sequences.count) {
+            const Sequence q = sequence_of(a.sequences, s);
+            first = q.first + (W - 1) - row0;
+            last = q.first + q.rows - row0;
+        }
+        first = first < 0 ? 0 : first;
+        last = last > kConvRows ? kConvRows : last;
+        const uint32_t mine = first < last ? (uint32_t)(((1ULL << (last - first)) - 1) << first) : 0u;
+        allowed |= (uint32_t)__builtin_amdgcn_readlane(sums_upto((int)mine), 63);
+        const int next = base + 64;
+        if (next >= a.sequences.count || a.sequences.cu[next] - row0 >= rows) break;
+    }
+    if (!active || allowed == 0) return;
     taps.load(a, c0, left);
     h8 x[W];
 #pragma unroll
@@ -112,17 +128,6 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(const ConvArg
         const int row = row0 - W + k;
         x[k] = row >= 0 ? load_halves(a.x + (int64_t)row * a.x_row + c0, left) : h8{};
     }
-    int first = 0, next = 0x7fffffff;  // of the sequence that the row belongs to; `first` passes all rows where it has none
-    auto enter = [&](int row) __attribute__((always_inline)) {
-        while (s + 1 < a.sequences.count && cu[s + 1] <= row) ++s;
-        first = 0x7fffffff;
-        next = s < a.sequences.count ? cu[s + 1] : 0x7fffffff;
-        if (s < 0) return;
-        const Sequence q = sequence_of(a.sequences, s);
-        if (row < q.first + q.rows) first = q.first;
-        else if (next <= row) next = 0x7fffffff;  // behind the last
-    };
-    enter(row0);
     const half_t* from = a.x + (int64_t)row0 * a.x_row + c0;
     half_t* to = a.out + (int64_t)row0 * a.out_row + c0;
 #pragma unroll 4
@@ -130,8 +135,7 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(const ConvArg
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) x[k] = x[k + 1];
         x[W - 1] = load_halves(from + (int64_t)r * a.x_row, left);
-        if (row0 + r >= next) enter(row0 + r);
-        if (row0 + r - (W - 1) >= first) store_halves(to + (int64_t)r * a.out_row, taps.apply(x, a.activation), left);
+        if ((allowed >> r) & 1) store_halves(to + (int64_t)r * a.out_row, taps.apply(x, a.activation), left);
     }
 }
 

@@ -34,7 +34,7 @@ struct ScanArgs {
     Sequences sequences;
     int heads, share, head_dim, states, softplus;  // share: heads of a group
     // set by the launch
-    int segments, head_blocks;
+    int segments, pieces, head_blocks;  // pieces: of a segment, in the first launch
     float* temp;
 };
 
@@ -158,13 +158,31 @@ __device__ __forceinline__ void store_halves(half_t* p, h8 v, int left) {
 __device__ __forceinline__ float silu_fast(float u) {
     return u * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * u));
 }
-// The length of a token's time step.  The logarithm's own function: log(1 + t) from a rounded 1 + t is off by 2^-24 / t.
-__device__ __forceinline__ float time_step(const ScanArgs& a, float dt, float bias) {
+// The length of a token's time step, log(1 + exp(u)) = max(u, 0) + log(1 + t) with t = exp(-|u|).  The logarithm by its series
+// 2 (r + r^3 / 3 + ..), r = t / (2 + t) <= 1/3, whose next term is below 2^-32 of it: the logarithm of a rounded 1 + t would be off by
+// 2^-24 / t, which the states, summed up in fp32, would show.  The exponential's argument is kept in two parts for the same reason.
+__device__ __forceinline__ float time_step(float dt, float bias, int softplus, float dt_min, float dt_max) {
     float u = dt + bias;
-    if (a.softplus) u = fmaxf(u, 0.f) + log1pf(expf(-fabsf(u)));
+    if (softplus) {
+        const float size = -fabsf(u), hi = size * 1.4426950408889634f;
+        const float lo = __builtin_fmaf(size, 1.4426950408889634f, -hi) + size * 1.925963033500e-8f;
+        const float e = __builtin_amdgcn_exp2f(hi), t = hi > -126.f ? __builtin_fmaf(e, lo * 0.6931471805599453f, e) : e;
+        const float sum = 2.0f + t, about = __builtin_amdgcn_rcpf(sum), per = __builtin_fmaf(__builtin_fmaf(-sum, about, 1.0f), about, about);
+        const float r = t * per, q = r * r;
+        float v = 1.0f / 17.0f;
+        v = __builtin_fmaf(v, q, 1.0f / 15.0f);
+        v = __builtin_fmaf(v, q, 1.0f / 13.0f);
+        v = __builtin_fmaf(v, q, 1.0f / 11.0f);
+        v = __builtin_fmaf(v, q, 1.0f / 9.0f);
+        v = __builtin_fmaf(v, q, 1.0f / 7.0f);
+        v = __builtin_fmaf(v, q, 1.0f / 5.0f);
+        v = __builtin_fmaf(v, q, 1.0f / 3.0f);
+        v = __builtin_fmaf(v * q, r, r);
+        u = fmaxf(u, 0.f) + 2.0f * v;
+    }
     // (comparisons, which let a NaN pass)
-    u = u < a.dt_min ? a.dt_min : u;
-    return u > a.dt_max ? a.dt_max : u;
+    u = u < dt_min ? dt_min : u;
+    return u > dt_max ? dt_max : u;
 }
 
 }  // namespace uniql

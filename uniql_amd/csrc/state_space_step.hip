@@ -54,7 +54,8 @@ __global__ __launch_bounds__(kStepThreads) void state_space_step_kernel(const Sc
         const int p = p0 + r * kAtOnce;
         x[r] = p < a.head_dim ? (float)x_from[p] : 0.f;
     }
-    const float step = time_step(a, (float)a.dt[(int64_t)q.first * a.dt_row + head], a.dt_bias ? a.dt_bias[head] : 0.f);
+    const float step = time_step((float)a.dt[(int64_t)q.first * a.dt_row + head], a.dt_bias ? a.dt_bias[head] : 0.f, a.softplus,
+                                 a.dt_min, a.dt_max);
     const float decay = expf(step * a.a[head]), skip = a.d ? a.d[head] : 0.f;
     float y[ROWS];
 #pragma unroll
@@ -101,14 +102,26 @@ static int go(ScanArgs& a, hipStream_t stream) {
     return hipGetLastError() == hipSuccess ? UNIQL_OK : UNIQL_E_LAUNCH;
 }
 
+// A row of `states` by 8 lanes, PARTS vectors of four each: whole lines of 128 bytes a row in each access, no lane without work where the states
+// are a multiple of 32, and three steps to sum a row up.
+template <int PARTS>
+static int by_eight(ScanArgs& a, hipStream_t stream) {
+    return go<8, 4, PARTS, (PARTS > 4 ? 1 : (PARTS > 2 ? 2 : 4))>(a, stream);
+}
+
 int state_space_step_launch(const ScanArgs& args, hipStream_t stream) {
     ScanArgs a = args;
-    const bool whole = a.states % 4 == 0;
-    if (!whole) return go<64, 1, 4, 2>(a, stream);
-    if (a.states <= 32) return go<8, 4, 1, 2>(a, stream);
-    if (a.states <= 64) return go<16, 4, 1, 4>(a, stream);
-    if (a.states <= 128) return go<32, 4, 1, 8>(a, stream);
-    return go<64, 4, 1, 8>(a, stream);
+    if (a.states % 4 != 0) return go<64, 1, 4, 2>(a, stream);
+    switch ((a.states + 31) / 32) {
+        case 1: return by_eight<1>(a, stream);
+        case 2: return by_eight<2>(a, stream);
+        case 3: return by_eight<3>(a, stream);
+        case 4: return by_eight<4>(a, stream);
+        case 5: return by_eight<5>(a, stream);
+        case 6: return by_eight<6>(a, stream);
+        case 7: return by_eight<7>(a, stream);
+        default: return by_eight<8>(a, stream);
+    }
 }
 
 }  // namespace uniql
