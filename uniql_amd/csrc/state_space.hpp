@@ -20,7 +20,8 @@ struct ConvArgs {
     half_t *state_out, *out;
     int64_t x_row, out_row;
     Sequences sequences;
-    int channels, tiles, activation;
+    int channels, activation;
+    int run, tiles;  // set by the launch: rows of a run, and the runs
 };
 
 struct ScanArgs {

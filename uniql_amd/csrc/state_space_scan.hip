@@ -14,6 +14,13 @@
 // the state of the sequence that goes on behind it, and the decay over it.  The second launch puts them together where a segment begins
 // within a sequence.
 //
+// Bound by the path from L2 to the compute units (48 KiB a chunk and head, at some 10 bytes a clock and compute unit, where rows of 20480 bytes
+// share few sets of the first cache: rows 256 bytes longer 495 -> 420 us) and by latency within a chunk, some 5000 clocks: 128 heads of 64, 8
+// groups of 128 states, 16384 tokens 390 to 460 us in two launches (the first one 77), 1.6 TB/s and 0.4 PFLOP/s of matrix instructions; 4096
+// tokens of 256 states 200; 333 tokens 18, six chunks of 2.4 us each behind a launch.
+// Tried and taken out: two heads that share b and c in a workgroup of sixteen waves (128 registers each: operands cannot be asked for ahead, 430
+// to 460 us), one set of four waves for everything with two workgroups a compute unit (530), more segments (530).
+//
 // S, all sums and the decays are fp32, L is summed up in 64 bits (its differences matter, also behind a token that wipes the state).
 // Rounded to fp16 are the weights and S for the outputs, which are fp16 themselves, each relative to the largest
 // of its row, so that no finite value overflows or vanishes; what goes into S is split into two fp16 numbers, 22 bits.  An infinity or
@@ -306,7 +313,11 @@ __global__ __launch_bounds__(64 * scan_waves(N32, THROUGH, LAST), !LAST && N32 <
         // (With a row for each of sixteen neighbouring lanes instead, each lane's piece is an access of its own: 2710 a chunk and head, with
         // all that stands behind waiting, and now 960.)
         const int my_row = lane >> 2, my_part = lane & 3;
-        // (a common address and a lane's 32-bit distance from it, which 16 rows do not pass)
+        // (a common address and a lane's distance from it, 32 bits of it where rows are near each other)
+        auto distance = [&](int rows, int64_t stride, int more) __attribute__((always_inline)) {
+            if constexpr (THROUGH) return rows * stride + more;
+            else return (unsigned)(rows * (int)stride + more);
+        };
         const half_t* c_tile = k0->c + (int64_t)(row + 16 * W) * c_stride + group * k0->c_group;
         half_t* y_tile = k0->y + (int64_t)(row + 16 * W) * y_stride + head * k0->y_head + p0;
         auto from_lane = [&](uint32_t v, int from) __attribute__((always_inline)) { return (uint32_t)__builtin_amdgcn_ds_bpermute(4 * from, (int)v); };
@@ -318,7 +329,7 @@ __global__ __launch_bounds__(64 * scan_waves(N32, THROUGH, LAST), !LAST && N32 <
             // (W's rows may all lie behind the chunk: its last row then)
             const int last_row = rows - 1 - 16 * W;
             const half_t* const from = uniform(c_tile + (last_row < 0 ? last_row * c_stride : 0)) +
-                                       (unsigned)((my_row < last_row ? my_row : (last_row < 0 ? 0 : last_row)) * (int)c_stride + 8 * my_part);
+                                       distance(my_row < last_row ? my_row : (last_row < 0 ? 0 : last_row), c_stride, 8 * my_part);
             if (!THROUGH && states == 32 * N32) {
 #pragma unroll
                 for (int k = 0; k < N32; ++k) c[k] = load_halves(from + 32 * k, 8);
@@ -331,7 +342,7 @@ __global__ __launch_bounds__(64 * scan_waves(N32, THROUGH, LAST), !LAST && N32 <
                     if constexpr (THROUGH) {
                         c[k] = load_halves(from + 32 * k, states - n);
                     } else {
-                        const h8 v = load_halves(from + (n < states ? 32 * k : 0), 8);
+                        const h8 v = load_halves(from + (n < states ? 32 * k : -n0), 8);  // (behind the states: the row's first ones, unused)
                         c[k] = n < states ? v : h8{};
                     }
                 }
@@ -351,7 +362,7 @@ __global__ __launch_bounds__(64 * scan_waves(N32, THROUGH, LAST), !LAST && N32 <
         h4 held[4];
         int held_rows = 0;
         auto store_outputs = [&]() __attribute__((always_inline)) {
-            half_t* const to = uniform(y_tile) + (unsigned)(my_row * (int)y_stride + 4 * my_part);
+            half_t* const to = uniform(y_tile) + distance(my_row, y_stride, 4 * my_part);
             const bool there = 16 * W + my_row < held_rows;
             if (there && head_dim >= 64) {
 #pragma unroll
@@ -764,7 +775,7 @@ __global__ __launch_bounds__(64 * scan_waves(N32, THROUGH, LAST), !LAST && N32 <
         }
     };
 
-    while (true) {
+    while (index < a.sequences.count) {
         const ArgsAgain k = args_again();
         const Sequences all = sequences_again(k);
         Sequence q = sequence_of(all, index);
@@ -788,7 +799,6 @@ __global__ __launch_bounds__(64 * scan_waves(N32, THROUGH, LAST), !LAST && N32 <
         if (budget <= 0) break;
         do ++index;
         while (index < all.count && sequence_of(all, index).rows == 0);
-        if (index >= all.count) break;
     }
 }
 
@@ -842,10 +852,11 @@ int state_space_scan_launch(const ScanArgs& args, hipStream_t stream) {
     a.head_blocks = (a.head_dim + 63) / 64;
     const Shares s = shares_of(a.sequences.rows, a.sequences.count, a.heads * a.head_blocks);
     a.segments = s.segments, a.pieces = s.pieces;
-    // straight to LDS: pieces at multiples of 4 bytes, whole ones of b, 64 rows below 2^31 bytes
+    // straight to LDS: pieces at multiples of 4 bytes, whole ones of b; 64 rows below 2^31 bytes
     const int64_t far = 1LL << 23, strides = a.x_row | a.x_head | a.b_row | a.b_group;
     const uintptr_t bases = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.b);
-    const bool near = a.x_row >= 8 && a.b_row >= a.states && a.x_row <= far && a.b_row <= far;
+    const bool near = a.x_row >= 8 && a.b_row >= a.states && a.c_row >= 0 && a.y_row >= 0 && a.x_row <= far && a.b_row <= far && a.c_row <= far &&
+                      a.y_row <= far;
     const bool through = !(near && (strides & 1) == 0 && (bases & 3) == 0 && a.states % 8 == 0);
     switch (tiles_of(a.states)) {
         case 4: go<2>(a, through, stream); break;

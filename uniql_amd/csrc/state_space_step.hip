@@ -4,7 +4,8 @@
 // Lanes lie along the states, four to a lane, so that rows of S come and go in whole lines; a wave takes 64 / LANES rows of the head at
 // once, and a thread ROWS of them, all on their way before the first is used.  The products with c are summed over the lanes.
 //
-// Bound by HBM: the state is read and written once.
+// Bound by HBM: the state is read and written once.  256 requests of 128 heads of 64 x 128 400 us, 5.4 TB/s; 48 of 54 x 96 67 us where the
+// states come from memory, 54 where the last-level cache holds some.
 #include "state_space.hpp"
 
 namespace uniql {
@@ -103,24 +104,30 @@ static int go(ScanArgs& a, hipStream_t stream) {
 }
 
 // A row of `states` by 8 lanes, PARTS vectors of four each: whole lines of 128 bytes a row in each access, no lane without work where the states
-// are a multiple of 32, and three steps to sum a row up.
+// are a multiple of 32, and three steps to sum a row up.  Eight vectors of a thread on their way at once, fewer where there are few states or
+// few heads (`spread`: one user's 128 heads 5.8 -> 5.4 us).
 template <int PARTS>
-static int by_eight(ScanArgs& a, hipStream_t stream) {
+static int by_eight(ScanArgs& a, bool spread, hipStream_t stream) {
+    if (spread) return go<8, 4, PARTS, 1>(a, stream);
     return go<8, 4, PARTS, (PARTS > 4 ? 1 : (PARTS > 2 ? 2 : 4))>(a, stream);
 }
 
 int state_space_step_launch(const ScanArgs& args, hipStream_t stream) {
     ScanArgs a = args;
     if (a.states % 4 != 0) return go<64, 1, 4, 2>(a, stream);
+    const bool spread = (int64_t)a.sequences.count * a.heads < 2048;
+    // 128 and 256 states fill 32 and 64 lanes, which then read a row in one piece (256 requests of 128 heads 410 -> 400 us)
+    if (a.states == 128 && !spread) return go<32, 4, 1, 8>(a, stream);
+    if (a.states == 256 && !spread) return go<64, 4, 1, 8>(a, stream);
     switch ((a.states + 31) / 32) {
-        case 1: return by_eight<1>(a, stream);
-        case 2: return by_eight<2>(a, stream);
-        case 3: return by_eight<3>(a, stream);
-        case 4: return by_eight<4>(a, stream);
-        case 5: return by_eight<5>(a, stream);
-        case 6: return by_eight<6>(a, stream);
-        case 7: return by_eight<7>(a, stream);
-        default: return by_eight<8>(a, stream);
+        case 1: return by_eight<1>(a, spread, stream);
+        case 2: return by_eight<2>(a, spread, stream);
+        case 3: return by_eight<3>(a, spread, stream);
+        case 4: return by_eight<4>(a, spread, stream);
+        case 5: return by_eight<5>(a, spread, stream);
+        case 6: return by_eight<6>(a, spread, stream);
+        case 7: return by_eight<7>(a, spread, stream);
+        default: return by_eight<8>(a, spread, stream);
     }
 }
 
