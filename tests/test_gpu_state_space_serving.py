@@ -265,6 +265,23 @@ def test_scan_refusals(gpu):
     assert f(x[:0], dt[:0], a, b[:0], c[:0], state=state, cu=ints([0, 0], gpu)).shape == (0, 4, 8)
 
 
+def test_outputs_in_the_inputs(gpu):
+    from uniql_amd import ops
+    memory = torch.zeros(4096, dtype=torch.int32, device=gpu)
+    halves, floats = memory.view(torch.float16), memory.view(torch.float32)
+    small = memory[:3].copy_(ints([0, 2, 6], gpu))
+    h = lambda *s: torch.zeros(*s, dtype=torch.float16, device=gpu)
+    x, w, b = h(6, 16), h(16, 4), h(6, 1, 8)
+    for kw in (dict(cu=small), dict(cu=ints([0, 2, 6], gpu), places=small[:2]), dict(cu=ints([0, 2, 6], gpu), starts=small[:2])):
+        refuses("share memory", ops.causal_conv, x, w, state=halves[:96].view(2, 3, 16), **kw)
+        refuses("share memory", ops.causal_conv, x, w, state=h(2, 3, 16), out=halves[:96].view(6, 16), **kw)
+        refuses("share memory", ops.state_space_scan, x.view(6, 2, 8), h(6, 2), torch.zeros(2, device=gpu), b, b, state=floats[:256].view(2, 2, 8, 8), **kw)
+        refuses("share memory", ops.state_space_scan, x.view(6, 2, 8), h(6, 2), torch.zeros(2, device=gpu), b, b, state=torch.zeros(2, 2, 8, 8, device=gpu),
+                out=halves[:96].view(6, 2, 8), **kw)
+    refuses("share memory", ops.causal_conv, x, halves[:64].view(16, 4), cu=ints([0, 6], gpu), out=halves[:96].view(6, 16))
+    refuses("share memory", ops.state_space_scan, x.view(6, 2, 8), h(6, 2), floats[:2], b, b, state=floats[:128].view(1, 2, 8, 8), cu=ints([0, 6], gpu))
+
+
 def test_norm_refusals(gpu):
     from uniql_amd import ops
     x = torch.zeros(6, 16, dtype=torch.float16, device=gpu)

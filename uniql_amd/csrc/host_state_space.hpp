@@ -50,6 +50,11 @@ Tensor rows_output(const std::optional<Tensor>& out, const Tensor& like) {
     return *out;
 }
 
+// Outputs and new states are written while others read; neither may lie in what is read.
+void require_apart(const Tensor& out, const char* name, const std::optional<Tensor>& other, const char* other_name) {
+    if (other && ranges_meet(out, *other)) fail(std::string(name) + " must not be " + other_name + " or share memory with it");
+}
+
 // The sequences of a call and the states that they read and replace: `state` and `state_out` are [places, ...] with `shape` behind.
 struct States {
     uniql_sequences sequences;
@@ -105,15 +110,12 @@ States states_of(const std::optional<Tensor>& state, const std::optional<Tensor>
         if (starts->size(0) != count) fail("starts must have one entry per sequence");
         s.sequences.starts = starts->data_ptr<int>();
     }
+    if (s.to)
+        for (const auto* t : {&cu, &places, &starts}) require_apart(state_out ? *state_out : *state, "state_out", *t, "cu, places or starts");
     s.sequences.count = (int)count;
     s.sequences.pool = (int)pool;
     return s;
 }
-// Outputs and new states are written while others read; neither may lie in what is read.
-void require_apart(const Tensor& out, const char* name, const std::optional<Tensor>& other, const char* other_name) {
-    if (other && ranges_meet(out, *other)) fail(std::string(name) + " must not be " + other_name + " or share memory with it");
-}
-
 Tensor causal_conv(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias, const std::optional<Tensor>& state,
                    const std::optional<Tensor>& cu, const std::optional<Tensor>& places, const std::optional<Tensor>& starts,
                    const std::optional<Tensor>& state_out, bool activation, const std::optional<Tensor>& out_in, uintptr_t stream) {
@@ -135,8 +137,14 @@ Tensor causal_conv(const Tensor& x, const Tensor& weight, const std::optional<Te
     if (out_in) {
         if (share_memory(as_heads(out), as_heads(x))) fail("out must not be x or share memory with it");
         for (const auto* t : {&state, &state_out}) require_apart(out, "out", *t, "a state");
+        require_apart(out, "out", weight, "weight");
+        for (const auto* t : {&bias, &cu, &places, &starts}) require_apart(out, "out", *t, "an input");
     }
-    if (s.to) require_apart(state_out ? *state_out : *state, "state_out", x, "x");
+    if (s.to) {
+        const Tensor& to = state_out ? *state_out : *state;
+        for (const Tensor* t : {&x, &weight}) require_apart(to, "state_out", *t, "an input");
+        require_apart(to, "state_out", bias, "bias");
+    }
     check(p_conv(x.data_ptr(), x.stride(0), weight.data_ptr(), bias ? bias->data_ptr() : nullptr, s.from, s.to, &s.sequences, out.data_ptr(),
                  out.stride(0), (int)rows, (int)channels, (int)width, activation, reinterpret_cast<void*>(stream)),
           "uniql_causal_conv");
@@ -172,9 +180,14 @@ Tensor state_space_scan(const Tensor& x, const Tensor& dt, const Tensor& a, cons
         if (share_memory(out, x) || share_memory(out, b) || share_memory(out, c) || share_memory(out, as_heads(dt)))
             fail("out must not be x, dt, b or c or share memory with them");
         for (const auto* t : {&state, &state_out}) require_apart(out, "out", *t, "a state");
+        require_apart(out, "out", a, "a");
+        for (const auto* t : {&d, &dt_bias, &cu, &places, &starts}) require_apart(out, "out", *t, "an input");
     }
-    if (s.to)
-        for (const Tensor* t : {&x, &dt, &b, &c}) require_apart(state_out ? *state_out : *state, "state_out", *t, "an input");
+    if (s.to) {
+        const Tensor& to = state_out ? *state_out : *state;
+        for (const Tensor* t : {&x, &dt, &b, &c, &a}) require_apart(to, "state_out", *t, "an input");
+        for (const auto* t : {&d, &dt_bias}) require_apart(to, "state_out", *t, "an input");
+    }
     size_t need = 0;
     if (cu)
         check(p_scan_workspace((int)rows, s.sequences.count, (int)heads, (int)groups, (int)head_dim, (int)states, &need),
