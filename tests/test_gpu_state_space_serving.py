@@ -182,6 +182,30 @@ def test_rows_far_apart(gpu):
         del buf, far, x, b, c
 
 
+def test_rows_that_overlap(gpu):
+    """x as windows of one sequence of numbers, whose last one is an infinity: it belongs to the last row alone"""
+    from uniql_amd import ops
+    for rows in (5, 70):
+        pr = Problem([rows], 1, 1, 24, 16, seed=6, starts=[0])
+        numbers = torch.randn(8 * (rows - 1) + 24, generator=torch.Generator().manual_seed(6)).half()
+        windows = lambda t: t.as_strided((rows, 1, 24), (8, 24, 1))
+        finite = numbers.clone()
+        finite[-1] = 1
+        numbers[-1] = float("inf")
+        on = lambda t: on_gpu(t, gpu)
+        got = []
+        for t in (finite, numbers):
+            state = torch.zeros(1, 1, 24, 16, device=gpu)
+            got.append((ops.state_space_scan(windows(t.to(gpu)), on(pr.dt), pr.a.to(gpu), on(pr.b), on(pr.c), dt_bias=pr.dt_bias.to(gpu), state=state,
+                                             cu=ints([0, rows], gpu)), state))
+        want, tol, S, S_tol = R.scan(windows(finite).contiguous(), pr.dt, pr.a, pr.b, pr.c, None, pr.dt_bias, torch.zeros(1, 24, 16))
+        within(got[0][0], want, tol), within(got[0][1][0], S, S_tol)
+        # all but the last channel of the last row, and of the state
+        within(got[1][0][:-1], want[:-1], tol[:-1]), within(got[1][0][-1, :, :-1], want[-1, :, :-1], tol[-1, :, :-1])
+        within(got[1][1][0, :, :-1], S[:, :-1], S_tol[:, :-1])
+        assert not got[1][1][0, 0, -1].isfinite().any() and not got[1][0][-1, 0, -1].isfinite()
+
+
 def test_places_far_apart(gpu):
     """a pool of more than 2^31 numbers"""
     from uniql_amd import ops
