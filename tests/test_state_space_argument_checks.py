@@ -118,7 +118,8 @@ for rows, count, (heads, p, n) in itertools.product((1, 2, 63, 64, 65, 333, 4096
     need = Z(0)
     assert lib.uniql_state_space_scan_workspace(rows, count, heads, 1, p, n, ctypes.byref(need)) == 0
     code, launches = call(rows, count, heads, p, n, need.value)
-    assert code == 0 and launches == (2 if need.value else 1), (rows, count, heads, code, launches)
+    singles = count >= 4 and count * heads < 1 << 20   # single tokens among several sequences have a launch of their own
+    assert code == 0 and launches == (2 if need.value else 1) + singles, (rows, count, heads, code, launches)
     if need.value:
         assert call(rows, count, heads, p, n, need.value - 1) == (-4, 0)
     if rows <= 4096:
@@ -129,7 +130,7 @@ assert hip.fake_refused() == 0 and hip.fake_attributes() == 0
 
 
 def test_scratch_memory_is_asked_for_where_a_launch_needs_it(tmp_path):
-    """two launches where there is scratch memory, one where there is none, and no attribute set (calls are recorded into graphs)"""
+    """two launches where there is scratch memory, one where there is none, one more for single tokens, and no attribute set (calls are recorded into graphs)"""
     if shutil.which("g++") is None or not os.path.exists(LIB_PATH):
         pytest.skip("g++ and the built library are needed")
     recorder = str(tmp_path / "fake_hip.so")

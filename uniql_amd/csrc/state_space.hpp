@@ -9,7 +9,9 @@ namespace uniql {
 struct Sequences {
     const int32_t *cu, *starts, *places;  // any may be null: a row each; all continued; place s
     int count, pool, rows;
+    int only;  // 0: sequences of any length have rows; kSingle: those of one row; kLonger: the others
 };
+constexpr int kSingle = 1, kLonger = 2;
 struct Sequence {
     int first, rows, place;
     bool continued;
@@ -61,6 +63,7 @@ __device__ __forceinline__ Sequence sequence_of(const Sequences& all, int s) {
     }
     q.place = all.places ? all.places[s] : s;
     if ((unsigned)q.place >= (unsigned)all.pool) q.rows = 0;
+    if (all.only && (q.rows == 1) != (all.only == kSingle)) q.rows = 0;
     q.continued = !all.starts || all.starts[s] > 0;
     return q;
 }

@@ -174,7 +174,8 @@ __device__ __forceinline__ ArgsAgain args_again() {
     return p;
 }
 __device__ __forceinline__ Sequences sequences_again(ArgsAgain p) {
-    return {p->sequences.cu, p->sequences.starts, p->sequences.places, p->sequences.count, p->sequences.pool, p->sequences.rows};
+    return {p->sequences.cu, p->sequences.starts, p->sequences.places, p->sequences.count, p->sequences.pool, p->sequences.rows,
+            p->sequences.only};
 }
 
 // Who asks for the tiles.  For outputs over up to 128 states waves of their own, one, or four where the values pass through their registers: asking
