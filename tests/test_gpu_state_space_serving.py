@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests import state_space_reference as R
-from tests.test_gpu_state_space import Problem, ints, on_gpu, run_scan, within
+from tests.test_gpu_state_space import Problem, check_scan, ints, on_gpu, run_scan, within
 
 pytestmark = pytest.mark.gpu
 
@@ -111,6 +111,22 @@ def test_without_states(gpu):
     near(m(h, cu=ints([0, 40, 40, 90], gpu)), in_64_bits(m, h, [40, 0, 50], torch.zeros(3, 3, CHANNELS), torch.zeros(3, HEADS, P, N), [0] * 3)[0])
     with pytest.raises(RuntimeError, match="state"):
         m(h)
+
+
+@pytest.mark.parametrize("p,n", [(8, 16), (12, 33), (100, 96), (64, 128), (54, 256), (1, 1)])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_single_tokens_among_prompts(gpu, p, n, in_place):
+    """each length next to each other, left out, beginning and continued; fewer sequences than four; offsets in front and rows behind"""
+    for lengths in ([1, 5, 1, 0, 1, 130, 1, 64, 1], [1, 1, 1, 1, 1, 1], [1, 2, 1], [3, 0, 2, 65], [1], [0, 0, 0, 1]):
+        pr = Problem(lengths, 4, 2, p, n, seed=11, first=2, behind=3)
+        if len(lengths) > 4:
+            pr.places[2] = -1
+            pr.places[5] = -1
+        check_scan(pr, gpu, in_place=in_place)
+
+
+def test_more_heads_and_sequences_than_steps_take(gpu):
+    check_scan(Problem([1] * 36 + [3, 1], 1 << 15, 1, 1, 1, seed=12), gpu)
 
 
 @pytest.mark.parametrize("single", [True, False])

@@ -1,5 +1,5 @@
-// One more token of every request, or of those of a batch that have one, through a state-space layer: S' = exp(s a) S + s x b^T, y = S' c + d x, with the time step
-// s = softplus(dt + bias), for each head's matrix S [head_dim][states] of fp32.
+// One more token of every request, or of those of a batch that have one, through a state-space layer: S' = exp(s a) S + s x b^T,
+// y = S' c + d x, with the time step s = softplus(dt + bias), for each head's matrix S [head_dim][states] of fp32.
 //
 // Lanes lie along the states, four to a lane, so that rows of S come and go in whole lines; a wave takes 64 / LANES rows of the head at
 // once, and a thread ROWS of them, all on their way before the first is used.  The products with c are summed over the lanes.
