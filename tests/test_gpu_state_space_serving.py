@@ -105,6 +105,31 @@ def test_between_the_projections(gpu):
     within(pieces.ssm, whole.ssm.cpu().double(), 2.0 ** -18 * whole.ssm.abs().max().cpu().double().expand(whole.ssm.shape))
 
 
+def test_next_to_a_cache(gpu):
+    """offsets and starts from the pages; a request that they refuse keeps its states and is asked for again, one that ends makes room"""
+    from uniql_amd.quantize.quant_kv_cache import KVPages
+    from uniql_amd.state_space import StateSpaceStates
+    m = mixer(gpu)
+    states, pages = StateSpaceStates.like(m, 3), KVPages(8, 16, 3, 8, device=gpu)
+    conv, ssm = states.conv.clone(), states.ssm.clone()
+    for step, (new, refused) in enumerate((([40, 17, 0], [0, 0, 0]), ([1, 64, 2], [0, 1, 1]), ([-1, 60, 20], [0, 0, 0]), ([1, 1, 1], [0, 0, 0]))):
+        starts = pages.lengths.clone()
+        s = pages.assign(ints(new, gpu), 128)
+        assert s.refused.tolist() == refused
+        places = torch.where(s.refused > 0, -1, torch.arange(3, dtype=torch.int32, device=gpu))
+        h = projected(128, gpu, seed=20 + step)
+        got = m(h, states, cu=s.cu, places=places, starts=starts)
+        cu, had = s.cu.tolist(), starts.tolist()
+        for r in range(3):
+            if refused[r] or new[r] <= 0:
+                continue
+            want, c, S = in_64_bits(m, h[cu[r]:cu[r + 1]], [new[r]], conv[r:r + 1], ssm[r:r + 1], [had[r]])
+            near(got[cu[r]:cu[r + 1]], want)
+            conv, ssm = conv.cpu().double(), ssm.cpu().double()
+            conv[r], ssm[r] = c[0], S[0]
+        near(states.ssm, ssm.cpu().double())
+
+
 def test_without_states(gpu):
     m = mixer(gpu)
     h = projected(90, gpu)

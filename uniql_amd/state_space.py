@@ -9,8 +9,10 @@ modeling/mamba/mamba2_qblocks.py.)
     h = mixer(h, states, cu=step.cu, starts=lengths_before)      # prompts, pieces of prompts and single tokens in one batch
     x = block.out_proj(h, residual=x)
 
-With attention layers in the model, `cu` is KVStep.cu, and `starts` what KVPages.lengths held before the step; requests that KVPages refused
-are left out with places = torch.where(step.refused > 0, -1, torch.arange(max_requests)).  All of it runs from what is on the device and can be
+With attention layers in the model, `cu` is KVStep.cu, and `starts` a copy of what KVPages.lengths held before the step.  Requests that KVPages
+refused keep their rows there, and are left out with
+    places = torch.where(step.refused > 0, -1, torch.arange(max_requests, dtype=torch.int32, device="cuda"))
+All of it runs from what is on the device and can be
 recorded into a graph.  Nothing is recorded for autograd."""
 from __future__ import annotations
 
