@@ -74,7 +74,8 @@ __device__ __forceinline__ bool finite(half_t v) { return __builtin_fabsf16(v) <
 
 // What is known of a chunk's rows before its products: the logarithms L (base 2) of the decay up to each row, rounded to floats; their
 // rests r as factors, 2^r, and the time steps with the same taken off, s 2^-r: exp2(L_i - L_j) of the rounded ones times both is off by
-// the difference's own rounding alone; what a row adds to the state (its time step, faded), and the decays.
+// the roundings of the difference (2^-24 of it) and of the three exponentials alone; what a row adds to the state (its time step, faded), and
+// the decays.
 struct RowValues {
     float log[kChunk], rest[kChunk], step[kChunk], into[kChunk], decay[kChunk];
     float unit, per_unit;  // of `into`, a power of two, and its inverse
@@ -557,9 +558,12 @@ __global__ __launch_bounds__(64 * scan_waves(N32, THROUGH, LAST), !LAST && N32 <
         // One wave works out a chunk's row values, a row a lane.
         auto row_values = [&](half_t dt, int rows, RowValues& to) __attribute__((always_inline)) {
             const float step = lane < rows ? time_step((float)dt, bias, softplus, dt_min, dt_max) : 0.f;
-            const double log = sums_upto(lane < rows ? (double)step * (double)rate * 1.4426950408889634 : 0.0);
+            // (A row that fades by 2^-300 leaves nothing of any fp32 state, as one that fades by more: L of a chunk stays below 2^15, and its rest small.)
+            double row_log = (double)step * (double)rate * 1.4426950408889634;
+            row_log = row_log < -300.0 ? -300.0 : row_log;
+            const double log = sums_upto(lane < rows ? row_log : 0.0);
             const double all = __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(log), 63), __builtin_amdgcn_readlane(__double2loint(log), 63));
-            const float hi = (float)log, rest = (float)(log - (double)hi) * 0.6931471805599453f;
+            const float hi = (float)log, rest = (float)(log - (double)hi);
             const float into = lane < rows ? __builtin_amdgcn_exp2f((float)(all - log)) * step : 0.f;
             float most = max_of_sixteenths(into);
             most = fmaxf(most, dpp_from<0x140>(most));
@@ -568,10 +572,11 @@ __global__ __launch_bounds__(64 * scan_waves(N32, THROUGH, LAST), !LAST && N32 <
             most = fmaxf(most, dpp_from<0xB1>(most));
             const int e = clamp_to(exponent_of(most), -60, 60);
             to.log[lane] = hi;
-            to.rest[lane] = 1.0f + rest;
-            to.step[lane] = step * (1.0f - rest);
+            const float factor = __builtin_amdgcn_exp2f(rest);
+            to.rest[lane] = factor;
+            to.step[lane] = step * __builtin_amdgcn_exp2f(-rest);
             to.into[lane] = into * power_of_two(-1 - e);
-            to.decay[lane] = __builtin_amdgcn_exp2f(hi) * (1.0f + rest);
+            to.decay[lane] = __builtin_amdgcn_exp2f(hi) * factor;
             if (lane == 0) to.unit = power_of_two(e + 1), to.per_unit = power_of_two(-1 - e), to.all = all;
         };
         // Lane: channel 16 wave + low, states 16 t + 4 high + r, in units of `unit_s` (a power of two of the channel's own).
