@@ -7,6 +7,7 @@
 //
 // Bound by HBM: 16384 rows of 10240 channels 136 to 147 us, 4.6 to 4.9 TB/s, what a copy reaches.  48 single tokens 4.2 us: offsets, then state and
 // rows, then the store, each a round trip.
+#include "row_mask.hpp"
 #include "state_space.hpp"
 
 namespace uniql {
@@ -59,6 +60,19 @@ __device__ __forceinline__ int last_not_behind(const int32_t* cu, int count, int
     return below;
 }
 
+// The rows of any lane's mask, in each lane.
+__device__ __forceinline__ uint32_t rows_of_all(uint32_t mask) {
+    int v = (int)mask;
+    auto join = [&](int other) __attribute__((always_inline)) { v = (int)rows_of_either((uint32_t)v, (uint32_t)other); };
+    join(dpp_or_zero<0x111, 0xf>(v));  // one, two, four, eight lanes below, within sixteen
+    join(dpp_or_zero<0x112, 0xf>(v));
+    join(dpp_or_zero<0x114, 0xf>(v));
+    join(dpp_or_zero<0x118, 0xf>(v));
+    join(dpp_or_zero<0x142, 0xa>(v));  // the last of the sixteen below, for the second and fourth sixteen
+    join(dpp_or_zero<0x143, 0xc>(v));  // lane 31, for the upper half
+    return (uint32_t)__builtin_amdgcn_readlane(v, 63);
+}
+
 template <int W>
 __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(const ConvArgs a) {
     const int c0 = (blockIdx.y * kConvThreads + threadIdx.x) * 8, left = a.channels - c0;
@@ -103,23 +117,19 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(const ConvArg
         return;
     }
     const int row0 = blockIdx.x * a.run, rows = a.sequences.rows - row0 < a.run ? a.sequences.rows - row0 : a.run;
-    // Rows that have W - 1 others of their sequence in front of them, a bit each: 64 sequences at a time, which share no bits.
+    // Rows that have W - 1 others of their sequence in front of them, a bit each: 64 sequences at a time.
     const int lane = threadIdx.x & 63;
     uint32_t allowed = 0;
     for (int base = __builtin_amdgcn_readfirstlane(last_not_behind(a.sequences.cu, a.sequences.count, row0)); base < a.sequences.count; base += 64) {
         const int s = base + lane;
-        int first = rows, last = rows;
+        uint32_t mine = 0;
         if (s >= 0 && s < a.sequences.count) {
             const Sequence q = sequence_of(a.sequences, s);
-            first = q.first + (W - 1) - row0;
-            last = q.first + q.rows - row0;
+            mine = rows_between(q.first + (W - 1) - row0, q.first + q.rows - row0, rows);
         }
-        first = first < 0 ? 0 : first;
-        last = last > rows ? rows : last;
-        const uint32_t mine = first < last ? (uint32_t)(((1ULL << (last - first)) - 1) << first) : 0u;
-        allowed |= (uint32_t)__builtin_amdgcn_readlane(sums_upto((int)mine), 63);
+        allowed = rows_of_either(allowed, rows_of_all(mine));
         const int next = base + 64;
-        if (next >= a.sequences.count || a.sequences.cu[next] - row0 >= rows) break;
+        if (next >= a.sequences.count || a.sequences.cu[next] >= row0 + rows) break;
     }
     if (!active || allowed == 0) return;
     taps.load(a, c0, left);
