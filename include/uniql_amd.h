@@ -483,7 +483,9 @@ int uniql_prompt_attention(const void* q, int64_t q_row, int64_t q_head, const v
  * this library's own.  fp16 rows, states of the convolution in fp16, of the scan in fp32.
  *
  * Which rows belong to which sequence (request), and where its states lie in a pool of `pool` places:
- *   cu       device, int32 [count + 1]: the rows cu[s] .. cu[s + 1] are sequence s's (ascending); NULL: a row each (count == rows)
+ *   cu       device, int32 [count + 1]: the rows cu[s] .. cu[s + 1] are sequence s's (ascending); NULL: a row each (count == rows).
+ *            Offsets outside the rows count as the nearest inside.  Where offsets fall, the call's rows and named places hold anything
+ *            afterwards; nothing else is written
  *   starts   device, int32 [count]: tokens that a sequence has had before; where it is 0 (or less) the sequence begins with an empty state, whatever
  *            its place holds; NULL: all are continued
  *   places   device, int32 [count]: a sequence's place in the pool; NULL: place s.  Sequences whose place is outside the pool (-1) are

@@ -82,7 +82,8 @@ struct RowValues {
     double all;            // the last row's logarithm
 };
 
-// Chunks in all sequences.
+// Chunks in all sequences.  Rows that belong to one sequence at most make no more than a chunk each 64 and one a sequence: more come of offsets
+// that fall and rise again, whose walk would take as long as they like.  Such a call does nothing.
 __device__ __forceinline__ int count_chunks(const Sequences& all) {
     const int lane = threadIdx.x & 63;
     int total = 0;
@@ -90,7 +91,7 @@ __device__ __forceinline__ int count_chunks(const Sequences& all) {
         const int s = base + lane;
         const int mine = s < all.count ? (sequence_of(all, s).rows + kChunk - 1) / kChunk : 0;
         total += __builtin_amdgcn_readlane(sums_upto(mine), 63);
-        if (total > 0x3fffffff) return 0;  // (offsets that fall and rise again)
+        if (total > all.rows / kChunk + all.count) return 0;
     }
     return total;
 }
