@@ -859,13 +859,14 @@ int state_space_scan_launch(const ScanArgs& args, hipStream_t stream) {
     a.head_blocks = (a.head_dim + 63) / 64;
     const Shares s = shares_of(a.sequences.rows, a.sequences.count, a.heads * a.head_blocks);
     a.segments = s.segments, a.pieces = s.pieces;
-    // straight to LDS: pieces at multiples of 4 bytes, whole ones of b; rows that do not overlap (what lies behind a chunk's rows then lies
-    // behind the buffer), 64 of them below 2^31 bytes
+    // straight to LDS: pieces at multiples of 4 bytes, whole ones of b and whole words of x (a buffer that ends within a word: its last value
+    // would be lost, or the next one read); rows that do not overlap (what lies behind a chunk's rows then lies behind the buffer), 64 of them below
+    // 2^31 bytes
     const int64_t far = 1LL << 23, strides = a.x_row | a.x_head | a.b_row | a.b_group;
     const uintptr_t bases = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.b);
     const bool near = a.x_row >= (a.head_dim < 64 ? a.head_dim : 64) && a.b_row >= a.states && a.c_row >= 0 && a.y_row >= 0 && a.x_row <= far && a.b_row <= far && a.c_row <= far &&
                       a.y_row <= far;
-    const bool through = !(near && (strides & 1) == 0 && (bases & 3) == 0 && a.states % 8 == 0);
+    const bool through = !(near && (strides & 1) == 0 && (bases & 3) == 0 && a.head_dim % 2 == 0 && a.states % 8 == 0);
     switch (tiles_of(a.states)) {
         case 4: go<2>(a, through, stream); break;
         case 6: go<3>(a, through, stream); break;
