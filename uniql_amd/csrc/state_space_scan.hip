@@ -731,7 +731,8 @@ __global__ __launch_bounds__(64 * scan_waves(N32, THROUGH, LAST), !LAST && N32 <
                         into_lo[k][4 * h + r] = lo[0], into_lo[k][4 * h + r + 1] = lo[1];
                     }
                 }
-            if (__any(!all_zero(zero))) {
+            const bool infinities = __any(!all_zero(zero));
+            if (infinities) {
                 asm volatile("");  // infinities have no rest
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
@@ -752,6 +753,15 @@ __global__ __launch_bounds__(64 * scan_waves(N32, THROUGH, LAST), !LAST && N32 <
 #pragma unroll
                 for (int t = t0; t < t0 + 4 && t < kTiles; ++t) S[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand[step % (kAhead + 1)][t - t0], into_lo[k], S[t], 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
+            }
+            if (infinities && states < 32 * N32) {
+                // b is zero behind the states, and zero times an infinity would stay there for the outputs' products
+                int n0 = 4 * high;
+                asm volatile("" : "+v"(n0));
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[t][r] = 16 * t + n0 + r < states ? S[t][r] : 0.f;
             }
             if (next_rows > 0) {
                 if constexpr (LAST) leave_copy(s_next, unit);
