@@ -571,7 +571,7 @@ __global__ __launch_bounds__(64 * scan_waves(N32, THROUGH, LAST), !LAST && N32 <
             most = fmaxf(most, dpp_from<0x141>(most));
             most = fmaxf(most, dpp_from<0x4E>(most));
             most = fmaxf(most, dpp_from<0xB1>(most));
-            const int e = clamp_to(exponent_of(most), -60, 60);
+            const int e = clamp_to(exponent_of(most), -95, 100);
             to.log[lane] = hi;
             const float factor = __builtin_amdgcn_exp2f(rest);
             to.rest[lane] = factor;
@@ -671,6 +671,31 @@ __global__ __launch_bounds__(64 * scan_waves(N32, THROUGH, LAST), !LAST && N32 <
                 }
             }
         }
+        // The largest finite size among a lane's channel's states, in their units.
+        auto largest_state = [&]() __attribute__((always_inline)) {
+            float top = 0.f;
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(S[t][r]) < INFINITY ? fabsf(S[t][r]) : 0.f);
+            return max_of_sixteenths(top);
+        };
+        // What the inverse of a chunk's units stays below as long as no finite state can pass fp32: one that the walk begins with, or one that it adds
+        // up to (64 rows a chunk, time steps up to the longest, values of x and b below 2^16, 2^21 chunks).
+        float room;
+        {
+            int most = exponent_of(fmaxf(fminf(65505.f + fabsf(bias), dt_max), dt_min)) + 61;
+            if (offset > 0 || (k0->state && q.continued)) {
+                float top = largest_state();
+                top = fmaxf(top, dpp_from<0x140>(top));
+                top = fmaxf(top, dpp_from<0x141>(top));
+                top = fmaxf(top, dpp_from<0x4E>(top));
+                top = fmaxf(top, dpp_from<0xB1>(top));
+                const int e = uniform(exponent_of(top));
+                most = e > most ? e : most;
+            }
+            room = power_of_two(125 - clamp_to(most, 0, 125));
+        }
         double walk_log = 0.0;
         Tiles tiles = tiles_at(row);
         if constexpr (kLoading == 0) fetch(tiles, last - row < kChunk ? last - row : kChunk, (lds_bytes)b_even, (lds_bytes)x_even);
@@ -707,13 +732,26 @@ __global__ __launch_bounds__(64 * scan_waves(N32, THROUGH, LAST), !LAST && N32 <
             // (exact: no x becomes larger than 2^15, and smaller only where the largest is 2^15 and more)
             const int up = 14 - e < 15 ? 14 - e : 15;
             const half_t by = (half_t)power_of_two(up);
-            const float unit_x = power_of_two(e - 14) * now.unit, per_unit_x = power_of_two(14 - e) * now.per_unit;
+            float unit_x = power_of_two(e - 14) * now.unit, per_unit_x = power_of_two(14 - e) * now.per_unit;
 #pragma unroll
             for (int k = 0; k < 2; ++k) x[k] *= by;
-            if (__any(14 - e > 15)) {
+            if (__any(14 - e > 15 || per_unit_x >= room)) {
                 asm volatile("");
 #pragma unroll
                 for (int k = 0; k < 2; ++k) x[k] *= (half_t)power_of_two(14 - e - up);
+                if (__any(per_unit_x >= room)) {
+                    // The state might pass fp32 in units of what the chunk adds, which is little: larger ones where it would, in which that little keeps the
+                    // digits that matter beside such a state.
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) S[t] *= unit_s;
+                    unit_s = 1.f;
+                    const int more = clamp_to(exponent_of(largest_state()) + exponent_of(per_unit_x) - 120, 0, 126);
+                    unit_x *= power_of_two(more), per_unit_x *= power_of_two(-more);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) x[k][j] = (half_t)((float)x[k][j] * power_of_two(-more));
+                }
             }
             float one = 1.f;
             asm volatile("" : "+s"(one));  // (v - one hi is one instruction for an fp16 hi, v - hi two)
