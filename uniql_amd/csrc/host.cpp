@@ -353,6 +353,7 @@ PYBIND11_MODULE(_host, module) {
     module.def("causal_conv", &causal_conv);
     module.def("state_space_scan", &state_space_scan);
     module.def("gated_group_norm", &gated_group_norm);
+    module.def("check_state_space_layer", &check_state_space_layer);
     module.def("share_memory", &share_memory);
     module.def("overlaps_itself", &overlaps_itself);
     py::class_<KvPool>(module, "KvPool")

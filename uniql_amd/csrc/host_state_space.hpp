@@ -151,6 +151,17 @@ Tensor causal_conv(const Tensor& x, const Tensor& weight, const std::optional<Te
     return out;
 }
 
+void require_limits(double dt_min, double dt_max) {
+    if (!(dt_min >= 0.0 && dt_min <= dt_max)) fail("dt_limit must be two numbers from 0 on, the smaller one first");
+}
+// The weight of the norm and its groups.
+void require_norm(const Tensor& weight, int64_t channels, int64_t groups, double eps, const Tensor& like) {
+    require_plain(weight, "weight", at::kHalf, 1, like);
+    if (weight.size(0) != channels) fail("weight must have one entry per channel");
+    if (groups < 1 || channels % groups) fail("groups must divide the channels");
+    if (!(eps >= 0.0)) fail("eps must not be negative");
+}
+
 Tensor state_space_scan(const Tensor& x, const Tensor& dt, const Tensor& a, const Tensor& b, const Tensor& c, const std::optional<Tensor>& d,
                         const std::optional<Tensor>& dt_bias, bool softplus, double dt_min, double dt_max, const std::optional<Tensor>& state,
                         const std::optional<Tensor>& cu, const std::optional<Tensor>& places, const std::optional<Tensor>& starts,
@@ -170,7 +181,7 @@ Tensor state_space_scan(const Tensor& x, const Tensor& dt, const Tensor& a, cons
     if (b.size(0) != rows || c.sizes() != b.sizes()) fail("b and c must have x's rows, and the same groups and states");
     if (heads % groups) fail("x's heads must be a multiple of b's groups");
     if (head_dim > 128 || states > 256) fail("heads must be 1 to 128 wide, with 1 to 256 states");
-    if (!(dt_min >= 0.0 && dt_min <= dt_max)) fail("dt_limit must be two numbers from 0 on, the smaller one first");
+    require_limits(dt_min, dt_max);
     const float* const rate = per_head(a, "a", heads, x);
     const float *const skip = per_head(d, "d", heads, x), *const bias = per_head(dt_bias, "dt_bias", heads, x);
     const c10::DeviceGuard guard(x.device());
@@ -212,10 +223,7 @@ Tensor gated_group_norm(const Tensor& x, const Tensor& z, const Tensor& weight, 
     require_rows(z, "z");
     const int64_t rows = x.size(0), channels = x.size(1);
     if (z.sizes() != x.sizes()) fail("z must have x's shape");
-    require_plain(weight, "weight", at::kHalf, 1, x);
-    if (weight.size(0) != channels) fail("weight must have one entry per channel");
-    if (groups < 1 || channels % groups) fail("groups must divide the channels");
-    if (!(eps >= 0.0)) fail("eps must not be negative");
+    require_norm(weight, channels, groups, eps, x);
     const c10::DeviceGuard guard(x.device());
     Tensor out = rows_output(out_in, x);
     if (out_in) {
@@ -228,4 +236,26 @@ Tensor gated_group_norm(const Tensor& x, const Tensor& z, const Tensor& weight, 
                  (int)channels, (int)groups, (float)eps, reinterpret_cast<void*>(stream)),
           "uniql_gated_group_norm");
     return out;
+}
+
+// What the scan and the norm of a layer would refuse of its parameters and states, asked before the convolution replaces its own states: all three
+// are one step of the requests, or none is.
+void check_state_space_layer(const Tensor& rows, const Tensor& a, const std::optional<Tensor>& d, const std::optional<Tensor>& dt_bias, double dt_min,
+                             double dt_max, const Tensor& state, const std::optional<Tensor>& cu, const std::optional<Tensor>& places,
+                             const std::optional<Tensor>& starts, const Tensor& norm_weight, int64_t norm_groups, double eps, int64_t heads,
+                             int64_t head_dim, int64_t groups, int64_t states) {
+    require_gpu(rows, "projected");
+    require_rows(rows, "projected");
+    per_head(a, "a", heads, rows);
+    per_head(d, "d", heads, rows);
+    per_head(dt_bias, "dt_bias", heads, rows);
+    require_limits(dt_min, dt_max);
+    const States s = states_of(state, std::nullopt, cu, places, starts, at::kFloat, {heads, head_dim, states}, rows.size(0), rows);
+    if (reinterpret_cast<uintptr_t>(s.to) & 15u) fail("state must be 16-byte aligned");
+    for (const Tensor* t : {&rows, &a}) require_apart(state, "state", *t, "an input");
+    for (const auto* t : {&d, &dt_bias}) require_apart(state, "state", *t, "an input");
+    size_t need = 0;
+    check(p_scan_workspace((int)rows.size(0), s.sequences.count, (int)heads, (int)groups, (int)head_dim, (int)states, &need),
+          "uniql_state_space_scan_workspace");
+    require_norm(norm_weight, heads * head_dim, norm_groups, eps, rows);
 }

@@ -19,7 +19,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
-from . import ops
+from . import _capi, ops
 
 
 class StateSpaceStates(nn.Module):
@@ -76,14 +76,19 @@ class StateSpaceMixer(nn.Module):
                               ("norm_weight", norm_weight, self.inner)):
             if t is not None and t.numel() != size:
                 raise ValueError(f"{name} must have {size} entries")
+        if not eps >= 0.0:
+            raise ValueError("eps must not be negative")
+        if len(dt_limit) != 2 or not 0.0 <= dt_limit[0] <= dt_limit[1]:
+            raise ValueError("dt_limit must be two numbers from 0 on, the smaller one first")
         self.conv_width, self.norm_groups, self.eps, self.dt_limit = weight.shape[1], norm_groups, eps, tuple(dt_limit)
+        conv_bias, a_log, d, dt_bias, norm_weight = (None if t is None else t.detach().reshape(-1) for t in (conv_bias, a_log, d, dt_bias, norm_weight))
         half = dict(dtype=torch.float16)
         self.register_buffer("weight", weight.to(**half).contiguous())
-        self.register_buffer("bias", None if conv_bias is None else conv_bias.detach().to(**half).contiguous())
-        self.register_buffer("a", -torch.exp(a_log.detach().float()).contiguous())
-        self.register_buffer("d", None if d is None else d.detach().float().contiguous())
-        self.register_buffer("dt_bias", None if dt_bias is None else dt_bias.detach().float().contiguous())
-        self.register_buffer("norm_weight", norm_weight.detach().to(**half).contiguous())
+        self.register_buffer("bias", None if conv_bias is None else conv_bias.to(**half).contiguous())
+        self.register_buffer("a", -torch.exp(a_log.float()).contiguous())
+        self.register_buffer("d", None if d is None else d.float().contiguous())
+        self.register_buffer("dt_bias", None if dt_bias is None else dt_bias.float().contiguous())
+        self.register_buffer("norm_weight", norm_weight.to(**half).contiguous())
 
     def _apply(self, fn, recurse=True):
         # .half() and .to(dtype) leave rates, skips and biases of the time step in 32 bits
@@ -110,13 +115,16 @@ class StateSpaceMixer(nn.Module):
                 places: torch.Tensor | None = None, starts: torch.Tensor | None = None) -> torch.Tensor:
         """projected fp16 [..., inner + channels + heads], in_proj's output (rows may be longer).  cu, places and starts: as for ops.causal_conv;
         without cu every row is one more token of a request, without states every sequence begins and ends in the call.
-        Returns fp16 [..., inner]; rows in no sequence hold nothing of meaning."""
+        Returns fp16 [..., inner]; rows in no sequence hold nothing of meaning.  A refused call leaves all states as they were."""
         width = self.inner + self.channels + self.num_heads
         if projected.shape[-1] < width:
             raise RuntimeError(f"projected has {projected.shape[-1]} columns, z | x | b | c | dt take {width}")
         rows = projected.reshape(-1, projected.shape[-1])
         z, mixed, dt = rows[:, :self.inner], rows[:, self.inner:self.inner + self.channels], rows[:, self.inner + self.channels:width]
         conv, ssm = (None, None) if states is None else (states.conv, states.ssm)
+        if states is not None:
+            _capi.host().check_state_space_layer(rows, self.a, self.d, self.dt_bias, *self.dt_limit, ssm, cu, places, starts, self.norm_weight,
+                                                 self.norm_groups, self.eps, self.num_heads, self.head_dim, self.n_groups, self.state_size)
         mixed = ops.causal_conv(mixed, self.weight, self.bias, state=conv, cu=cu, places=places, starts=starts)
         x, b, c = mixed.split((self.inner, self.n_groups * self.state_size, self.n_groups * self.state_size), dim=1)
         y = ops.state_space_scan(x.unflatten(1, (self.num_heads, self.head_dim)), dt, self.a, b.unflatten(1, (self.n_groups, self.state_size)),
