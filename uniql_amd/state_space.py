@@ -102,11 +102,22 @@ class StateSpaceMixer(nn.Module):
     @classmethod
     def from_block(cls, block, norm_groups=None) -> "StateSpaceMixer":
         """Of a block with the reference's attributes (num_heads, head_dim, n_groups, ssm_state_size, conv1d, A_log, D, dt_bias, norm), whole
-        or cut (slicing.slice_conv1d, slice_norm).  norm_groups: the norm's own when None (group_size or n_groups of it), or one."""
+        or cut (slicing.slice_conv1d, slice_norm).  norm_groups: the norm's own when None (group_size or n_groups of it), or one.  Refused are
+        blocks that compute something else - another activation, the norm in front of the gate - and, without norm_groups, a norm whose
+        group_size gives neither one group nor the block's n_groups, as that of a cut block does which kept the size of before."""
         inner = block.num_heads * block.head_dim
+        for part in (block, block.norm):
+            if getattr(part, "norm_before_gate", False):
+                raise ValueError("the gate comes in front of the norm here, not behind it")
+            activation = getattr(part, "activation", None)
+            if isinstance(activation, str) and activation not in ("silu", "swish"):
+                raise ValueError(f"the activation must be silu, not {activation}")
         if norm_groups is None:
             size = getattr(block.norm, "group_size", None)
-            norm_groups = inner // size if size else getattr(block.norm, "n_groups", 1)
+            norm_groups = inner / size if size else getattr(block.norm, "n_groups", None) or 1
+            if norm_groups not in (1, block.n_groups):
+                raise ValueError(f"the norm's groups ({norm_groups:g} over {inner} channels) are neither one nor the block's {block.n_groups}: give norm_groups")
+            norm_groups = int(norm_groups)
         eps = getattr(block.norm, "variance_epsilon", getattr(block.norm, "eps", 1e-5))
         return cls(block.num_heads, block.head_dim, block.n_groups, block.ssm_state_size, block.conv1d.weight, block.conv1d.bias, block.A_log, block.D,
                    block.dt_bias, block.norm.weight, norm_groups, eps, getattr(block, "time_step_limit", (0.0, float("inf"))))
