@@ -52,3 +52,35 @@ for heads, p, n in ((2, 53, 96), (4, 1, 8), (1, 27, 128), (2, 65, 64), (3, 127, 
     assert all(code == 0 for code, _ in (direct, odd, through, even_through))
     assert odd[1] == through[1] == even_through[1] != direct[1], (p, n)
 """, tmp_path)
+
+
+def test_large_calls_are_several_launches(tmp_path):
+    """what the prototypes allow is not refused for its number of workgroups, and no launch has 2^32 threads"""
+    run(r"""
+def recorded(code, workgroups, several):
+    assert code == 0 and hip.recorder_too_large() == 0
+    assert hip.recorder_workgroups() == workgroups, (hip.recorder_workgroups(), workgroups)
+    assert (hip.recorder_launches() > 1) == several, hip.recorder_launches()
+most = (1 << 24) - 1
+# single tokens: rows of eight of a head a workgroup where states are no fours
+for rows, heads, p, n, blocks in ((8191, 128, 128, 130, 16), (8192, 128, 128, 130, 16), (1 << 24, 1, 1, 1, 1), (40000, 1 << 15, 1, 4, 1), (1 << 24, 5, 100, 128, 2)):
+    code, _ = scan(rows, rows, heads, p, n, heads * p, p, cu=None)
+    recorded(code, rows * heads * blocks, rows * heads * blocks > most)
+def conv(rows, count, channels, cu=fake):
+    s = Sequences(cu, None, None, count, 1 << 30)
+    hip.recorder_reset()
+    return lib.uniql_causal_conv(fake, channels, fake, None, fake, fake, ctypes.addressof(s), fake, channels, rows, channels, 4, 1, None)
+recorded(conv(most, most, 8, None), most, False)
+recorded(conv(1 << 24, 1 << 24, 8, None), 1 << 24, True)
+recorded(conv(1 << 27, 1 << 24, 8), (1 << 24) + (1 << 27) // 32, True)
+recorded(conv(1 << 27, 1 << 24, 4096), 2 * ((1 << 24) + (1 << 27) // 32), True)
+def norm(rows, channels, groups):
+    hip.recorder_reset()
+    return lib.uniql_gated_group_norm(fake, channels, fake, channels, fake, fake, channels, rows, channels, groups, 1e-5, None)
+recorded(norm(1 << 27, 1024, 1), 1 << 25, True)
+recorded(norm(1 << 27, 64, 8), 1 << 28, True)
+recorded(norm(1 << 25, 4096, 1), 1 << 25, True)
+recorded(norm(1 << 24, 4096, 1), 1 << 24, True)
+recorded(norm(most, 4096, 1), most, False)
+recorded(norm(3, 64, 8), 6, False)
+""", tmp_path)

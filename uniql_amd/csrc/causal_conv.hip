@@ -78,9 +78,10 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(const ConvArg
     const int c0 = (blockIdx.y * kConvThreads + threadIdx.x) * 8, left = a.channels - c0;
     Taps<W> taps;
     const bool active = left > 0;
-    if ((int)blockIdx.x >= a.tiles) {
+    const int index = (int)blockIdx.x + a.begin;
+    if (index >= a.tiles) {
         // a sequence's first rows and its state
-        const Sequence q = sequence_of(a.sequences, blockIdx.x - a.tiles);
+        const Sequence q = sequence_of(a.sequences, index - a.tiles);
         if (q.rows == 0 || !active) return;
         h8 x[2 * (W - 1)];  // the state, the first rows
         const int64_t at = ((int64_t)q.place * (W - 1)) * a.channels + c0;
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(kConvThreads) void causal_conv_kernel(const ConvArg
             }
         return;
     }
-    const int row0 = blockIdx.x * a.run, rows = a.sequences.rows - row0 < a.run ? a.sequences.rows - row0 : a.run;
+    const int row0 = index * a.run, rows = a.sequences.rows - row0 < a.run ? a.sequences.rows - row0 : a.run;
     // Rows that have W - 1 others of their sequence in front of them, a bit each: 64 sequences at a time.
     const int lane = threadIdx.x & 63;
     uint32_t allowed = 0;
@@ -165,11 +166,14 @@ int causal_conv_launch(const ConvArgs& args, int width, hipStream_t stream) {
     while (a.run > 8 && a.sequences.rows / a.run * down < 1024) a.run /= 2;
     a.tiles = a.sequences.cu ? (a.sequences.rows + a.run - 1) / a.run : 0;
     const int64_t across = (int64_t)a.tiles + a.sequences.count;
-    if (across * kConvThreads >= (1LL << 32) || down > 65535) return UNIQL_E_SHAPE;
-    const dim3 grid((unsigned)across, (unsigned)down), block(kConvThreads);
-    if (width == 2) hipLaunchKernelGGL(causal_conv_kernel<2>, grid, block, 0, stream, a);
-    else if (width == 3) hipLaunchKernelGGL(causal_conv_kernel<3>, grid, block, 0, stream, a);
-    else hipLaunchKernelGGL(causal_conv_kernel<4>, grid, block, 0, stream, a);
+    if (down > 65535) return UNIQL_E_SHAPE;
+    for (int64_t begin = 0; begin < across; begin += kMostWorkgroups) {
+        a.begin = (int)begin;
+        const dim3 grid((unsigned)(across - begin < kMostWorkgroups ? across - begin : kMostWorkgroups), (unsigned)down), block(kConvThreads);
+        if (width == 2) hipLaunchKernelGGL(causal_conv_kernel<2>, grid, block, 0, stream, a);
+        else if (width == 3) hipLaunchKernelGGL(causal_conv_kernel<3>, grid, block, 0, stream, a);
+        else hipLaunchKernelGGL(causal_conv_kernel<4>, grid, block, 0, stream, a);
+    }
     return hipGetLastError() == hipSuccess ? UNIQL_OK : UNIQL_E_LAUNCH;
 }
 

@@ -14,7 +14,7 @@ __global__ __launch_bounds__(256) void gated_group_norm_kernel(const NormArgs a)
     constexpr int kThreads = 64 * WAVES;
     __shared__ float sums[4];
     const int tid = threadIdx.x % kThreads;
-    const int64_t index = (int64_t)blockIdx.x * (256 / kThreads) + threadIdx.x / kThreads;
+    const int64_t index = (a.begin + blockIdx.x) * (256 / kThreads) + threadIdx.x / kThreads;
     const int64_t all = (int64_t)a.rows * a.groups;
     const bool there = index < all;
     const int64_t row = there ? index / a.groups : 0;
@@ -65,10 +65,12 @@ __global__ __launch_bounds__(256) void gated_group_norm_kernel(const NormArgs a)
 }
 
 template <int WAVES, int PIECES, bool REREAD>
-static int go(const NormArgs& a, hipStream_t stream) {
+static int go(NormArgs a, hipStream_t stream) {
     const int64_t each = 4 / WAVES, blocks = ((int64_t)a.rows * a.groups + each - 1) / each;
-    if (blocks * 256 >= (1LL << 32)) return UNIQL_E_SHAPE;
-    hipLaunchKernelGGL((gated_group_norm_kernel<WAVES, PIECES, REREAD>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    for (a.begin = 0; a.begin < blocks; a.begin += kMostWorkgroups) {
+        const int64_t count = blocks - a.begin < kMostWorkgroups ? blocks - a.begin : kMostWorkgroups;
+        hipLaunchKernelGGL((gated_group_norm_kernel<WAVES, PIECES, REREAD>), dim3((unsigned)count), dim3(256), 0, stream, a);
+    }
     return hipGetLastError() == hipSuccess ? UNIQL_OK : UNIQL_E_LAUNCH;
 }
 

@@ -23,7 +23,7 @@ struct ConvArgs {
     int64_t x_row, out_row;
     Sequences sequences;
     int channels, activation;
-    int run, tiles;  // set by the launch: rows of a run, and the runs
+    int run, tiles, begin;  // set by the launch: rows of a run, and the runs; the launch's first workgroup
 };
 
 struct ScanArgs {
@@ -37,7 +37,7 @@ struct ScanArgs {
     Sequences sequences;
     int heads, share, head_dim, states, softplus;  // share: heads of a group
     // set by the launch
-    int segments, pieces, head_blocks;  // pieces: of a segment, in the first launch
+    int segments, pieces, head_blocks, begin;  // pieces: of a segment, in the first launch; begin: a step's first sequence
     float* temp;
 };
 
@@ -47,7 +47,11 @@ struct NormArgs {
     int64_t x_row, z_row, out_row;
     int rows, groups, width;
     float eps;
+    int64_t begin;  // set by the launch: its first workgroup
 };
+
+// Workgroups of 256 threads that a launch takes (fewer than 2^32 threads); calls of more are several launches.
+constexpr int64_t kMostWorkgroups = (1 << 24) - 1;
 
 // ---- sequences ---------------------------------------------------------------------------------------------------------
 // Whatever the arrays hold, rows and places lie within the call's; sequences without a place have no rows.

@@ -19,7 +19,7 @@ __global__ __launch_bounds__(kStepThreads) void state_space_step_kernel(const Sc
     const unsigned per_sequence = (unsigned)(a.heads * a.head_blocks);
     const unsigned s = blockIdx.x / per_sequence, rest = blockIdx.x % per_sequence;
     const int head = rest / a.head_blocks, block = rest % a.head_blocks;
-    const Sequence q = sequence_of(a.sequences, (int)s);
+    const Sequence q = sequence_of(a.sequences, a.begin + (int)s);
     if (q.rows == 0) return;
     const int lane = threadIdx.x % LANES, p0 = block * kAtOnce * ROWS + threadIdx.x / LANES;
     const int64_t size = (int64_t)a.head_dim * a.states;
@@ -97,9 +97,12 @@ template <int LANES, int EACH, int PARTS, int ROWS>
 static int go(ScanArgs& a, hipStream_t stream) {
     constexpr int rows = kStepThreads / LANES * ROWS;
     a.head_blocks = (a.head_dim + rows - 1) / rows;
-    const int64_t blocks = (int64_t)a.sequences.count * a.heads * a.head_blocks;
-    if (blocks * kStepThreads >= (1LL << 32)) return UNIQL_E_SHAPE;
-    hipLaunchKernelGGL((state_space_step_kernel<LANES, EACH, PARTS, ROWS>), dim3((unsigned)blocks), dim3(kStepThreads), 0, stream, a);
+    const int each = a.heads * a.head_blocks, most = (int)(kMostWorkgroups / each);  // (sequences of a launch)
+    for (int64_t begin = 0; begin < a.sequences.count; begin += most) {
+        a.begin = (int)begin;
+        const int64_t count = a.sequences.count - begin < most ? a.sequences.count - begin : most;
+        hipLaunchKernelGGL((state_space_step_kernel<LANES, EACH, PARTS, ROWS>), dim3((unsigned)(count * each)), dim3(kStepThreads), 0, stream, a);
+    }
     return hipGetLastError() == hipSuccess ? UNIQL_OK : UNIQL_E_LAUNCH;
 }
 
