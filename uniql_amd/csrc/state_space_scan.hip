@@ -14,18 +14,20 @@
 // the state of the sequence that goes on behind it, and the decay over it.  The second launch puts them together where a segment begins
 // within a sequence.
 //
-// Bound by the path from L2 to the compute units (48 KiB a chunk and head, at some 10 bytes a clock and compute unit, where rows of 20480 bytes
-// share few sets of the first cache: rows 256 bytes longer 495 -> 420 us) and by latency within a chunk, some 5000 clocks: 128 heads of 64, 8
-// groups of 128 states, 16384 tokens 390 to 460 us in two launches (the first one 77), 1.6 TB/s and 0.4 PFLOP/s of matrix instructions; 4096
-// tokens of 256 states 200; 333 tokens 18, six chunks of 2.4 us each behind a launch.
-// Tried and taken out: two heads that share b and c in a workgroup of sixteen waves (128 registers each: operands cannot be asked for ahead, 430
-// to 460 us), one set of four waves for everything with two workgroups a compute unit (530), more segments (530).
+// Bound by latency within a chunk.  Of its 5900 clocks (counters of the second launch, 16384 tokens of 128 heads of 64, 8 groups of 128 states) a SIMD
+// has 2400 of vector instructions and 1000 of matrix instructions, LDS 2000 (320 of them bank conflicts); a request to L2 takes 560, and waves
+// wait in 54 % of their cycles, for each other, for LDS and for loads.  397 us in two launches (the first one 78), 1.6 TB/s and 0.4 PFLOP/s of
+// matrix instructions.  Rows of 20480 bytes share few sets of the first cache: 256 bytes longer the call takes 390 us on a card where it takes 443.
+// 4096 tokens of 256 states 207 us (9200 clocks a chunk: 3400, 2000 and 3400); 333 tokens 18.8, six chunks of 2.4 us each behind a launch.
+// Tried and taken out, against 390 us: two heads that share b and c in a workgroup of sixteen waves (128 registers each: operands cannot be asked
+// for ahead, 430 to 460), one set of four waves for everything with two workgroups a compute unit (530), more segments (530).
 //
 // S, all sums and the decays are fp32, L is summed up in 64 bits (its differences matter, also behind a token that wipes the state).
-// Rounded to fp16 are the weights and S for the outputs, which are fp16 themselves, each relative to the largest
-// of its row, so that no finite value overflows or vanishes; what goes into S is split into two fp16 numbers, 22 bits.  An infinity or
-// NaN in x must not reach rows in front of it, also as zero times it: where a result shows one, such values are taken out of the product
-// and added on their own.
+// Rounded to fp16 are the weights and S for the outputs, which are fp16 themselves (distance from 64 bits 2.2e-4 to 2.5e-4 of the outputs, 2.1e-4
+// where only they are rounded; two fp16 numbers for each would double the second and third products and their reads).  Both are relative to the
+// largest of their row: none overflows, and what is below 2^-28 of that one loses digits, below 2^-39 itself, which shows only where x or c is zero
+// at the largest.  What goes into S is split into two fp16 numbers, 22 bits.  An infinity or NaN in x must not reach rows in front of it, also as
+// zero times it: where a result shows one, such values are taken out of the product and added on their own.
 #include <type_traits>
 
 #include "state_space.hpp"
@@ -857,8 +859,8 @@ __global__ __launch_bounds__(64 * scan_waves(N32, THROUGH, LAST), !LAST && N32 <
     }
 }
 
-// One workgroup a compute unit in the second launch, three in the first: as much as their LDS allows.  (16384 tokens of 128 heads: 2 segments
-// 460 us, 4 of them, whose second launch holds half of its workgroups back, 530; 6 pieces in the first launch 77, 4 as much.)
+// One workgroup a compute unit in the second launch, three in the first: as much as their LDS allows.  (16384 tokens of 128 heads when 2 segments took
+// 460 us: 4 of them, whose second launch holds half of its workgroups back, 530; 6 pieces in the first launch 77, 4 as much.)
 constexpr int kWorkgroups = 256, kFirstWorkgroups = 768;
 
 // How a call is shared out: segments, and pieces of a segment in the first launch.
